@@ -13,7 +13,7 @@
  *   - shapes are rank-4, left-padded with 1s, exactly what Shape::promote(_, 4) produces (shape.rs:92-96).
  *   - dtype codes: F32 = 0, F16 = 1 as DType::to_u32 (dtype/mod.rs:32-38); BF16 = 2, I32 = 3, U32 = 4 added.
  *   - the caller owns every device pointer; the library allocates nothing inside launch functions except scratch
- *     owned by rt_device (GroupNorm partial statistics, the f16 lookup tables).
+ *     owned by rt_device (GroupNorm partial statistics, attention's partial results, the f16 lookup tables).
  *   - calls on one rt_device must be serialised by the caller (the reference keeps its device behind a RwLock,
  *     gpu/device.rs:20-29).  rt_last_error() is thread-local.
  *   - results follow ratchet's CPU executor (the cpu/ directory), including its f16 rounding points.
@@ -215,7 +215,8 @@ int rt_softmax_masked(rt_device* dev, int dt, const void* x, const uint32_t x_sh
  * While capturing, calls that wait for the device or go to the driver for memory return RT_ERR_CAPTURE: rt_sync,
  * rt_h2d, rt_d2h, rt_pool_trim, event calls, an rt_malloc the pool cannot serve, and the first use of an op that builds
  * a lookup table or grows scratch (run the sequence once eagerly first).  A graph holds raw pointers: every buffer it
- * touches must stay allocated while the graph is in use. */
+ * touches must stay allocated while the graph is in use.  One that holds an attention or eviction call uses the recording
+ * device's scratch: rt_graph_launch takes it on that rt_device only, and it is not launched after that device is destroyed. */
 typedef struct rt_graph rt_graph;
 int rt_capture_begin(rt_device* dev);
 int rt_capture_end(rt_device* dev, rt_graph** out);
@@ -247,6 +248,64 @@ int rt_unary_via_f32(rt_device* dev, int op, int io_dt, const void* x, void* y, 
  * so the two slices of the fused projection need no copies: crates/ratchet-models/src/phi3/mlp.rs:32-38. */
 int rt_gated_mul_via_f32(rt_device* dev, int op, int io_dt, const void* gate, uint64_t gate_row_stride, const void* up,
                          uint64_t up_row_stride, void* y, uint64_t rows, uint32_t cols);
+
+/* ---- Attention and the paged KV cache -------------------------------------------------------------------------------
+ * What the models build from a product, scale, mask, softmax and a second product (phi2/attn.rs:113-153,
+ * phi3/attn.rs:143-153, whisper/mha.rs:115-124) without the scores ever reaching memory; the reference has no such op and no paged
+ * cache.  Query head h reads KV head h / (heads / kv_heads).  Scores, softmax statistics and the sums over the keys are
+ * f32; the result is rounded once to the element type (F32, F16, BF16).  With p the position of a query and len the
+ * keys there are, key t is visible iff t < len and, where causal, 0 <= t <= p and (window == 0 or p - t < window or t < sinks):
+ * a sliding window, and `sinks` first keys that stay in sight.  A query that sees no key yields 0 and an lse of -inf;
+ * what hidden keys and values hold, infinities and NaN included, does not matter.  y and lse overlap no input. */
+
+/* q [B, heads, Sq, D], k and v [B, kv_heads, Sk, D], y as q; strides in elements (NULL: contiguous), the last one 1 where D > 1,
+ * so that q, k and v may be windows of one projection and y [B, Sq, heads, D] in memory; elements of y do not overlap.  lens (NULL: Sk for all): i32 [B] on
+ * the device, the keys of each batch entry, taken into [0, Sk].  The last query sits at position len - 1 (p = len - Sq + i).
+ * lse (NULL: not wanted): f32 [B, heads, Sq], log of the sum of exp(scale * q.k) over the visible keys.  window and sinks need causal.
+ * D at most 512. */
+int rt_attention(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4], const uint64_t q_strides[4], const void* k,
+                 const uint64_t k_strides[4], const void* v, const uint64_t v_strides[4], const uint32_t kv_shape[4], const int32_t* lens,
+                 void* y, const uint64_t y_strides[4], float* lse, float scale, int causal, uint32_t window, uint32_t sinks);
+
+/* A KV cache in pages.  k and v: [pages, kv_heads, page_len, head_dim], contiguous.  table: i32 [seqs, table_len], the pages
+ * of each sequence in order; token t of sequence b is row t % page_len of page table[b][t / page_len].  An entry outside [0, pages)
+ * is a page that is not there: its tokens are not written, are visible to no query and are evicted as zero rows.  lens: i32
+ * [seqs], the tokens of each sequence, negative ones taken as 0; tokens beyond table_len * page_len are not there.
+ * table and lens live on the device and are read when the work runs, so a recorded graph replays on what they then hold. */
+typedef struct rt_paged_kv {
+    void* k;
+    void* v;
+    const int32_t* table;
+    const int32_t* lens;
+    uint32_t pages, kv_heads, page_len, head_dim, seqs, table_len;
+} rt_paged_kv;
+
+/* The new tokens of a call: rows starts[b] .. starts[b + 1] - 1 of `tokens` rows belong to sequence b (starts: i32 [seqs + 1] on the
+ * device, not decreasing, taken into [0, tokens]); they are the last ones that lens counts, at positions lens[b] - count .. lens[b] - 1.
+ * Rows before starts[0] and from starts[seqs] on belong to no sequence: nothing is read or written for them. */
+
+/* Append: rows of k and v [tokens, kv_heads, head_dim] into their pages.  strides: elements from token to token and from head to
+ * head (NULL: contiguous).  elem_bytes 2 or 4. */
+int rt_paged_append(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const int32_t* starts, uint32_t tokens, const void* k,
+                    const uint64_t k_strides[2], const void* v, const uint64_t v_strides[2]);
+
+/* Causal attention of the new tokens over the cache: single tokens and chunks of any length in one call.  q [tokens, heads, D],
+ * strides as above; y [tokens, heads, D] contiguous; lse (NULL: not wanted) f32 [tokens, heads].  weights_out (NULL: not wanted) f32
+ * [seqs, kv_heads, table_len * page_len]: for every token t < lens[b] the attention weight it has received,
+ * (t is new ? 0 : weights[b, g, t]) + the sum of its softmax weights over the call's queries of the heads that share KV head g,
+ * added up in a fixed order; entries beyond are left as they were.  weights and weights_out may be the same array. */
+int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_strides[2], uint32_t tokens, uint32_t heads,
+                       const rt_paged_kv* kv, const int32_t* starts, void* y, float* lse, const float* weights, float* weights_out, float scale,
+                       uint32_t window, uint32_t sinks);
+
+/* Eviction by accumulated weight: of a sequence with more than `keep` tokens the first `first`, the last `recent` and, for
+ * each KV head on its own, the keep - first - recent others with the largest weights stay (equal weights: the lower
+ * token; NaN ranks lowest), in their order, as tokens 0 .. keep - 1; shorter sequences stay whole.  The rows go into the pages of
+ * table_out [seqs, table_len], their weights into weights_out, min(len, keep) into lens_out.  Each of the three may be its
+ * input, the same pointer (the cache is then compacted in place); otherwise it overlaps no input, and the pages that table_out
+ * names are none of table's, none of them named twice.  Rows whose page in table_out is not there are dropped; other rows of the pages stay as they were. */
+int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const float* weights, uint32_t keep, uint32_t first, uint32_t recent,
+                   const int32_t* table_out, int32_t* lens_out, float* weights_out);
 
 #ifdef __cplusplus
 }

@@ -28,7 +28,14 @@ EXPORTS = [
     "rt_free", "rt_pool_trim", "rt_pool_begin_pass", "rt_pool_stats", "rt_pool_peak", "rt_capture_begin", "rt_capture_end", "rt_graph_launch", "rt_graph_destroy", "rt_memset0", "rt_h2d", "rt_d2h", "rt_d2d", "rt_event_create", "rt_event_destroy", "rt_event_record",
     "rt_event_elapsed_ms", "rt_binary", "rt_binary_bcast", "rt_unary", "rt_cast", "rt_permute", "rt_slice", "rt_broadcast",
     "rt_concat", "rt_cache", "rt_index_select", "rt_index_select_q8_0", "rt_index_write", "rt_rope", "rt_softmax", "rt_softmax_masked", "rt_layer_norm", "rt_rms_norm", "rt_group_norm", "rt_group_norm_static", "rt_norm_via_f32", "rt_softmax_via_f32", "rt_unary_via_f32", "rt_gated_mul_via_f32",
+    "rt_attention", "rt_paged_append", "rt_paged_attention", "rt_paged_evict",
 ]
+
+
+class PagedKV(ctypes.Structure):
+    """rt_paged_kv"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "table", "lens")] + [
+        (n, ctypes.c_uint32) for n in ("pages", "kv_heads", "page_len", "head_dim", "seqs", "table_len")]
 
 
 class RatchetError(RuntimeError):
@@ -101,6 +108,11 @@ def load():
     L.rt_softmax_via_f32.argtypes = [vp, i, vp, sh, vp, sh, vp, i]
     L.rt_unary_via_f32.argtypes = [vp, i, i, vp, vp, u64]
     L.rt_gated_mul_via_f32.argtypes = [vp, i, i, vp, u64, vp, u64, vp, u64, u32]
+    st, kv = ctypes.POINTER(u64), ctypes.POINTER(PagedKV)
+    L.rt_attention.argtypes = [vp, i, vp, sh, st, vp, st, vp, st, sh, vp, vp, st, vp, f, i, u32, u32]
+    L.rt_paged_append.argtypes = [vp, i, kv, vp, u32, vp, st, vp, st]
+    L.rt_paged_attention.argtypes = [vp, i, vp, st, u32, u32, kv, vp, vp, vp, vp, vp, f, u32, u32]
+    L.rt_paged_evict.argtypes = [vp, i, kv, vp, u32, u32, u32, vp, vp, vp]
     for name in EXPORTS:
         fn = getattr(L, name)
         if name not in ("rt_last_error", "rt_status_name"):
@@ -127,3 +139,9 @@ def buffer_shape4(shape):
     """shape4 of a buffer's own shape or of another tuple of ints.  The array is shared by all calls of a shape and belongs to nobody: the
     library only reads it (0.1 us a call, 0.7 when it is built each time; a decode step makes eight)."""
     return shape4(shape)
+
+
+@functools.lru_cache(maxsize=4096)
+def strides_array(strides):
+    """a tuple of element strides as the library takes it; shared like buffer_shape4's"""
+    return (ctypes.c_uint64 * len(strides))(*strides)

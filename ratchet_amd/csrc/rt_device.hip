@@ -3,6 +3,7 @@
 // storage/gpu_buffer.rs in crates/ratchet-core/src).
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <map>
 #include <mutex>
@@ -14,6 +15,12 @@ struct rt_graph {
     hipGraph_t graph;
     hipGraphExec_t exec;
     int ordinal;
+    rt_device* scratch_owner;      // the device whose workspace the recorded calls use, NULL if they use none
+};
+
+struct rt_retired {
+    void* ptr;
+    rt_retired* next;
 };
 
 struct rt_parked {
@@ -52,6 +59,40 @@ int rt_enter(rt_device* dev) {
     if (!dev) return rt_fail(RT_ERR_NULL_DEVICE, "rt_device is NULL");
     hipError_t e = hipSetDevice(dev->ordinal);
     if (e != hipSuccess) return rt_fail_hip(e, "hipSetDevice");
+    return RT_OK;
+}
+
+// A recorded graph keeps the address of the block it was recorded with, so a block that one has seen stays where it is until the
+// device goes, also when a larger one takes its place.
+int rt_scratch(rt_device* dev, size_t bytes, void** out) {
+    if (bytes > dev->scratch_bytes) {
+        RT_NO_CAPTURE(dev, "growing the attention workspace");
+        const size_t size = (bytes + bytes / 4 + ((1u << 20) - 1)) >> 20 << 20;
+        rt_retired* keep = nullptr;
+        if (dev->scratch && dev->scratch_recorded) {
+            keep = (rt_retired*)malloc(sizeof(rt_retired));
+            RT_REQUIRE(keep, RT_ERR_SIZE, "growing the attention workspace: out of host memory");
+        }
+        void* fresh = nullptr;
+        hipError_t e = hipMalloc(&fresh, size);
+        if (e != hipSuccess) {
+            free(keep);
+            return rt_fail_hip(e, "hipMalloc(attention workspace)");
+        }
+        if (keep) {
+            keep->ptr = dev->scratch;
+            keep->next = dev->retired;
+            dev->retired = keep;
+        } else if (dev->scratch) {
+            (void)hipStreamSynchronize(dev->stream);             // queued work may still use it
+            (void)hipFree(dev->scratch);
+        }
+        dev->scratch = fresh;
+        dev->scratch_bytes = size;
+        dev->scratch_recorded = 0;
+    }
+    if (dev->capturing) dev->scratch_recorded = dev->capture_used_scratch = 1;
+    *out = dev->scratch;
     return RT_OK;
 }
 
@@ -205,6 +246,13 @@ int rt_device_destroy(rt_device* dev) {
         }
     if (dev->gn_scratch) (void)hipFree(dev->gn_scratch);
     if (dev->sm_mask_tiles) (void)hipFree(dev->sm_mask_tiles);
+    if (dev->scratch) (void)hipFree(dev->scratch);
+    while (dev->retired) {
+        rt_retired* next = dev->retired->next;
+        (void)hipFree(dev->retired->ptr);
+        free(dev->retired);
+        dev->retired = next;
+    }
     // buffers the caller never returned are released with the device, like the parked ones
     for (auto& kv : dev->pool->parked) (void)hipFree(kv.second.ptr);
     for (auto& kv : dev->pool->live) (void)hipFree(kv.first);
@@ -446,6 +494,7 @@ int rt_capture_begin(rt_device* dev) {
     // thread-local mode: only this thread's calls on this stream are checked, other threads and devices carry on
     RT_HIP(hipStreamBeginCapture(dev->stream, hipStreamCaptureModeThreadLocal));
     dev->capturing = 1;
+    dev->capture_used_scratch = 0;
     return RT_OK;
 }
 
@@ -469,6 +518,7 @@ int rt_capture_end(rt_device* dev, rt_graph** out) {
     g->graph = graph;
     g->exec = exec;
     g->ordinal = dev->ordinal;
+    g->scratch_owner = dev->capture_used_scratch ? dev : nullptr;
     *out = g;
     return RT_OK;
 }
@@ -479,6 +529,8 @@ int rt_graph_launch(rt_device* dev, rt_graph* graph) {
     if (rc) return rc;
     RT_NO_CAPTURE(dev, "rt_graph_launch");
     RT_REQUIRE(graph->ordinal == dev->ordinal, RT_ERR_ARG, "rt_graph_launch: the graph was captured on device %d", graph->ordinal);
+    RT_REQUIRE(!graph->scratch_owner || graph->scratch_owner == dev, RT_ERR_ARG,
+               "rt_graph_launch: the graph uses the workspace of the rt_device that recorded it");
     RT_HIP(hipGraphLaunch(graph->exec, dev->stream));
     return RT_OK;
 }

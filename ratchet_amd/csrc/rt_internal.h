@@ -50,6 +50,12 @@ struct rt_device {
     // caching allocator behind rt_malloc / rt_free (defined in rt_device.hip)
     struct rt_pool* pool;
     int capturing;          // between rt_capture_begin and rt_capture_end
+    // workspace of the attention and eviction calls (rt_scratch): every call writes what it reads of it, and the device's stream orders the calls
+    void* scratch;
+    size_t scratch_bytes;
+    int scratch_recorded;          // a recorded graph uses this block: it is not freed before the device
+    int capture_used_scratch;      // the capture that is running has asked for it
+    struct rt_retired* retired;    // outgrown blocks that graphs still use
 };
 
 struct rt_event {
@@ -110,6 +116,13 @@ static const uint64_t RT_MAX_NUMEL = 1ull << 40;
 
 // Makes dev's ordinal current.  Every entry point calls it first.
 int rt_enter(rt_device* dev);
+
+// At least `bytes` of the device's workspace, 256-byte aligned; grown outside of a capture only (RT_ERR_CAPTURE otherwise).
+int rt_scratch(rt_device* dev, size_t bytes, void** out);
+
+// rt_attention.hip: what every call on a paged cache asks of it, and of rows [tokens, heads, dim] with strides (NULL: contiguous)
+int rt_paged_rules(const char* who, const rt_paged_kv* kv, size_t elem_bytes);
+int rt_rows_rules(const char* who, const char* what, uint32_t tokens, uint32_t heads, uint32_t dim, const uint64_t strides[2], uint64_t* token, uint64_t* head);
 
 // rt_norm.hip: resolves the device-side address of the fixed GroupNorm scratch array for the current device
 int rt_norm_device_init(rt_device* dev);

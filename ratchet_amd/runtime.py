@@ -11,7 +11,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from ._lib import RatchetError, buffer_shape4, check, shape4  # noqa: F401
+from ._lib import RatchetError, buffer_shape4, check, shape4, strides_array  # noqa: F401
 
 _NP_TO_DT = {np.dtype(np.float32): _lib.F32, np.dtype(np.float16): _lib.F16, np.dtype(np.int32): _lib.I32,
              np.dtype(np.uint32): _lib.U32}
@@ -155,6 +155,44 @@ class Event:
                 self.ptr = None
         except Exception:
             pass
+
+
+class PagedCache:
+    """A KV cache in pages: k_pages and v_pages [pages, kv_heads, page_len, head_dim], table I32 [seqs, table_len] (the pages of each
+    sequence in order, -1 where there is none) and lens I32 [seqs] (its tokens); the buffers stay the caller's to fill and update."""
+
+    def __init__(self, k_pages, v_pages, table, lens):
+        if len(k_pages.shape) != 4 or k_pages.shape != v_pages.shape or k_pages.dt != v_pages.dt:
+            raise ValueError(f"k_pages {k_pages.shape} and v_pages {v_pages.shape} are not two alike [pages, kv_heads, page_len, head_dim]")
+        if len(table.shape) != 2 or table.dt != _lib.I32 or lens.dt != _lib.I32 or lens.shape != (table.shape[0],):
+            raise ValueError("table and lens have to be I32 [seqs, table_len] and [seqs]")
+        self.k_pages, self.v_pages, self.table, self.lens, self.dt = k_pages, v_pages, table, lens, k_pages.dt
+        self.pages, self.kv_heads, self.page_len, self.head_dim = k_pages.shape
+        self.seqs, self.table_len = table.shape
+        self.handle = _lib.PagedKV(k_pages.ptr.value, v_pages.ptr.value, table.ptr.value, lens.ptr.value, *k_pages.shape, *table.shape)
+        self.ref = ctypes.byref(self.handle)
+
+    @property
+    def weights_shape(self):
+        return (self.seqs, self.kv_heads, self.table_len * self.page_len)
+
+
+def _require(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _strided(x, strides):
+    """what the library takes for `strides` (elements, one for each extent of x but the last where x is a row list), checked against the memory behind x"""
+    if strides is None:
+        return None
+    strides = tuple(map(int, strides))
+    parent = getattr(x, "parent", x)
+    at = (x.ptr.value - parent.ptr.value) // _DT_BYTES[x.dt]
+    _require(min(strides) >= 0, f"negative stride in {strides}")
+    last = at + sum((n - 1) * s for n, s in zip(x.shape, strides)) + (x.shape[-1] - 1 if len(strides) < len(x.shape) else 0)
+    _require(last < parent.numel, f"{x.shape} with strides {strides} reaches beyond its buffer")
+    return strides_array(strides)
 
 
 class Device:
@@ -379,3 +417,56 @@ class Device:
         check(fn(self.handle, x.dt, x.ptr, scale.ptr if scale is not None else None,
                  bias.ptr if bias is not None else None, out.ptr, B, C, L, groups, eps))
         return out
+
+    # ---- attention, the paged KV cache
+    def attention(self, q, k, v, lens=None, causal=True, window=0, sinks=0, scale=None, q_strides=None, k_strides=None, v_strides=None, out=None, out_strides=None,
+                  lse=None):
+        """softmax(scale q k^T over the visible keys) v: q [B, heads, Sq, D], k and v [B, kv_heads, Sk, D]; the strides (elements, one for each extent) say
+        where they lie in memory, out's too.  lens: I32 [B], the keys of each entry; the last query is at the last key.  window: a query
+        sees that many last keys and the first `sinks`; scale: 1 / sqrt(D) unless given; lse: F32 [B, heads, Sq] for the log of each row's sum."""
+        _require(len(q.shape) == 4 and len(k.shape) == 4 and k.shape == v.shape and q.dt == k.dt == v.dt, f"attention of {q.shape}, {k.shape}, {v.shape}")
+        _require(lens is None or (lens.dt == _lib.I32 and lens.shape == (q.shape[0],)), "lens has to be I32 [B]")
+        out = out or Buffer(self, q.shape, q.dt)
+        _require(out.dt == q.dt and out.numel == q.numel and (lse is None or (lse.dt == _lib.F32 and lse.numel * q.shape[3] == q.numel)), "out or lse does not fit")
+        _require(out_strides is None or out.shape == q.shape, "out with strides has the shape of q")
+        check(self.lib.rt_attention(self.handle, q.dt, q.ptr, buffer_shape4(q.shape), _strided(q, q_strides), k.ptr, _strided(k, k_strides), v.ptr, _strided(v, v_strides),
+                                    buffer_shape4(k.shape), lens.ptr if lens is not None else None, out.ptr, _strided(out, out_strides), lse.ptr if lse is not None else None,
+                                    q.shape[3] ** -0.5 if scale is None else scale, 1 if causal else 0, window, sinks))
+        return out
+
+    def paged_cache(self, k_pages, v_pages, table, lens):
+        return PagedCache(k_pages, v_pages, table, lens)
+
+    def paged_append(self, cache, starts, k, v, k_strides=None, v_strides=None):
+        """Rows of k and v [tokens, kv_heads, head_dim] into the cache: rows starts[b] .. starts[b + 1] - 1 are the last tokens that cache.lens counts
+        of sequence b.  starts: I32 [seqs + 1]; strides: elements from token to token and from head to head."""
+        _require(k.shape == v.shape and k.shape[1:] == (cache.kv_heads, cache.head_dim) and k.dt == v.dt == cache.dt, f"{k.shape} and {v.shape} do not fit the cache")
+        _require(starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,), "starts has to be I32 [seqs + 1]")
+        check(self.lib.rt_paged_append(self.handle, _DT_BYTES[cache.dt], cache.ref, starts.ptr, k.shape[0], k.ptr, _strided(k, k_strides), v.ptr, _strided(v, v_strides)))
+        return cache
+
+    def paged_attention(self, q, cache, starts, window=0, sinks=0, scale=None, q_strides=None, out=None, lse=None, weights=None, weights_out=None):
+        """Causal attention of the new tokens q [tokens, heads, head_dim] (starts as in paged_append, whose rows are in the cache already).
+        weights: F32 cache.weights_shape, the attention weight each cached token has received, updated in place or into weights_out."""
+        _require(len(q.shape) == 3 and q.shape[2] == cache.head_dim and q.dt == cache.dt, f"{q.shape} does not fit the cache")
+        _require(starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,), "starts has to be I32 [seqs + 1]")
+        out = out or Buffer(self, q.shape, q.dt)
+        _require(out.dt == q.dt and out.numel == q.numel and (lse is None or (lse.dt == _lib.F32 and lse.numel * q.shape[2] == q.numel)), "out or lse does not fit")
+        _require(weights is not None or weights_out is None, "weights_out without weights")
+        if weights is not None:
+            weights_out = weights if weights_out is None else weights_out
+            _require(weights.dt == weights_out.dt == _lib.F32 and weights.shape == weights_out.shape == cache.weights_shape, f"weights have to be F32 {cache.weights_shape}")
+        check(self.lib.rt_paged_attention(self.handle, q.dt, q.ptr, _strided(q, q_strides), q.shape[0], q.shape[1], cache.ref, starts.ptr, out.ptr,
+                                          lse.ptr if lse is not None else None, weights.ptr if weights is not None else None,
+                                          weights_out.ptr if weights is not None else None, q.shape[2] ** -0.5 if scale is None else scale, window, sinks))
+        return out
+
+    def paged_evict(self, cache, weights, keep, first=0, recent=0, to=None, lens_out=None, weights_out=None):
+        """Cuts every sequence of more than `keep` tokens to its first `first`, its last `recent` and the others with the largest weights, each KV head
+        on its own, in their order: in place, or into the pages of the table `to` (none of them in use by the cache), lens_out and weights_out.
+        Returns the cache with what it then holds."""
+        to, lens_out, weights_out = to or cache.table, lens_out or cache.lens, weights_out or weights
+        _require(to.dt == lens_out.dt == _lib.I32 and to.shape == cache.table.shape and lens_out.shape == cache.lens.shape, "to or lens_out does not fit the cache")
+        _require(weights.dt == weights_out.dt == _lib.F32 and weights.shape == weights_out.shape == cache.weights_shape, f"weights have to be F32 {cache.weights_shape}")
+        check(self.lib.rt_paged_evict(self.handle, _DT_BYTES[cache.dt], cache.ref, weights.ptr, keep, first, recent, to.ptr, lens_out.ptr, weights_out.ptr))
+        return cache if to is cache.table and lens_out is cache.lens else PagedCache(cache.k_pages, cache.v_pages, to, lens_out)
