@@ -35,9 +35,26 @@ struct AttnArgs {
     FastDiv group_div;             // by group
     float c;                       // scale * log2(e)
     int32_t causal, window, sinks;
+    size_t own_lse;                // bytes of lse that the call itself needs and keeps at the front of the workspace
 };
 
-// rt_attention_rows.hip etc. return RT_OK with *done = false where the problem is not theirs
+// The device's workspace with room for lse, if it is the call's own (a.lse is then set), and `bytes` behind it
+static inline int at_workspace(rt_device* dev, AttnArgs& a, size_t bytes, void** rest) {
+    const size_t front = (a.own_lse + 255) / 256 * 256;
+    if (front + bytes == 0) return RT_OK;
+    void* p;
+    int rc = rt_scratch(dev, front + bytes, &p);
+    if (rc) return rc;
+    if (front) a.lse = (float*)p;
+    *rest = (unsigned char*)p + front;
+    return RT_OK;
+}
+
+// The matrix-unit kernels (rt_attention_tile.h), a source to each element type.  RT_OK with *done = false where the operands are not laid out for them
+int rt_attention_tile_f32(rt_device* dev, AttnArgs& a, bool paged, bool* done);
+int rt_attention_tile_f16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
+int rt_attention_tile_bf16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
+
 #ifdef __HIPCC__
 
 // One sequence's part of a call

@@ -137,7 +137,12 @@ template <typename T> int launch_weights_any(rt_device* dev, const AttnArgs& a, 
     return RT_OK;
 }
 
-int dispatch(rt_device* dev, int dt, const AttnArgs& a, bool paged) {
+int dispatch(rt_device* dev, int dt, AttnArgs& a, bool paged) {
+    bool done;
+    int rc = dt == RT_F32 ? rt_attention_tile_f32(dev, a, paged, &done) : dt == RT_F16 ? rt_attention_tile_f16(dev, a, paged, &done) : rt_attention_tile_bf16(dev, a, paged, &done);
+    if (rc || done) return rc;
+    void* none = nullptr;
+    if ((rc = at_workspace(dev, a, 0, &none))) return rc;
     switch (dt) {
         case RT_F32: return launch_any<float>(dev, a, paged);
         case RT_F16: return launch_any<half_t>(dev, a, paged);
@@ -295,11 +300,7 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
     a.table_len = kv->table_len;
     a.page_div = make_fastdiv(kv->page_len);
     a.causal = 1;
-    if (weights_out && !lse) {
-        void* p;
-        if ((rc = rt_scratch(dev, (size_t)tokens * heads * sizeof(float), &p))) return rc;
-        a.lse = (float*)p;
-    }
+    a.own_lse = weights_out && !lse ? (size_t)tokens * heads * sizeof(float) : 0;
     if ((rc = dispatch(dev, dt, a, true))) return rc;
     if (!weights_out) return RT_OK;
     switch (dt) {

@@ -1,0 +1,707 @@
+// Attention on the matrix units: 128 query rows to a block, 32 to a wave, the keys in tiles through LDS.
+//
+// A row is a (token, head of the group) pair, so the heads that share a KV head share its tiles.  Everything is computed transposed, with the queries
+// along the columns of the 32 x 32 products:
+//     S^T = K Q^T      K from LDS (16-byte chunks of a key's row), Q in registers for the whole walk
+//     O^T += V^T P^T   V^T read transposed from LDS, P^T the registers that S^T was computed into
+// In the products' layout lane l holds column l % 32 and, of every 8 rows, the 4 at 4 * (l / 32): a query's scores lie in two lanes, so
+// its maximum and sum are a walk over registers and one exchange.  The operand layout of P^T (8 keys a lane and step) is that of the S^T registers
+// if the 16 keys of a step are taken in the order {4h..4h+3, 8+4h..8+4h+3}, h = l / 32, and any order will do as long as V^T is read in the same one.
+//
+// What hidden keys hold is kept out of the scores by a select and out of the maxima and sums by that; their values meet a weight of 0, and 0 times
+// what is not finite is NaN, which stays.  So a row tile whose result is not finite is computed again, one row at a time, over the visible keys only.
+#ifndef RT_ATTENTION_TILE_H
+#define RT_ATTENTION_TILE_H
+
+#include "rt_attention.h"
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t AT_ROWS = 128, AT_WAVES = 4, AT_BLOCK = 64 * AT_WAVES;
+constexpr uint32_t AT_TARGET = 1024;             // work items that fill the chip: two blocks on each of 256 CUs, twice
+constexpr uint32_t AT_LEAST_TILES = 4;           // tiles that a piece of the keys is worth
+
+// ------------------------------------------------------------------------------------------------- who does what
+// Tiles of KT keys that a tile of rows of sequence s may see at most; 1 where there are no keys, for the block that writes the zeros
+template <int KT> __device__ __forceinline__ uint32_t at_span(const AttnArgs& a, const AttnSeq& s) {
+    uint32_t n = ((uint32_t)s.keys + KT - 1) / KT;
+    if (a.window != AT_FAR) {
+        const uint64_t w = ((uint64_t)a.window + AT_ROWS) / KT + 2 + ((uint64_t)a.sinks + KT - 1) / KT;
+        n = w < n ? (uint32_t)w : n;
+    }
+    return n ? n : 1;
+}
+__device__ __forceinline__ uint32_t at_row_tiles(const AttnArgs& a, const AttnSeq& s) { return (s.count * a.group + AT_ROWS - 1) / AT_ROWS; }
+
+template <typename T> __device__ __forceinline__ T at_wave_sum(T x) {
+#pragma unroll
+    for (int i = 32; i; i >>= 1) x += __shfl_xor(x, i);
+    return x;
+}
+
+// Tiles in a piece of the keys: as many as give AT_TARGET work items in all, and no fewer than AT_LEAST_TILES.  The same in every wave.
+template <int KT> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a) {
+    uint64_t work = 0;
+    for (uint32_t b = __lane_id(); b < a.seqs; b += 64) {
+        const AttnSeq s = at_seq<true>(a, b);
+        work += (uint64_t)at_row_tiles(a, s) * at_span<KT>(a, s);
+    }
+    work = at_wave_sum(work) * a.kv_heads;
+    const uint64_t n = (work + AT_TARGET - 1) / AT_TARGET;
+    return n < AT_LEAST_TILES ? AT_LEAST_TILES : n > 0x7fffffffu ? 0x7fffffffu : (uint32_t)n;
+}
+
+// Sequence b's items are numbered row tile by row tile, at_items of them, after those of the sequences before it.
+template <int KT> __device__ __forceinline__ uint32_t at_items(const AttnArgs& a, uint32_t b, uint32_t piece) {
+    const AttnSeq s = at_seq<true>(a, b);
+    return at_row_tiles(a, s) * ((at_span<KT>(a, s) + piece - 1) / piece);
+}
+// The sequence that item `at` belongs to (a.seqs: none); `at` becomes its number there.  All lanes of a wave take part.
+template <int KT> __device__ __forceinline__ uint32_t at_locate(const AttnArgs& a, uint32_t piece, uint32_t& at) {
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < a.seqs; b0 += 64) {
+        const uint32_t b = b0 + __lane_id(), n = b < a.seqs ? at_items<KT>(a, b, piece) : 0;
+        uint32_t sum = n;                                       // of this lane and those below
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) {
+            const uint32_t x = __shfl_up(sum, i);
+            if ((int)__lane_id() >= i) sum += x;
+        }
+        const uint64_t holds = __ballot(at >= before + sum - n && at < before + sum);
+        if (holds) {
+            const int lane = __builtin_ctzll(holds);
+            at -= before + __shfl(sum, lane) - __shfl(n, lane);
+            return b0 + lane;
+        }
+        before += __shfl(sum, 63);
+    }
+    return a.seqs;
+}
+template <int KT> __device__ __forceinline__ uint32_t at_before(const AttnArgs& a, uint32_t piece, uint32_t until) {
+    uint32_t sum = 0;
+    for (uint32_t b = __lane_id(); b < until; b += 64) sum += at_items<KT>(a, b, piece);
+    return at_wave_sum(sum);
+}
+
+// A row tile's walk over the keys: `tiles` of them, the first `head` from key 0 on, the others from key `from` on
+struct AttnWalk {
+    uint32_t tiles, head;
+    int32_t from;
+};
+template <int KT> __device__ __forceinline__ AttnWalk at_walk(const AttnArgs& a, const AttnSeq& s, uint32_t row0, uint32_t rows) {
+    const uint32_t j0 = fd_div(row0, a.group_div), j1 = fd_div(row0 + rows - 1, a.group_div);
+    const int32_t last = at_limit(a, s, j1);
+    AttnWalk w = {0, 0, 0};
+    if (last < 0) return w;
+    if (a.window != AT_FAR) {
+        const int32_t first = at_position(s, j0) - a.window + 1;                // the first key of the first row's window
+        const int32_t from = first > 0 ? first / KT * KT : 0;
+        const uint32_t head = ((uint32_t)(a.sinks < from ? a.sinks : from) + KT - 1) / KT;
+        if ((int32_t)(head * KT) < from) {
+            w.head = head;
+            w.from = from;
+            if (from > last) {                                  // rows beyond the last key there is room for: only the sinks are left
+                w.tiles = head < (uint32_t)last / KT + 1 ? head : (uint32_t)last / KT + 1;
+                return w;
+            }
+        }
+    }
+    w.tiles = w.head + (uint32_t)(last - w.from) / KT + 1;
+    return w;
+}
+
+// ----------------------------------------------------------------------------------------------------- elements
+template <typename T> struct AtMma;
+template <> struct AtMma<half_t> {
+    static __device__ __forceinline__ v16f qk(v4u k, v4u q, v16f s) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, k), __builtin_bit_cast(v8h, q), s, 0, 0, 0);
+    }
+    // round to nearest even, as all roundings here
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+        const v2h p = {(_Float16)x, (_Float16)y};
+        return __builtin_bit_cast(uint32_t, p);
+    }
+    static constexpr uint32_t SIGNS = 0x80008000u;
+};
+template <> struct AtMma<bf16_t> {
+    static __device__ __forceinline__ v16f qk(v4u k, v4u q, v16f s) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, k), __builtin_bit_cast(v8b, q), s, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        uint32_t r;
+        asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
+        return r;
+    }
+    static constexpr uint32_t SIGNS = 0x80008000u;
+};
+template <> struct AtMma<float> {
+    static __device__ __forceinline__ v16f qk(v4u k, v4u q, v16f s) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q[e]), s, 0, 0, 0);
+        return s;
+    }
+    static __device__ __forceinline__ uint32_t pack(float, float) { return 0; }
+    static constexpr uint32_t SIGNS = 0x80000000u;
+};
+
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+__device__ __forceinline__ v4u at_lds16(const lds_byte* at) { return *(const __attribute__((address_space(3))) v4u*)at; }
+__device__ __forceinline__ float at_lds4(const lds_byte* at) { return *(const __attribute__((address_space(3))) float*)at; }
+// Lane i of each 16 gives the address of 4 elements and receives, of the 4 rows that lanes 4r .. 4r + 3 address, column i
+__device__ __forceinline__ v2u at_lds_turned(const lds_byte* at) {
+    return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)const_cast<lds_byte*>(at)));
+}
+// 16 bytes a lane from memory to LDS: lane i's to at + 16 i
+__device__ __forceinline__ void at_to_lds(const void* from, lds_byte* at) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)from, (__attribute__((address_space(3))) void*)at, 16, 0, 0);
+}
+// x and the other half's value of the same column
+__device__ __forceinline__ float at_other(float x) {
+    typedef unsigned int v2 __attribute__((ext_vector_type(2)));
+    const v2 r = __builtin_bit_cast(v2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return __uint_as_float(__lane_id() < 32 ? r[1] : r[0]);
+}
+
+// ------------------------------------------------------------------------------------------------------- shape
+// Head dims up to DT columns; EXACT: DT itself, known to the compiler.
+template <typename T, int DT> struct AtShape {
+    static constexpr int CE = 16 / sizeof(T);                  // elements of a chunk
+    static constexpr int STEPS = (DT + 2 * CE - 1) / (2 * CE); // pairs of chunks in a row
+    static constexpr int BLOCKS = (DT + 31) / 32;              // 32-column blocks of the result
+    static constexpr int KT = sizeof(T) == 2 && DT <= 128 ? 64 : 32;
+    static constexpr int HALVES = KT / 32;
+    static constexpr int CHUNKS = DT / CE;                     // of a row, at most
+    static constexpr int LOADS = (KT * CHUNKS + AT_BLOCK - 1) / AT_BLOCK;      // of a tile of keys (or values), by each wave
+    // a wave's last load of a tile may reach beyond it, and so may the transposed reads of the last block of columns
+    static constexpr int TILE = (KT * CHUNKS * 16 + 1023) / 1024 * 1024;
+    static constexpr int LDS = 4 * TILE + 256;
+};
+
+// 16-byte chunks of a row are rotated by an amount that goes by the row, so that what the lanes of one access read spreads over the banks: keys are read a
+// chunk from each of 16 rows at a time, values 32 bytes from each of 8 rows.
+__device__ __forceinline__ uint32_t at_turn_k(uint32_t row, uint32_t chunks) {
+    const uint32_t z = chunks % 16 == 0 ? 4 : chunks % 8 == 0 ? 3 : chunks % 4 == 0 ? 2 : chunks % 2 == 0 ? 1 : 0;
+    return (row & 15) >> (4 - z);
+}
+template <typename T> __device__ __forceinline__ uint32_t at_turn_v(uint32_t row, uint32_t chunks) {
+    if (sizeof(T) == 4 || chunks % 2) return 0;
+    const uint32_t z = chunks % 16 == 0 ? 3 : chunks % 8 == 0 ? 2 : chunks % 4 == 0 ? 1 : 0;
+    return 2 * ((row & 7) >> (3 - z));
+}
+
+// One row over the keys of tiles [tile0, tile1) of a walk, a lane to a key for the scores and to columns for the result: visible keys alone are touched.
+template <typename T, int DT, bool PAGED, int KT>
+__device__ __forceinline__ void at_row_again(const AttnArgs& a, uint32_t b, uint32_t g, AttnSeq s, AttnWalk w, uint32_t tile0, uint32_t tile1, uint32_t row, float* o, float& m_out,
+                                          float& l_out) {
+    constexpr int COLS = (DT + 63) / 64;
+    const uint32_t lane = __lane_id(), D = a.dim, j = fd_div(row, a.group_div), h = g * a.group + (row - j * a.group);
+    const T* q = (const T*)a.q + b * a.q_b + h * a.q_h + (uint64_t)(s.first + j) * a.q_t;
+    const T* k = (const T*)a.k + g * a.k_h + (PAGED ? 0 : b * a.k_b);
+    const T* v = (const T*)a.v + g * a.v_h + (PAGED ? 0 : b * a.v_b);
+    const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < COLS; i++) o[i] = 0.0f;
+    for (uint32_t tile = tile0; tile < tile1; tile++) {
+        const int32_t t = (tile < w.head ? (int32_t)(tile * KT) : w.from + (int32_t)((tile - w.head) * KT)) + (int32_t)lane;
+        bool seen = lane < KT && at_visible(a, t, limit, p);
+        uint64_t k_at = 0, v_at = 0;
+        if (seen) {
+            if (PAGED) {
+                uint32_t slot;
+                const int32_t page = at_page(a, b, (uint32_t)t, slot);
+                seen = page >= 0;
+                k_at = (uint64_t)(seen ? page : 0) * a.k_b + slot * a.k_t;
+                v_at = (uint64_t)(seen ? page : 0) * a.v_b + slot * a.v_t;
+            } else {
+                k_at = (uint64_t)t * a.k_t;
+                v_at = (uint64_t)t * a.v_t;
+            }
+        }
+        float x = -INFINITY;
+        if (seen) {
+            float dot = 0.0f;
+            for (uint32_t d = 0; d < D; d++) dot = __builtin_fmaf(Ar<T>::widen(q[d]), Ar<T>::widen(k[k_at + d]), dot);
+            x = dot * a.c;
+        }
+        uint64_t todo = __ballot(seen);
+        if (!todo) continue;
+        float top = x;
+        for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+        const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.0f : m_new;
+        const float old = at_exp2(m - base), e = seen ? at_exp2(x - base) : 0.0f;
+        m = m_new;
+        l = __builtin_fmaf(l, old, at_wave_sum(e));
+#pragma unroll
+        for (int i = 0; i < COLS; i++) o[i] *= old;
+        while (todo) {
+            const int src = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const float ei = __shfl(e, src);
+            const uint64_t from = __shfl(v_at, src);
+#pragma unroll
+            for (int i = 0; i < COLS; i++)
+                if (i * 64 + lane < D) o[i] = __builtin_fmaf(ei, Ar<T>::widen(v[from + i * 64 + lane]), o[i]);
+        }
+    }
+    m_out = m;
+    l_out = l;
+}
+
+struct AttnPartial {
+    float* o;                      // [items * kv heads][AT_ROWS][dim], unnormalised
+    float* ml;                     // [items * kv heads][AT_ROWS][2]: m (of scaled scores, base 2), l
+    uint32_t pieces;               // contiguous: pieces of the keys a row tile is split into, `piece` tiles each
+    uint32_t piece;
+    uint32_t row_tiles;            // contiguous: of each batch entry
+    uint32_t blocks;               // of the launch: what there are partial results of
+};
+
+template <typename T, int DT, bool EXACT, bool PAGED>
+__global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) attention_tile_kernel(AttnArgs a, AttnPartial part) {
+    typedef AtShape<T, DT> S;
+    constexpr int KT = S::KT, CE = S::CE;
+    extern __shared__ unsigned char smem[];
+    lds_byte* const lds = (lds_byte*)smem;
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
+    const uint32_t D = EXACT ? DT : a.dim, chunks = D / CE, pitch = D * sizeof(T);
+
+    // ---- which rows, which keys
+    uint32_t b, g, tile, piece_at, piece;
+    if (PAGED) {
+        g = blockIdx.x % a.kv_heads;
+        uint32_t at = blockIdx.x / a.kv_heads;
+        piece = __builtin_amdgcn_readfirstlane(at_piece<KT>(a));
+        b = __builtin_amdgcn_readfirstlane(at_locate<KT>(a, piece, at));
+        if (b >= a.seqs) return;
+        tile = __builtin_amdgcn_readfirstlane(at);
+        piece_at = 0;
+    } else {
+        const uint32_t pairs = a.seqs * a.kv_heads, pair = blockIdx.x % pairs, at = blockIdx.x / pairs;
+        b = pair / a.kv_heads;
+        g = pair - b * a.kv_heads;
+        piece = part.piece;
+        tile = part.row_tiles - 1 - at / part.pieces;                           // the longest walks first
+        piece_at = at % part.pieces;
+    }
+    const AttnSeq s = at_seq<PAGED>(a, b);
+    if (PAGED) {
+        const uint32_t pieces = (at_span<KT>(a, s) + piece - 1) / piece, at = tile;
+        tile = at / pieces;
+        piece_at = at - tile * pieces;
+        tile = at_row_tiles(a, s) - 1 - tile;
+    }
+    const uint32_t all = s.count * a.group, row0 = tile * AT_ROWS, rows = all - row0 < AT_ROWS ? all - row0 : AT_ROWS;
+    const AttnWalk w = at_walk<KT>(a, s, row0, rows);
+    const uint32_t tile0 = piece_at * piece, tile1 = w.tiles - tile0 < piece || tile0 >= w.tiles ? w.tiles : tile0 + piece;
+    const bool whole = w.tiles <= piece;                        // no other block has keys of these rows
+    if (tile0 >= w.tiles && piece_at > 0) return;
+
+    // ---- this lane's row
+    const uint32_t r = wave * 32 + col, row = row0 + (r < rows ? r : rows - 1);
+    const uint32_t j = fd_div(row, a.group_div), h = g * a.group + (row - j * a.group);
+    const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
+    // and what all rows of the wave see, and any of them
+    const bool busy = wave * 32 < rows;
+    const uint32_t ja = fd_div(row0 + (busy ? wave * 32 : 0), a.group_div), jz = fd_div(row0 + (wave * 32 + 31 < rows ? wave * 32 + 31 : rows - 1), a.group_div);
+    const int32_t limit_a = at_limit(a, s, ja), limit_z = at_limit(a, s, jz), p_a = at_position(s, ja), p_z = at_position(s, jz);
+
+    v4u q[S::STEPS];
+    {
+        const T* from = (const T*)a.q + b * a.q_b + h * a.q_h + (uint64_t)(s.first + j) * a.q_t;
+        const uint32_t flip = a.c < 0.0f ? AtMma<T>::SIGNS : 0;
+#pragma unroll
+        for (int i = 0; i < S::STEPS; i++) {
+            q[i] = v4u{0, 0, 0, 0};
+            if ((2 * i + half) * CE < D) q[i] = *(const v4u*)(from + (2 * i + half) * CE);
+            q[i] ^= v4u{flip, flip, flip, flip};
+        }
+    }
+    // |scale| log2 e; never 0, so that a hidden key's -inf stays
+    const float c = fmaxf(__builtin_fabsf(a.c), 1e-37f);
+
+    // ---- this lane's part of a tile's loads: LDS chunk `slot` belongs to row slot / chunks
+    uint32_t l_row[S::LOADS], l_k[S::LOADS], l_v[S::LOADS];
+    const uint32_t slots = KT * chunks, loads = (slots + 63) / 64;
+#pragma unroll
+    for (int i = 0; i < S::LOADS; i++) {
+        uint32_t slot = (i * AT_WAVES + wave) * 64 + lane;
+        slot = slot < slots ? slot : slots - 1;
+        const uint32_t rr = slot / chunks, cc = slot - rr * chunks;
+        const uint32_t tk = at_turn_k(rr, chunks), tv = at_turn_v<T>(rr, chunks);
+        l_row[i] = rr;
+        l_k[i] = (cc >= tk ? cc - tk : cc + chunks - tk) * 16;
+        l_v[i] = (cc >= tv ? cc - tv : cc + chunks - tv) * 16;
+    }
+    const unsigned char* kb = (const unsigned char*)a.k + (g * a.k_h + (PAGED ? 0 : b * a.k_b)) * sizeof(T);
+    const unsigned char* vb = (const unsigned char*)a.v + (g * a.v_h + (PAGED ? 0 : b * a.v_b)) * sizeof(T);
+    const uint32_t k_row = (uint32_t)(a.k_t * sizeof(T)), v_row = (uint32_t)(a.v_t * sizeof(T));
+    const uint32_t k_page = PAGED ? (uint32_t)(a.k_b * sizeof(T)) : 0;
+    auto start_of = [&](uint32_t n) -> int32_t { return n < w.head ? (int32_t)(n * KT) : w.from + (int32_t)((n - w.head) * KT); };
+    // paged: the page of key `lane` of tile n, and its row there
+    auto look = [&](uint32_t n, uint32_t& slot) -> int32_t {
+        int32_t t = start_of(n) + (int32_t)(lane % KT);
+        t = t < s.keys ? t : s.keys - 1;
+        return at_page(a, b, (uint32_t)t, slot);
+    };
+    auto fetch = [&](uint32_t n, lds_byte* to, int32_t page, uint32_t slot) __attribute__((always_inline)) {
+        const int32_t t0 = start_of(n);
+#pragma unroll
+        for (int i = 0; i < S::LOADS; i++) {
+            if (i * AT_WAVES + wave >= loads) break;
+            lds_byte* const at = to + (i * AT_WAVES + wave) * 1024;
+            uint64_t k_off, v_off;
+            if (PAGED) {
+                int32_t pg = __shfl(page, (int)l_row[i]);
+                const uint32_t sl = (uint32_t)__shfl((int)slot, (int)l_row[i]);
+                pg = pg < 0 ? 0 : pg;
+                k_off = (uint64_t)(uint32_t)pg * k_page + sl * (uint64_t)k_row;
+                v_off = k_off;
+            } else {
+                int32_t t = t0 + (int32_t)l_row[i];
+                t = t < s.keys ? t : s.keys - 1;
+                k_off = (uint64_t)(uint32_t)t * k_row;
+                v_off = (uint64_t)(uint32_t)t * v_row;
+            }
+            at_to_lds(kb + k_off + l_k[i], at);
+            at_to_lds(vb + v_off + l_v[i], at + S::TILE);
+        }
+    };
+
+    // ---- where this lane reads a tile
+    uint32_t k_at[S::STEPS], v_at[S::BLOCKS];
+#pragma unroll
+    for (int i = 0; i < S::STEPS; i++) {
+        uint32_t cc = 2 * i + half;
+        cc = cc < chunks ? cc : 0;                              // beyond the row: replaced by 0 below
+        cc += at_turn_k(col, chunks);
+        k_at[i] = col * pitch + (cc >= chunks ? cc - chunks : cc) * 16;
+    }
+    const uint32_t v_key = 4 * half + (lane % 16) / 4;
+#pragma unroll
+    for (int i = 0; i < S::BLOCKS; i++) {
+        if (sizeof(T) == 2) {
+            uint32_t cc = 4 * i + 2 * ((lane / 16) & 1);
+            if (cc >= chunks) cc = 0;                           // columns of nobody
+            cc += at_turn_v<T>(v_key, chunks);
+            if (cc >= chunks) cc -= chunks;
+            v_at[i] = S::TILE + v_key * pitch + cc * 16 + (lane % 4) * 8;
+        } else {
+            v_at[i] = S::TILE + 4 * half * pitch + (i * 32 + col < D ? i * 32 + col : 0) * 4;
+        }
+    }
+
+    v16f o[S::BLOCKS];
+#pragma unroll
+    for (int i = 0; i < S::BLOCKS; i++) o[i] = v16f{0};
+    float m = -INFINITY, l = 0.0f;                              // l: of this lane's half of the keys
+
+    int32_t page = 0;
+    uint32_t slot = 0;
+    uint64_t there = ~0ull;                                     // keys of the tile at hand that have a page
+    if (tile0 < tile1) {
+        if (PAGED) page = look(tile0, slot);
+        fetch(tile0, lds, page, slot);
+    }
+    // One tile: the loads of the next one go into `next` while this one is read from `cur`.  The two never overlap, which is what lets the compiler
+    // leave the loads in flight: the wait for them stands at the top of the next step.
+    auto step = [&](uint32_t n, lds_byte* __restrict next, const lds_byte* __restrict cur) __attribute__((always_inline)) {
+        if (n + 1 < tile1) fetch(n + 1, next, page, slot);
+        const int32_t t0 = start_of(n);
+        if (!busy || t0 > limit_z || (t0 >= a.sinks && p_a - (t0 + KT - 1) >= a.window)) return;
+
+        v16f x[S::HALVES];
+#pragma unroll
+        for (int kk = 0; kk < S::HALVES; kk++) {
+            x[kk] = v16f{0};
+#pragma unroll
+            for (int i = 0; i < S::STEPS; i++) {
+                if (!EXACT && (uint32_t)(2 * i * CE) >= D) break;
+                v4u k = at_lds16(cur + (k_at[i] + kk * 32 * pitch));
+                if ((EXACT ? DT % (2 * CE) != 0 : true) && (2 * i + 2) * CE > (int)D && half) k = v4u{0, 0, 0, 0};
+                x[kk] = AtMma<T>::qk(k, q[i], x[kk]);
+            }
+        }
+        if (t0 + KT - 1 > limit_a || (t0 + KT > a.sinks && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
+            // key 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile
+            const int32_t lim = limit - t0 - 4 * (int32_t)half, near = p - t0 - 4 * (int32_t)half, sink = a.sinks - t0 - 4 * (int32_t)half;
+            const uint64_t have = there >> (4 * half);
+#pragma unroll
+            for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int32_t t = 32 * kk + e % 4 + 8 * (e / 4);
+                    const bool seen = t <= lim && (near - t < a.window || t < sink) && (!PAGED || (have >> t) & 1);
+                    x[kk][e] = seen ? x[kk][e] : -INFINITY;
+                }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = fmaxf(top, x[kk][e]);
+        top = fmaxf(top, at_other(top)) * c;
+        if (__ballot(top > m)) {
+            const float m_new = fmaxf(m, top), old = at_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
+            m = m_new;
+            l *= old;
+#pragma unroll
+            for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[i][e] *= old;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                x[kk][e] = at_exp2(__builtin_fmaf(x[kk][e], c, -base));
+                sum += x[kk][e];
+            }
+        l += sum;
+#pragma unroll
+        for (int kk = 0; kk < S::HALVES; kk++) {
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {                   // 16 keys at a time
+                    v4u w8;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w8[e] = AtMma<T>::pack(x[kk][8 * u + 2 * e], x[kk][8 * u + 2 * e + 1]);
+#pragma unroll
+                    for (int i = 0; i < S::BLOCKS; i++) {
+                        if (!EXACT && (uint32_t)(32 * i) >= D) break;
+                        const uint32_t at = v_at[i] + (32 * kk + 16 * u) * pitch;
+                        const v2u lo = at_lds_turned(cur + at), hi = at_lds_turned(cur + (at + 8 * pitch));
+                        o[i] = AtMma<T>::qk(v4u{lo[0], lo[1], hi[0], hi[1]}, w8, o[i]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+#pragma unroll
+                    for (int i = 0; i < S::BLOCKS; i++) {
+                        if (!EXACT && (uint32_t)(32 * i) >= D) break;
+                        const float v = at_lds4(cur + (v_at[i] + (32 * kk + e % 4 + 8 * (e / 4)) * pitch));
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x[kk][e], o[i], 0, 0, 0);
+                    }
+            }
+        }
+    };
+    for (uint32_t n = tile0; n < tile1; n++) {
+        if (PAGED) {
+            there = __ballot(page >= 0);
+            if (n + 1 < tile1) page = look(n + 1, slot);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);                     // vmcnt(0): this wave's loads have arrived
+        __syncthreads();                                        // and everyone's; and everyone is done with the other stage
+        const uint32_t stage = (n - tile0) & 1;
+        step(n, lds + (stage ^ 1) * 2 * S::TILE, lds + stage * 2 * S::TILE);
+    }
+    if (!busy) return;
+
+    // ---- result: lane's columns of d are 32 i + 8 (e / 4) + 4 half + e % 4
+    l += at_other(l);
+    const uint64_t out = (uint64_t)blockIdx.x * AT_ROWS + r;    // of the partial results
+    bool fine = __builtin_isfinite(l) && m < INFINITY;
+#pragma unroll
+    for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            if (32 * i + 8 * (e / 4) + 4 * half < D) fine = fine && __builtin_isfinite(o[i][e]);
+    if (__ballot(r < rows && !fine)) {
+        const uint32_t end = wave * 32 + 32 < rows ? wave * 32 + 32 : rows;
+        for (uint32_t rr = wave * 32; rr < end; rr++) {
+            float oo[(DT + 63) / 64], mm, ll;
+            at_row_again<T, DT, PAGED, KT>(a, b, g, s, w, tile0, tile1, row0 + rr, oo, mm, ll);
+            const uint32_t jj = fd_div(row0 + rr, a.group_div), hh = g * a.group + (row0 + rr - jj * a.group);
+            const uint64_t slot_at = (uint64_t)blockIdx.x * AT_ROWS + rr;
+            const float inv = whole ? (ll == 0.0f ? 0.0f : 1.0f / ll) : 1.0f;
+            T* y = (T*)a.y + b * a.y_b + hh * a.y_h + (uint64_t)(s.first + jj) * a.y_t;
+            for (uint32_t i = 0; i < (DT + 63) / 64; i++)
+                if (i * 64 + lane < D) {
+                    if (whole) y[i * 64 + lane] = Ar<T>::conv(oo[i] * inv);
+                    else part.o[slot_at * D + i * 64 + lane] = oo[i];
+                }
+            if (lane == 0) {
+                if (!whole) {
+                    part.ml[2 * slot_at] = mm;
+                    part.ml[2 * slot_at + 1] = ll;
+                } else if (a.lse) {
+                    a.lse[b * a.l_b + hh * a.l_h + (uint64_t)(s.first + jj) * a.l_t] = at_lse(mm, ll);
+                }
+            }
+        }
+        return;
+    }
+    if (r >= rows) return;
+    if (whole) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        T* y = (T*)a.y + b * a.y_b + h * a.y_h + (uint64_t)(s.first + j) * a.y_t;
+#pragma unroll
+        for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const uint32_t d = 32 * i + 8 * (e / 4) + 4 * half;
+                if (d >= D) continue;
+                if constexpr (sizeof(T) == 2) {
+                    const v2u put = {AtMma<T>::pack(o[i][e] * inv, o[i][e + 1] * inv), AtMma<T>::pack(o[i][e + 2] * inv, o[i][e + 3] * inv)};
+                    *(v2u*)(y + d) = put;
+                } else {
+                    typedef float v4f __attribute__((ext_vector_type(4)));
+                    *(v4f*)(y + d) = v4f{o[i][e] * inv, o[i][e + 1] * inv, o[i][e + 2] * inv, o[i][e + 3] * inv};
+                }
+            }
+        if (a.lse && half == 0) a.lse[b * a.l_b + h * a.l_h + (uint64_t)(s.first + j) * a.l_t] = at_lse(m, l);
+    } else {
+        typedef float v4f __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int i = 0; i < S::BLOCKS; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const uint32_t d = 32 * i + 8 * (e / 4) + 4 * half;
+                if (d < D) *(v4f*)(part.o + out * D + d) = v4f{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+            }
+        if (half == 0) {
+            part.ml[2 * out] = m;
+            part.ml[2 * out + 1] = l;
+        }
+    }
+}
+
+// Joins the pieces of rows whose keys several blocks walked: a wave to a (token, head) row.
+template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_BLOCK) attention_join_kernel(AttnArgs a, AttnPartial part, uint64_t rows_all) {
+    const uint32_t lane = threadIdx.x % 64, D = a.dim;
+    const uint64_t id = (uint64_t)blockIdx.x * AT_WAVES + threadIdx.x / 64;
+    if (id >= rows_all) return;
+    const uint32_t h = (uint32_t)(id % a.heads), g = h / a.group;
+    const uint64_t token = id / a.heads;
+    uint32_t b, j, piece, pieces, first;
+    AttnSeq s;
+    if (PAGED) {
+        b = at_find(a.starts, a.seqs, (uint32_t)token);
+        if (b == a.seqs) return;
+        s = at_seq<true>(a, b);
+        if (token < s.first || token - s.first >= s.count) return;
+        j = (uint32_t)token - s.first;
+        piece = at_piece<KT>(a);
+    } else {
+        b = (uint32_t)(token / a.tokens);
+        j = (uint32_t)(token % a.tokens);
+        s = at_seq<false>(a, b);
+        piece = part.piece;
+    }
+    const uint32_t row = j * a.group + (h - g * a.group), tile = row / AT_ROWS, all = s.count * a.group;
+    const AttnWalk w = at_walk<KT>(a, s, tile * AT_ROWS, all - tile * AT_ROWS < AT_ROWS ? all - tile * AT_ROWS : AT_ROWS);
+    if (w.tiles <= piece) return;
+    const uint32_t used = (w.tiles + piece - 1) / piece;
+    uint64_t stride;
+    if (PAGED) {
+        pieces = (at_span<KT>(a, s) + piece - 1) / piece;
+        first = (at_before<KT>(a, piece, b) + (at_row_tiles(a, s) - 1 - tile) * pieces) * a.kv_heads + g;
+        stride = a.kv_heads;
+    } else {
+        first = (part.row_tiles - 1 - tile) * part.pieces * a.seqs * a.kv_heads + b * a.kv_heads + g;
+        stride = (uint64_t)a.seqs * a.kv_heads;
+    }
+    if (first + (used - 1) * stride >= part.blocks) return;    // rows counted more than once: starts that decrease
+    const uint32_t r = row - tile * AT_ROWS;
+    float m = -INFINITY;
+    for (uint32_t i = lane; i < used; i += 64) m = fmaxf(m, part.ml[2 * ((first + i * stride) * AT_ROWS + r)]);
+#pragma unroll
+    for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i = 0; i < used; i++) {
+        const uint64_t at = (first + i * stride) * AT_ROWS + r;
+        const float e = at_exp2(part.ml[2 * at] - base);
+        l = __builtin_fmaf(e, part.ml[2 * at + 1], l);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k * 64 + lane < D) o[k] = __builtin_fmaf(e, part.o[at * D + k * 64 + lane], o[k]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* y = (T*)a.y + b * a.y_b + h * a.y_h + (uint64_t)(s.first + j) * a.y_t;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (k * 64 + lane < D) y[k * 64 + lane] = Ar<T>::conv(o[k] * inv);
+    if (a.lse && lane == 0) a.lse[b * a.l_b + h * a.l_h + (uint64_t)(s.first + j) * a.l_t] = at_lse(m, l);
+}
+
+template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_device* dev, AttnArgs& a) {
+    typedef AtShape<T, DT> S;
+    AttnPartial part = {};
+    uint64_t items, rows_all;                                   // blocks per KV head (paged) or per (batch entry, KV head)
+    const uint64_t per = PAGED ? a.kv_heads : (uint64_t)a.seqs * a.kv_heads;
+    bool split;
+    if (PAGED) {
+        rows_all = (uint64_t)a.tokens * a.heads;
+        const uint64_t tiles = ((uint64_t)a.tokens * a.group) / AT_ROWS + a.seqs;
+        // sum over the row tiles of ceil(span / piece): at most AT_TARGET / kv_heads + 1 and one for each row tile
+        split = a.cap > AT_LEAST_TILES * S::KT;
+        items = tiles + (split ? AT_TARGET / a.kv_heads + 1 : 0);
+    } else {
+        rows_all = (uint64_t)a.seqs * a.tokens * a.heads;
+        part.row_tiles = (uint32_t)(((uint64_t)a.tokens * a.group + AT_ROWS - 1) / AT_ROWS);
+        uint64_t span = (a.cap + S::KT - 1) / S::KT;
+        if (a.window != AT_FAR) {
+            const uint64_t w = ((uint64_t)a.window + AT_ROWS) / S::KT + 2 + ((uint64_t)a.sinks + S::KT - 1) / S::KT;
+            span = w < span ? w : span;
+        }
+        uint64_t piece = (span * part.row_tiles * per + AT_TARGET - 1) / AT_TARGET;
+        piece = piece < AT_LEAST_TILES ? AT_LEAST_TILES : piece;
+        part.piece = (uint32_t)piece;
+        part.pieces = (uint32_t)((span + piece - 1) / piece);
+        split = part.pieces > 1;
+        items = (uint64_t)part.row_tiles * part.pieces;
+    }
+    const uint64_t blocks = items * per;
+    RT_REQUIRE(blocks <= 0x7fffffffull && (rows_all + AT_WAVES - 1) / AT_WAVES <= 0x7fffffffull, RT_ERR_SIZE, "attention: too many rows");
+    part.blocks = (uint32_t)blocks;
+    const size_t row_count = split ? (size_t)blocks * AT_ROWS : 0;
+    void* p = nullptr;
+    int rc = at_workspace(dev, a, row_count * ((size_t)a.dim + 2) * sizeof(float), &p);
+    if (rc) return rc;
+    part.ml = (float*)p;
+    part.o = part.ml + 2 * row_count;
+    const auto kernel = attention_tile_kernel<T, DT, EXACT, PAGED>;
+    const size_t lds = S::LDS;
+    static_assert(S::LDS <= 160 * 1024, "LDS");
+    static bool raised[16] = {};                                // per GPU; setting it twice does no harm
+    if (lds > 64 * 1024 && !(dev->ordinal < 16 && raised[dev->ordinal])) {
+        RT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        if (dev->ordinal < 16) raised[dev->ordinal] = true;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(AT_BLOCK), lds, dev->stream, a, part);
+    RT_CHECK_LAUNCH("attention_tile_kernel");
+    if (split) {
+        hipLaunchKernelGGL((attention_join_kernel<T, S::KT, PAGED>), dim3((unsigned)((rows_all + AT_WAVES - 1) / AT_WAVES)), dim3(AT_BLOCK), 0, dev->stream, a, part, rows_all);
+        RT_CHECK_LAUNCH("attention_join_kernel");
+    }
+    return RT_OK;
+}
+
+template <typename T> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool paged, bool* done) {
+    // rows of whole 16-byte chunks on 16-byte boundaries, 32-bit offsets of rows in a page and of pages
+    const uint64_t e = sizeof(T), most = 0xffffffffull / e;
+    const uint64_t strides[] = {a.dim, a.q_b, a.q_h, a.q_t, a.k_b, a.k_h, a.k_t, a.v_b, a.v_h, a.v_t, a.y_b, a.y_h, a.y_t};
+    bool fits = rt_aligned(a.q, 16) && rt_aligned(a.k, 16) && rt_aligned(a.v, 16) && rt_aligned(a.y, 16) && a.k_t <= most && a.v_t <= most && (!paged || a.k_b <= most) &&
+                (uint64_t)a.tokens * a.group <= 0x7fffffffull && a.dim <= 256;
+    for (uint64_t x : strides) fits = fits && x * e % 16 == 0;
+    *done = fits;
+    if (!fits) return RT_OK;
+#define RT_TILE(DT, EXACT) return paged ? at_launch_tile<T, DT, EXACT, true>(dev, a) : at_launch_tile<T, DT, EXACT, false>(dev, a)
+    if (a.dim == 64) RT_TILE(64, true);
+    if (sizeof(T) == 2 && a.dim == 80) RT_TILE(80, true);
+    if (sizeof(T) == 2 && a.dim == 96) RT_TILE(96, true);
+    if (sizeof(T) == 2 && a.dim == 128) RT_TILE(128, true);
+    if (a.dim <= 128) RT_TILE(128, false);
+    RT_TILE(256, false);
+#undef RT_TILE
+}
+
+#endif

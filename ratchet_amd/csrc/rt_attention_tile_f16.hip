@@ -1,0 +1,4 @@
+// The attention kernels of rt_attention_tile.h for f16
+#include "rt_attention_tile.h"
+
+int rt_attention_tile_f16(rt_device* dev, AttnArgs& a, bool paged, bool* done) { return at_dispatch_tile<half_t>(dev, a, paged, done); }
