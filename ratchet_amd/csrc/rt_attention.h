@@ -54,6 +54,10 @@ static inline int at_workspace(rt_device* dev, AttnArgs& a, size_t bytes, void**
 int rt_attention_tile_f32(rt_device* dev, AttnArgs& a, bool paged, bool* done);
 int rt_attention_tile_f16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
 int rt_attention_tile_bf16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
+// Received weights of a paged call that the kernel above took (rt_attention_weights.h); a.lse holds its rows' statistics
+int rt_attention_weights_f32(rt_device* dev, const AttnArgs& a, const float* weights, float* out);
+int rt_attention_weights_f16(rt_device* dev, const AttnArgs& a, const float* weights, float* out);
+int rt_attention_weights_bf16(rt_device* dev, const AttnArgs& a, const float* weights, float* out);
 
 #ifdef __HIPCC__
 

@@ -121,32 +121,36 @@ __global__ void __launch_bounds__(64) attention_weights_any_kernel(AttnArgs a, c
     if (t < s.keys) out[at] = sum;
 }
 
-template <typename T> int launch_any(rt_device* dev, const AttnArgs& a, bool paged) {
+template <typename T> int launch_any(rt_device* dev, const AttnArgs& a, bool paged, const float* weights, float* weights_out) {
     const uint64_t rows = (uint64_t)(paged ? 1 : a.seqs) * a.tokens * a.heads, blocks = (rows + WAVES - 1) / WAVES;
     RT_REQUIRE(blocks <= 0x7fffffffull, RT_ERR_SIZE, "attention: too many rows");
     if (paged) hipLaunchKernelGGL((attention_any_kernel<T, true>), dim3((unsigned)blocks), dim3(BLOCK), 0, dev->stream, a, rows);
     else hipLaunchKernelGGL((attention_any_kernel<T, false>), dim3((unsigned)blocks), dim3(BLOCK), 0, dev->stream, a, rows);
     RT_CHECK_LAUNCH("attention_any_kernel");
+    if (weights_out) {
+        hipLaunchKernelGGL((attention_weights_any_kernel<T>), dim3((a.cap + 63) / 64, a.kv_heads, a.seqs), dim3(64), 0, dev->stream, a, weights, weights_out);
+        RT_CHECK_LAUNCH("attention_weights_any_kernel");
+    }
     return RT_OK;
 }
 
-template <typename T> int launch_weights_any(rt_device* dev, const AttnArgs& a, const float* weights, float* out) {
-    const dim3 grid((a.cap + 63) / 64, a.kv_heads, a.seqs);
-    hipLaunchKernelGGL((attention_weights_any_kernel<T>), grid, dim3(64), 0, dev->stream, a, weights, out);
-    RT_CHECK_LAUNCH("attention_weights_any_kernel");
-    return RT_OK;
-}
-
-int dispatch(rt_device* dev, int dt, AttnArgs& a, bool paged) {
+int dispatch(rt_device* dev, int dt, AttnArgs& a, bool paged, const float* weights, float* weights_out) {
     bool done;
     int rc = dt == RT_F32 ? rt_attention_tile_f32(dev, a, paged, &done) : dt == RT_F16 ? rt_attention_tile_f16(dev, a, paged, &done) : rt_attention_tile_bf16(dev, a, paged, &done);
-    if (rc || done) return rc;
+    if (rc || (done && !weights_out)) return rc;
+    if (done) {
+        switch (dt) {
+            case RT_F32: return rt_attention_weights_f32(dev, a, weights, weights_out);
+            case RT_F16: return rt_attention_weights_f16(dev, a, weights, weights_out);
+            default: return rt_attention_weights_bf16(dev, a, weights, weights_out);
+        }
+    }
     void* none = nullptr;
     if ((rc = at_workspace(dev, a, 0, &none))) return rc;
     switch (dt) {
-        case RT_F32: return launch_any<float>(dev, a, paged);
-        case RT_F16: return launch_any<half_t>(dev, a, paged);
-        default: return launch_any<bf16_t>(dev, a, paged);
+        case RT_F32: return launch_any<float>(dev, a, paged, weights, weights_out);
+        case RT_F16: return launch_any<half_t>(dev, a, paged, weights, weights_out);
+        default: return launch_any<bf16_t>(dev, a, paged, weights, weights_out);
     }
 }
 
@@ -267,7 +271,7 @@ int rt_attention(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4
     a.tokens = q_shape[2];
     a.cap = kv_shape[2];
     a.causal = causal;
-    return dispatch(dev, dt, a, false);
+    return dispatch(dev, dt, a, false, nullptr, nullptr);
 }
 
 int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_strides[2], uint32_t tokens, uint32_t heads, const rt_paged_kv* kv,
@@ -301,13 +305,7 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
     a.page_div = make_fastdiv(kv->page_len);
     a.causal = 1;
     a.own_lse = weights_out && !lse ? (size_t)tokens * heads * sizeof(float) : 0;
-    if ((rc = dispatch(dev, dt, a, true))) return rc;
-    if (!weights_out) return RT_OK;
-    switch (dt) {
-        case RT_F32: return launch_weights_any<float>(dev, a, weights, weights_out);
-        case RT_F16: return launch_weights_any<half_t>(dev, a, weights, weights_out);
-        default: return launch_weights_any<bf16_t>(dev, a, weights, weights_out);
-    }
+    return dispatch(dev, dt, a, true, weights, weights_out);
 }
 
 }  // extern "C"
