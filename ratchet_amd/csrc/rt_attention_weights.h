@@ -110,8 +110,7 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : 2) attention_weights_
             v16f x = {0};
 #pragma unroll
             for (int i = 0; i < S::STEPS; i++) {
-                if (!EXACT && (uint32_t)(2 * i * CE) >= D) break;
-                x = AtMma<T>::qk(k[i], q[i], x);
+                if (EXACT || (uint32_t)(2 * i * CE) < D) x = AtMma<T>::qk(k[i], q[i], x);
             }
             const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
             const bool real = r + col < r1;

@@ -64,36 +64,17 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// exclusive sums over the block of two flags a thread, in thread order; totals to all
-__device__ __forceinline__ void block_ranks(bool x, bool y, uint32_t* lds, uint32_t& rank_x, uint32_t& rank_y, uint32_t& total_x, uint32_t& total_y) {
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const uint64_t bx = __ballot(x), by = __ballot(y), below = ((uint64_t)1 << lane) - 1;
-    if (lane == 0) {
-        lds[2 * wave] = (uint32_t)__popcll(bx);
-        lds[2 * wave + 1] = (uint32_t)__popcll(by);
-    }
-    __syncthreads();
-    rank_x = (uint32_t)__popcll(bx & below);
-    rank_y = (uint32_t)__popcll(by & below);
-    total_x = total_y = 0;
-    for (uint32_t i = 0; i < SELECT_BLOCK / 64; i++) {
-        if (i < wave) {
-            rank_x += lds[2 * i];
-            rank_y += lds[2 * i + 1];
-        }
-        total_x += lds[2 * i];
-        total_y += lds[2 * i + 1];
-    }
-    __syncthreads();
-}
-
 // A block to a (sequence, KV head).  The weight of the last token that stays is found digit by digit, eight bits at a time from the top
 // (a histogram of the candidates that share the digits found so far); then one walk over the tokens writes the list of those that stay and
-// moves their weights.  A weight moves to an index at or below its own and a walk's step reads its tokens before it writes, so weights_out may be weights.
+// moves their weights.  A round takes SELECT_ROUND tokens, 64 * SELECT_EACH of them in a row to a wave: one round's weights stay in registers
+// from the first digit to the walk.  A weight moves to an index at or below its own and a round reads its tokens before it writes, so weights_out may be weights.
+constexpr uint32_t SELECT_EACH = 8, SELECT_WAVES = SELECT_BLOCK / 64, SELECT_ROUND = SELECT_BLOCK * SELECT_EACH;
+constexpr uint32_t SELECT_COPIES = 4;            // of the histogram: weights crowd into few digits, and lanes that meet in a bin wait for each other
+
 __global__ void __launch_bounds__(SELECT_BLOCK) evict_select_kernel(EvictArgs a) {
-    __shared__ uint32_t hist[256], ranks[2 * SELECT_BLOCK / 64], digit, above;
-    const uint32_t g = blockIdx.x, b = blockIdx.y, pair = b * a.kv_heads + g, tid = threadIdx.x;
-    int32_t raw = a.lens[b];
+    __shared__ uint32_t hist[2][SELECT_COPIES][256], counts[SELECT_WAVES][2], digit, above;
+    const uint32_t g = blockIdx.x, b = blockIdx.y, pair = b * a.kv_heads + g, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const int32_t raw = a.lens[b];
     const uint32_t len = raw < 0 ? 0 : (uint32_t)raw < a.cap ? (uint32_t)raw : a.cap;
     const float* w = a.weights + (uint64_t)pair * a.cap;
     float* out = a.weights_out + (uint64_t)pair * a.cap;
@@ -107,47 +88,108 @@ __global__ void __launch_bounds__(SELECT_BLOCK) evict_select_kernel(EvictArgs a)
         return;
     }
     const uint32_t lo = a.first, hi = len - a.recent, need = a.keep - a.first - a.recent;      // candidates [lo, hi): more than need
+    const bool once = len <= SELECT_ROUND;
+    float x[SELECT_EACH];
+    const uint32_t mine = wave * (64 * SELECT_EACH) + lane;     // this thread's first token of a round; the others follow 64 apart
+    auto load = [&](uint32_t t0) {
+#pragma unroll
+        for (uint32_t i = 0; i < SELECT_EACH; i++) x[i] = t0 + mine + 64 * i < len ? w[t0 + mine + 64 * i] : 0.0f;
+    };
+    if (once) load(0);
+    hist[0][tid / 256][tid % 256] = 0;
+    __syncthreads();
     uint32_t found = 0, left = need;               // the digits so far; how many of the candidates that share them stay
     if (need)
         for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (uint32_t t = lo + tid; t < hi; t += SELECT_BLOCK) {
-                const uint32_t key = weight_key(w[t]);
-                if (shift == 24 || (key >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1u);
+            uint32_t* h = hist[(shift / 8 + 1) & 1][0];         // digits 3, 2, 1, 0
+            for (uint32_t t0 = 0; t0 < len; t0 += SELECT_ROUND) {
+                if (!once) load(t0);
+#pragma unroll
+                for (uint32_t i = 0; i < SELECT_EACH; i++) {
+                    const uint32_t t = t0 + mine + 64 * i, key = weight_key(x[i]);
+                    if (t >= lo && t < hi && (shift == 24 || (key >> (shift + 8)) == (found >> (shift + 8)))) atomicAdd(&h[(lane % SELECT_COPIES) * 256 + ((key >> shift) & 255)], 1u);
+                }
             }
             __syncthreads();
-            if (tid == 0) {
-                uint32_t sum = 0;
-                int d = 255;
-                for (; d > 0 && sum + hist[d] < left; d--) sum += hist[d];
-                digit = (uint32_t)d;
-                above = sum;
+            if (wave == 0) {                       // lane's digits: 255 - 4 lane and the three below; sums from the top
+                uint32_t n[4], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    n[i] = 0;
+#pragma unroll
+                    for (uint32_t y = 0; y < SELECT_COPIES; y++) n[i] += h[y * 256 + 255 - 4 * lane - i];
+                    sum += n[i];
+                }
+                uint32_t upto = sum;
+#pragma unroll
+                for (int i = 1; i < 64; i <<= 1) {
+                    const uint32_t y = __shfl_up(upto, i);
+                    if ((int)lane >= i) upto += y;
+                }
+                uint32_t before = upto - sum;
+                if (before < left && upto >= left) {            // one lane: the digit is among its four
+                    uint32_t i = 0;
+                    while (i < 3 && before + n[i] < left) before += n[i++];
+                    digit = 255 - 4 * lane - i;
+                    above = before;
+                }
+            } else {                                           // the other one is cleared for the next digit
+                for (uint32_t i = tid - 64; i < SELECT_COPIES * 256; i += SELECT_BLOCK - 64) hist[(shift / 8) & 1][0][i] = 0;
             }
             __syncthreads();
             found |= digit << shift;
             left -= above;
-            __syncthreads();
         }
     // tokens above `found` stay, and the first `left` of those that equal it
     uint32_t at = 0, equal_before = 0;
-    for (uint32_t t0 = 0; t0 < len; t0 += SELECT_BLOCK) {
-        const uint32_t t = t0 + tid;
-        const bool here = t < len, fixed = here && (t < lo || t >= hi), open = here && !fixed && need;
-        const float x = here ? w[t] : 0.0f;
-        const uint32_t key = weight_key(x);
-        const bool more = fixed || (open && key > found), equal = open && key == found;
-        uint32_t r_more, r_equal, n_more, n_equal;
-        block_ranks(more, equal, ranks, r_more, r_equal, n_more, n_equal);
-        // of the equal ones before this thread's, so many stay
-        const uint32_t room = left > equal_before ? left - equal_before : 0;
-        const uint32_t to = at + r_more + (r_equal < room ? r_equal : room);
-        if (more || (equal && r_equal < room)) {
-            kept[to] = t;
-            out[to] = x;
+    for (uint32_t t0 = 0; t0 < len; t0 += SELECT_ROUND) {
+        if (!once) load(t0);
+        uint32_t more_n = 0, equal_n = 0;
+        uint64_t more[SELECT_EACH], equal[SELECT_EACH];
+#pragma unroll
+        for (uint32_t i = 0; i < SELECT_EACH; i++) {
+            const uint32_t t = t0 + mine + 64 * i, key = weight_key(x[i]);
+            const bool fixed = t < len && (t < lo || t >= hi), open = t >= lo && t < hi && need;
+            more[i] = __ballot(fixed || (open && key > found));
+            equal[i] = __ballot(open && key == found);
+            more_n += (uint32_t)__popcll(more[i]);
+            equal_n += (uint32_t)__popcll(equal[i]);
         }
-        at += n_more + (n_equal < room ? n_equal : room);
-        equal_before += n_equal;
+        if (lane == 0) {
+            counts[wave][0] = more_n;
+            counts[wave][1] = equal_n;
+        }
+        __syncthreads();
+        // tokens of waves before this one that stay, and the round's totals
+        uint32_t m = lane < SELECT_WAVES ? counts[lane][0] : 0, q = lane < SELECT_WAVES ? counts[lane][1] : 0;
+#pragma unroll
+        for (int i = 1; i < (int)SELECT_WAVES; i <<= 1) {
+            const uint32_t ym = __shfl_up(m, i), yq = __shfl_up(q, i);
+            if ((int)lane >= i) {
+                m += ym;
+                q += yq;
+            }
+        }
+        uint32_t more_before = wave ? __shfl(m, (int)wave - 1) : 0, equal_at = equal_before + (wave ? __shfl(q, (int)wave - 1) : 0);
+        // equal ones stay while there is room: min(equal ones before, left) of those before a token
+        const uint64_t below = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+        for (uint32_t i = 0; i < SELECT_EACH; i++) {
+            const uint32_t t = t0 + mine + 64 * i, e = equal_at + (uint32_t)__popcll(equal[i] & below);
+            const uint32_t gone_before = equal_before < left ? equal_before : left;            // equal ones that earlier rounds placed: counted in `at`
+            const uint32_t to = at + more_before + (uint32_t)__popcll(more[i] & below) + (e < left ? e : left) - gone_before;
+            if ((more[i] >> lane) & 1 || ((equal[i] >> lane) & 1 && e < left)) {
+                kept[to] = t;
+                out[to] = x[i];
+            }
+            more_before += (uint32_t)__popcll(more[i]);
+            equal_at += (uint32_t)__popcll(equal[i]);
+        }
+        const uint32_t all_more = __shfl(m, (int)SELECT_WAVES - 1), all_equal = __shfl(q, (int)SELECT_WAVES - 1);
+        const uint32_t was = equal_before < left ? equal_before : left;
+        equal_before += all_equal;
+        at += all_more + (equal_before < left ? equal_before : left) - was;
+        __syncthreads();                                        // before the next round's counts, and before it reads what others may write
     }
     if (tid == 0) a.counts[pair] = a.keep;
 }
@@ -161,41 +203,58 @@ struct MoveArgs {
     FastDiv page_div, slice_div;
 };
 
-// A block moves some vectors (a slice) of the rows that stay of one (sequence, KV head), keys or values, `rows` of them; in place it is all rows, in order:
-// a row moves to an index at or below its own, so when a step has read its rows the places it writes hold nothing that a later step reads.
+// A block moves some vectors (a slice) of the rows that stay of one (sequence, KV head), keys or values, `rows` of them, MOVE_EACH a thread and step.  In
+// place it is all rows, in order: a row moves to an index at or below its own, so when a step has read its rows the places it writes hold nothing that a
+// later step reads.  Bound by memory, and in place by the chain list -> table -> row of each step.
+constexpr uint32_t MOVE_EACH = 4;
+
 template <typename VecT> __global__ void __launch_bounds__(BLOCK) evict_move_kernel(MoveArgs a) {
     const uint32_t part = blockIdx.x % (2 * a.slices), pair = blockIdx.x / (2 * a.slices), which = part & 1, slice = part >> 1;
     const uint32_t b = pair / a.kv_heads, g = pair - b * a.kv_heads, count = a.counts[pair];
     if (part == 0 && g == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.lens_out[b] = (int32_t)count;
-    const uint32_t c0 = slice * a.slice_v, width = a.row_v - c0 < a.slice_v ? a.row_v - c0 : a.slice_v;
-    const uint32_t step = BLOCK / a.slice_v, begin = blockIdx.y * a.rows, end = count - begin < a.rows ? count : begin + a.rows;
+    const uint32_t step = BLOCK / a.slice_v, begin = blockIdx.y * a.rows;
     if (begin >= count) return;
+    const uint32_t end = count - begin < a.rows ? count : begin + a.rows;
     VecT* pages = (VecT*)a.pages[which];
     uint32_t r, c;
     fd_divmod(threadIdx.x, a.slice_div, r, c);
+    c += slice * a.slice_v;
+    const bool mine = r < step && c < a.row_v;
     const int32_t* from_table = a.table + (uint64_t)b * a.table_len;
     const int32_t* to_table = a.table_out + (uint64_t)b * a.table_len;
-    for (uint32_t i0 = begin; i0 < end; i0 += step) {
-        const uint32_t i = i0 + r;
-        const bool mine = r < step && c < width && i < end;
-        VecT x = {};
-        uint64_t to = 0, from = 0;
-        bool put = false;
-        if (mine) {
-            uint32_t at, slot;
-            const uint32_t t = a.kept[(uint64_t)pair * a.keep + i];
-            fd_divmod(t, a.page_div, at, slot);
-            const uint32_t src = (uint32_t)from_table[at];
-            from = (((uint64_t)src * a.kv_heads + g) * a.page_len + slot) * a.row_v + c0 + c;
-            fd_divmod(i, a.page_div, at, slot);
-            const uint32_t dst = (uint32_t)to_table[at];
-            to = (((uint64_t)dst * a.kv_heads + g) * a.page_len + slot) * a.row_v + c0 + c;
-            put = dst < a.n_pages && !(src < a.n_pages && from == to);
-            if (put && src < a.n_pages) x = pages[from];
+    const uint32_t* kept = a.kept + (uint64_t)pair * a.keep;
+    for (uint32_t i0 = begin; i0 < end; i0 += step * MOVE_EACH) {
+        VecT x[MOVE_EACH];
+        uint64_t to[MOVE_EACH];
+        bool put[MOVE_EACH];
+        uint32_t t[MOVE_EACH];
+#pragma unroll
+        for (uint32_t k = 0; k < MOVE_EACH; k++) {
+            const uint32_t i = i0 + k * step + r;
+            put[k] = mine && i < end;
+            t[k] = put[k] ? kept[i] : 0;
         }
-        asm volatile("" : "+v"(x));                            // the value has arrived before anyone writes
+#pragma unroll
+        for (uint32_t k = 0; k < MOVE_EACH; k++) {
+            x[k] = VecT{};
+            to[k] = 0;
+            if (!put[k]) continue;
+            uint32_t at, slot;
+            fd_divmod(t[k], a.page_div, at, slot);
+            const uint32_t src = (uint32_t)from_table[at];
+            const uint64_t from = (((uint64_t)src * a.kv_heads + g) * a.page_len + slot) * a.row_v + c;
+            fd_divmod(i0 + k * step + r, a.page_div, at, slot);
+            const uint32_t dst = (uint32_t)to_table[at];
+            to[k] = (((uint64_t)dst * a.kv_heads + g) * a.page_len + slot) * a.row_v + c;
+            put[k] = dst < a.n_pages && !(src < a.n_pages && from == to[k]);
+            if (put[k] && src < a.n_pages) x[k] = pages[from];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < MOVE_EACH; k++) asm volatile("" : "+v"(x[k]));                  // the values have arrived before anyone writes
         __syncthreads();
-        if (put) pages[to] = x;
+#pragma unroll
+        for (uint32_t k = 0; k < MOVE_EACH; k++)
+            if (put[k]) pages[to[k]] = x[k];
     }
 }
 
@@ -281,11 +340,20 @@ int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const 
     m.kept = e.kept; m.counts = e.counts;
     m.n_pages = kv->pages; m.kv_heads = kv->kv_heads; m.page_len = kv->page_len; m.seqs = kv->seqs; m.table_len = kv->table_len; m.keep = keep;
     m.row_v = (uint32_t)((uint64_t)kv->head_dim * elem_bytes / vb);
-    m.slice_v = m.row_v < 4 ? m.row_v : 4;
+    // Elsewhere: whole rows.  In place the rows of a pair cannot be shared out, but their columns can: slices of 64 bytes at least, as many
+    // as give four blocks a CU.
+    const bool in_place = table_out == kv->table;
+    m.slice_v = m.row_v < (uint32_t)BLOCK ? m.row_v : BLOCK;
+    if (in_place)
+        while (m.slice_v > 4 && pairs * 2 * ((m.row_v + m.slice_v - 1) / m.slice_v) < 4ull * dev->num_cus) m.slice_v = (m.slice_v + 1) / 2;
     m.slices = (m.row_v + m.slice_v - 1) / m.slice_v;
     m.page_div = make_fastdiv(kv->page_len);
     m.slice_div = make_fastdiv(m.slice_v);
-    m.rows = table_out == kv->table || keep < 256 ? keep : 256;
+    const uint32_t one_step = BLOCK / m.slice_v * MOVE_EACH;
+    m.rows = one_step;                                          // of a block: one step where that gives no more than eight blocks a CU, as many as it takes otherwise
+    const uint64_t wanted = pairs * 2 * m.slices * keep / (8ull * dev->num_cus);
+    if (wanted > m.rows) m.rows = (uint32_t)((wanted + one_step - 1) / one_step * one_step);
+    if (in_place) m.rows = keep;
     const uint64_t blocks = pairs * 2 * m.slices, chunks = (keep + m.rows - 1) / m.rows;
     RT_REQUIRE(blocks <= 0x7fffffffull && chunks <= 65535, RT_ERR_SIZE, "%s: too many rows", who);
     const dim3 grid((unsigned)blocks, (unsigned)chunks), block(BLOCK);
