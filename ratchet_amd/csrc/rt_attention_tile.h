@@ -23,6 +23,9 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 constexpr uint32_t AT_ROWS = 128, AT_WAVES = 4, AT_BLOCK = 64 * AT_WAVES;
 constexpr uint32_t AT_TARGET = 1024;             // work items that fill the chip: two blocks on each of 256 CUs, twice
 constexpr uint32_t AT_LEAST_TILES = 4;           // tiles that a piece of the keys is worth
+constexpr uint32_t AT_MOST_PIECES = 60;          // of a row tile: their factors for its 128 rows fit the LDS of the smallest tiles
+constexpr uint32_t AT_FEW_ROWS = 16;             // rows of a sequence and KV head, on average, up to which a launch joins its own pieces
+constexpr uint32_t AT_JOIN_ROWS = 16;            // rows to a block of the joining kernel
 
 // ------------------------------------------------------------------------------------------------- who does what
 // Tiles of KT keys that a tile of rows of sequence s may see at most; 1 where there are no keys, for the block that writes the zeros
@@ -54,10 +57,17 @@ template <int KT> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a
     return n < AT_LEAST_TILES ? AT_LEAST_TILES : n > 0x7fffffffu ? 0x7fffffffu : (uint32_t)n;
 }
 
+// ... and in a piece of this sequence's
+__device__ __forceinline__ uint32_t at_piece_of(uint32_t piece, uint32_t span) {
+    const uint32_t least = (span + AT_MOST_PIECES - 1) / AT_MOST_PIECES;
+    return piece > least ? piece : least;
+}
+
 // Sequence b's items are numbered row tile by row tile, at_items of them, after those of the sequences before it.
 template <int KT> __device__ __forceinline__ uint32_t at_items(const AttnArgs& a, uint32_t b, uint32_t piece) {
     const AttnSeq s = at_seq<true>(a, b);
-    return at_row_tiles(a, s) * ((at_span<KT>(a, s) + piece - 1) / piece);
+    const uint32_t span = at_span<KT>(a, s), n = at_piece_of(piece, span);
+    return at_row_tiles(a, s) * ((span + n - 1) / n);
 }
 // The sequence that item `at` belongs to (a.seqs: none); `at` becomes its number there.  All lanes of a wave take part.
 template <int KT> __device__ __forceinline__ uint32_t at_locate(const AttnArgs& a, uint32_t piece, uint32_t& at) {
@@ -252,36 +262,158 @@ __device__ __forceinline__ void at_row_again(const AttnArgs& a, uint32_t b, uint
     l_out = l;
 }
 
+// Where the keys of a row tile are shared out over blocks (pieces), each block leaves its part of the result.  Who joins them:
+//   few rows (single tokens): the block that comes last.  Each counts itself in when its part is written, which for few rows is a few hundred bytes; parts then travel
+//       between blocks of one launch, and each XCD has an L2 of its own, so they are written and read as agent-scope atomics, which go past it, and a
+//       block counts itself in only when its writes have been acknowledged.
+//   many rows: a launch of its own, 16 rows to a block.  The last block alone would read a whole row tile's parts (64 KB each) through one CU.
 struct AttnPartial {
-    float* o;                      // [items * kv heads][AT_ROWS][dim], unnormalised
-    float* ml;                     // [items * kv heads][AT_ROWS][2]: m (of scaled scores, base 2), l
+    float* o;                      // [blocks][AT_ROWS][dim], unnormalised
+    float* ml;                     // [blocks][AT_ROWS][2]: m (of scaled scores, base 2), l
+    uint32_t* arrivals;            // [blocks]: of a row tile's first block
+    uint32_t split;                // 0: each block walks all keys
     uint32_t pieces;               // contiguous: pieces of the keys a row tile is split into, `piece` tiles each
     uint32_t piece;
     uint32_t row_tiles;            // contiguous: of each batch entry
-    uint32_t blocks;               // of the launch: what there are partial results of
 };
 
-template <typename T, int DT, bool EXACT, bool PAGED>
+__device__ __forceinline__ void at_leave(float* to, float x, float y) {
+    const uint64_t both = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+    __hip_atomic_store((uint64_t*)to, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void at_take(const float* from, float& x, float& y) {
+    const uint64_t both = __hip_atomic_load((const uint64_t*)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    x = __uint_as_float((uint32_t)both);
+    y = __uint_as_float((uint32_t)(both >> 32));
+}
+
+// Called by all threads of a block that has left its part.  True in the block that comes last of `used`.
+__device__ __forceinline__ bool at_last(uint32_t* arrivals, uint32_t used, volatile uint32_t* shared) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // this wave's part is where the others will read it
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const bool last = __hip_atomic_fetch_add(arrivals, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == used - 1;
+        *shared = last;
+        if (last) __hip_atomic_store(arrivals, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return *shared != 0;
+}
+
+template <bool ATOMIC> __device__ __forceinline__ void at_put(float* to, float x, float y) {
+    if (ATOMIC) {
+        at_leave(to, x, y);
+    } else {
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        *(v2f*)to = v2f{x, y};
+    }
+}
+template <bool ATOMIC> __device__ __forceinline__ void at_get(const float* from, float& x, float& y) {
+    if (ATOMIC) {
+        at_take(from, x, y);
+    } else {
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        const v2f both = *(const v2f*)from;
+        x = both[0];
+        y = both[1];
+    }
+}
+
+// Joins `used` parts, `stride` blocks apart from block `first` on, of rows r0 .. r1 - 1 of the row tile at row0.  factors: LDS for (r1 - r0) * used floats.
+// First each row's factors 2^(m_k - m) / l, then the sums, eight parts in flight.
+template <typename T, bool ATOMIC>
+__device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& part, const AttnSeq& s, uint32_t b, uint32_t g, uint32_t row0, uint32_t r0, uint32_t r1, uint64_t first,
+                                        uint64_t stride, uint32_t used, float* factors) {
+    const uint32_t D = a.dim, quads = D / 4, n = r1 - r0;
+    // the factors: 16 lanes to a row
+    const uint32_t part_lane = threadIdx.x % 16;
+    for (uint32_t i0 = 0; i0 < n; i0 += AT_BLOCK / 16) {
+        const uint32_t i = i0 + threadIdx.x / 16;
+        float mk[(AT_MOST_PIECES + 15) / 16], lk[(AT_MOST_PIECES + 15) / 16], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (uint32_t u = 0; u < (AT_MOST_PIECES + 15) / 16; u++) {
+            const uint32_t k = part_lane + 16 * u;
+            mk[u] = -INFINITY;
+            lk[u] = 0.0f;
+            if (i < n && k < used) at_get<ATOMIC>(part.ml + 2 * ((first + k * stride) * AT_ROWS + r0 + i), mk[u], lk[u]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < (AT_MOST_PIECES + 15) / 16; u++) m = fmaxf(m, mk[u]);
+#pragma unroll
+        for (int x = 8; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (uint32_t u = 0; u < (AT_MOST_PIECES + 15) / 16; u++) {
+            mk[u] = at_exp2(mk[u] - base);
+            l = __builtin_fmaf(mk[u], lk[u], l);
+        }
+#pragma unroll
+        for (int x = 8; x; x >>= 1) l += __shfl_xor(l, x);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (uint32_t u = 0; u < (AT_MOST_PIECES + 15) / 16; u++)
+            if (i < n && part_lane + 16 * u < used) factors[i * used + part_lane + 16 * u] = mk[u] * inv;
+        if (a.lse && i < n && part_lane == 0) {
+            const uint32_t row = row0 + r0 + i, j = fd_div(row, a.group_div), h = g * a.group + (row - j * a.group);
+            a.lse[b * a.l_b + h * a.l_h + (uint64_t)(s.first + j) * a.l_t] = at_lse(m, l);
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n * quads; i += AT_BLOCK) {
+        const uint32_t r = i / quads, d = (i - r * quads) * 4;
+        const float* from = part.o + (first * AT_ROWS + r0 + r) * D + d;
+        const uint64_t next = stride * AT_ROWS * D;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t k0 = 0; k0 < used; k0 += 8) {
+            float x[8][4];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; u++) {
+                const uint32_t k = k0 + u < used ? k0 + u : used - 1;
+                at_get<ATOMIC>(from + k * next, x[u][0], x[u][1]);
+                at_get<ATOMIC>(from + k * next + 2, x[u][2], x[u][3]);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 8; u++) {
+                const float f = k0 + u < used ? factors[r * used + k0 + u] : 0.0f;
+                if (k0 + u < used)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) o[y] = __builtin_fmaf(f, x[u][y], o[y]);
+            }
+        }
+        const uint32_t row = row0 + r0 + r, j = fd_div(row, a.group_div), h = g * a.group + (row - j * a.group);
+        T* y = (T*)a.y + b * a.y_b + h * a.y_h + (uint64_t)(s.first + j) * a.y_t + d;
+        if constexpr (sizeof(T) == 2) {
+            *(v2u*)y = v2u{AtMma<T>::pack(o[0], o[1]), AtMma<T>::pack(o[2], o[3])};
+        } else {
+            typedef float v4f __attribute__((ext_vector_type(4)));
+            *(v4f*)y = v4f{o[0], o[1], o[2], o[3]};
+        }
+    }
+}
+
+// FEW: pieces are joined by the block that comes last
+template <typename T, int DT, bool EXACT, bool PAGED, bool FEW>
 __global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) attention_tile_kernel(AttnArgs a, AttnPartial part) {
     typedef AtShape<T, DT> S;
     constexpr int KT = S::KT, CE = S::CE;
-    extern __shared__ unsigned char smem[];
+    extern __shared__ __align__(16) unsigned char smem[];
     lds_byte* const lds = (lds_byte*)smem;
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
     const uint32_t D = EXACT ? DT : a.dim, chunks = D / CE, pitch = D * sizeof(T);
 
     // ---- which rows, which keys
-    uint32_t b, g, tile, piece_at, piece;
+    uint32_t b, g, tile, piece_at, piece, stride;               // stride: in blocks, from piece to piece of a row tile
     if (PAGED) {
+        stride = a.kv_heads;
         g = blockIdx.x % a.kv_heads;
         uint32_t at = blockIdx.x / a.kv_heads;
-        piece = __builtin_amdgcn_readfirstlane(at_piece<KT>(a));
+        piece = part.split ? __builtin_amdgcn_readfirstlane(at_piece<KT>(a)) : 0x7fffffffu;
         b = __builtin_amdgcn_readfirstlane(at_locate<KT>(a, piece, at));
         if (b >= a.seqs) return;
         tile = __builtin_amdgcn_readfirstlane(at);
         piece_at = 0;
     } else {
-        const uint32_t pairs = a.seqs * a.kv_heads, pair = blockIdx.x % pairs, at = blockIdx.x / pairs;
+        const uint32_t pairs = stride = a.seqs * a.kv_heads, pair = blockIdx.x % pairs, at = blockIdx.x / pairs;
         b = pair / a.kv_heads;
         g = pair - b * a.kv_heads;
         piece = part.piece;
@@ -290,7 +422,9 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) 
     }
     const AttnSeq s = at_seq<PAGED>(a, b);
     if (PAGED) {
-        const uint32_t pieces = (at_span<KT>(a, s) + piece - 1) / piece, at = tile;
+        const uint32_t span = at_span<KT>(a, s), at = tile;
+        piece = at_piece_of(piece, span);
+        const uint32_t pieces = (span + piece - 1) / piece;
         tile = at / pieces;
         piece_at = at - tile * pieces;
         tile = at_row_tiles(a, s) - 1 - tile;
@@ -300,6 +434,8 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) 
     const uint32_t tile0 = piece_at * piece, tile1 = w.tiles - tile0 < piece || tile0 >= w.tiles ? w.tiles : tile0 + piece;
     const bool whole = w.tiles <= piece;                        // no other block has keys of these rows
     if (tile0 >= w.tiles && piece_at > 0) return;
+    // Starts that decrease can count more items than there are blocks: a row tile whose pieces are not all there is left alone (its counter would stay up).
+    if (!whole && blockIdx.x + (uint64_t)((w.tiles + piece - 1) / piece - 1 - piece_at) * stride >= gridDim.x) return;
 
     // ---- this lane's row
     const uint32_t r = wave * 32 + col, row = row0 + (r < rows ? r : rows - 1);
@@ -502,11 +638,9 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) 
         const uint32_t stage = (n - tile0) & 1;
         step(n, lds + (stage ^ 1) * 2 * S::TILE, lds + stage * 2 * S::TILE);
     }
-    if (!busy) return;
 
     // ---- result: lane's columns of d are 32 i + 8 (e / 4) + 4 half + e % 4
     l += at_other(l);
-    const uint64_t out = (uint64_t)blockIdx.x * AT_ROWS + r;    // of the partial results
     bool fine = __builtin_isfinite(l) && m < INFINITY;
 #pragma unroll
     for (int i = 0; i < S::BLOCKS; i++)
@@ -519,27 +653,20 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) 
             float oo[(DT + 63) / 64], mm, ll;
             at_row_again<T, DT, PAGED, KT>(a, b, g, s, w, tile0, tile1, row0 + rr, oo, mm, ll);
             const uint32_t jj = fd_div(row0 + rr, a.group_div), hh = g * a.group + (row0 + rr - jj * a.group);
-            const uint64_t slot_at = (uint64_t)blockIdx.x * AT_ROWS + rr;
-            const float inv = whole ? (ll == 0.0f ? 0.0f : 1.0f / ll) : 1.0f;
+            const uint64_t part_at = (uint64_t)blockIdx.x * AT_ROWS + rr;
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
             T* y = (T*)a.y + b * a.y_b + hh * a.y_h + (uint64_t)(s.first + jj) * a.y_t;
-            for (uint32_t i = 0; i < (DT + 63) / 64; i++)
-                if (i * 64 + lane < D) {
-                    if (whole) y[i * 64 + lane] = Ar<T>::conv(oo[i] * inv);
-                    else part.o[slot_at * D + i * 64 + lane] = oo[i];
-                }
-            if (lane == 0) {
-                if (!whole) {
-                    part.ml[2 * slot_at] = mm;
-                    part.ml[2 * slot_at + 1] = ll;
-                } else if (a.lse) {
-                    a.lse[b * a.l_b + hh * a.l_h + (uint64_t)(s.first + jj) * a.l_t] = at_lse(mm, ll);
-                }
+#pragma unroll
+            for (uint32_t i = 0; i < (DT + 63) / 64; i++) {
+                const float next = __shfl_down(oo[i], 1);
+                if (i * 64 + lane >= D) continue;
+                if (whole) y[i * 64 + lane] = Ar<T>::conv(oo[i] * inv);
+                else if (lane % 2 == 0) at_put<FEW>(part.o + part_at * D + i * 64 + lane, oo[i], next);
             }
+            if (lane == 0 && !whole) at_put<FEW>(part.ml + 2 * part_at, mm, ll);
+            if (lane == 0 && whole && a.lse) a.lse[b * a.l_b + hh * a.l_h + (uint64_t)(s.first + jj) * a.l_t] = at_lse(mm, ll);
         }
-        return;
-    }
-    if (r >= rows) return;
-    if (whole) {
+    } else if (r < rows && whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         T* y = (T*)a.y + b * a.y_b + h * a.y_h + (uint64_t)(s.first + j) * a.y_t;
 #pragma unroll
@@ -557,95 +684,82 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) 
                 }
             }
         if (a.lse && half == 0) a.lse[b * a.l_b + h * a.l_h + (uint64_t)(s.first + j) * a.l_t] = at_lse(m, l);
-    } else {
-        typedef float v4f __attribute__((ext_vector_type(4)));
+    } else if (r < rows) {
+        const uint64_t part_at = (uint64_t)blockIdx.x * AT_ROWS + r;
 #pragma unroll
         for (int i = 0; i < S::BLOCKS; i++)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const uint32_t d = 32 * i + 8 * (e / 4) + 4 * half;
-                if (d < D) *(v4f*)(part.o + out * D + d) = v4f{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+                if (d >= D) continue;
+                if (FEW) {
+                    at_leave(part.o + part_at * D + d, o[i][e], o[i][e + 1]);
+                    at_leave(part.o + part_at * D + d + 2, o[i][e + 2], o[i][e + 3]);
+                } else {
+                    typedef float v4f __attribute__((ext_vector_type(4)));
+                    *(v4f*)(part.o + part_at * D + d) = v4f{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+                }
             }
-        if (half == 0) {
-            part.ml[2 * out] = m;
-            part.ml[2 * out + 1] = l;
-        }
+        if (half == 0) at_put<FEW>(part.ml + 2 * part_at, m, l);
     }
+    if (!FEW || whole) return;
+    const uint32_t used = (w.tiles + piece - 1) / piece, first = blockIdx.x - piece_at * stride;
+    if (at_last(part.arrivals + first, used, (volatile uint32_t*)(smem + S::LDS - 16)))
+        at_join<T, true>(a, part, s, b, g, row0, 0, rows, first, stride, used, (float*)smem);
 }
 
-// Joins the pieces of rows whose keys several blocks walked: a wave to a (token, head) row.
-template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_BLOCK) attention_join_kernel(AttnArgs a, AttnPartial part, uint64_t rows_all) {
-    const uint32_t lane = threadIdx.x % 64, D = a.dim;
-    const uint64_t id = (uint64_t)blockIdx.x * AT_WAVES + threadIdx.x / 64;
-    if (id >= rows_all) return;
-    const uint32_t h = (uint32_t)(id % a.heads), g = h / a.group;
-    const uint64_t token = id / a.heads;
-    uint32_t b, j, piece, pieces, first;
+// blockIdx.y: which AT_JOIN_ROWS of a row tile.  blockIdx.x: paged: KV head, sequence and row tile of it, a row tile having more than one piece; contiguous: as the tiles' blocks
+template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_BLOCK) attention_join_kernel(AttnArgs a, AttnPartial part, uint32_t tile_blocks) {
+    __shared__ float factors[AT_JOIN_ROWS * AT_MOST_PIECES];
+    uint32_t b, g, tile, piece, pieces;
+    uint64_t first, stride;
     AttnSeq s;
     if (PAGED) {
-        b = at_find(a.starts, a.seqs, (uint32_t)token);
-        if (b == a.seqs) return;
+        // numbered as the items are, with one piece a row tile
+        g = blockIdx.x % a.kv_heads;
+        uint32_t at = blockIdx.x / a.kv_heads;
+        b = __builtin_amdgcn_readfirstlane(at_locate<KT>(a, 0x7fffffffu, at));
+        if (b >= a.seqs) return;
         s = at_seq<true>(a, b);
-        if (token < s.first || token - s.first >= s.count) return;
-        j = (uint32_t)token - s.first;
-        piece = at_piece<KT>(a);
+        tile = __builtin_amdgcn_readfirstlane(at);
+        const uint32_t span = at_span<KT>(a, s), all = __builtin_amdgcn_readfirstlane(at_piece<KT>(a));
+        piece = at_piece_of(all, span);
+        pieces = (span + piece - 1) / piece;
+        if (pieces == 1) return;
+        stride = a.kv_heads;
+        first = (__builtin_amdgcn_readfirstlane(at_before<KT>(a, all, b)) + (uint64_t)(at_row_tiles(a, s) - 1 - tile) * pieces) * stride + g;
     } else {
-        b = (uint32_t)(token / a.tokens);
-        j = (uint32_t)(token % a.tokens);
+        stride = (uint64_t)a.seqs * a.kv_heads;
+        const uint32_t pair = (uint32_t)(blockIdx.x % stride);
+        b = pair / a.kv_heads;
+        g = pair - b * a.kv_heads;
+        tile = (uint32_t)(blockIdx.x / stride);
         s = at_seq<false>(a, b);
         piece = part.piece;
+        first = (uint64_t)(part.row_tiles - 1 - tile) * part.pieces * stride + pair;
     }
-    const uint32_t row = j * a.group + (h - g * a.group), tile = row / AT_ROWS, all = s.count * a.group;
-    const AttnWalk w = at_walk<KT>(a, s, tile * AT_ROWS, all - tile * AT_ROWS < AT_ROWS ? all - tile * AT_ROWS : AT_ROWS);
-    if (w.tiles <= piece) return;
+    const uint32_t all_rows = s.count * a.group, row0 = tile * AT_ROWS, rows = all_rows - row0 < AT_ROWS ? all_rows - row0 : AT_ROWS;
+    const AttnWalk w = at_walk<KT>(a, s, row0, rows);
+    const uint32_t r0 = blockIdx.y * AT_JOIN_ROWS, r1 = r0 + AT_JOIN_ROWS < rows ? r0 + AT_JOIN_ROWS : rows;
+    if (w.tiles <= piece || r0 >= rows) return;
     const uint32_t used = (w.tiles + piece - 1) / piece;
-    uint64_t stride;
-    if (PAGED) {
-        pieces = (at_span<KT>(a, s) + piece - 1) / piece;
-        first = (at_before<KT>(a, piece, b) + (at_row_tiles(a, s) - 1 - tile) * pieces) * a.kv_heads + g;
-        stride = a.kv_heads;
-    } else {
-        first = (part.row_tiles - 1 - tile) * part.pieces * a.seqs * a.kv_heads + b * a.kv_heads + g;
-        stride = (uint64_t)a.seqs * a.kv_heads;
-    }
-    if (first + (used - 1) * stride >= part.blocks) return;    // rows counted more than once: starts that decrease
-    const uint32_t r = row - tile * AT_ROWS;
-    float m = -INFINITY;
-    for (uint32_t i = lane; i < used; i += 64) m = fmaxf(m, part.ml[2 * ((first + i * stride) * AT_ROWS + r)]);
-#pragma unroll
-    for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t i = 0; i < used; i++) {
-        const uint64_t at = (first + i * stride) * AT_ROWS + r;
-        const float e = at_exp2(part.ml[2 * at] - base);
-        l = __builtin_fmaf(e, part.ml[2 * at + 1], l);
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (k * 64 + lane < D) o[k] = __builtin_fmaf(e, part.o[at * D + k * 64 + lane], o[k]);
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* y = (T*)a.y + b * a.y_b + h * a.y_h + (uint64_t)(s.first + j) * a.y_t;
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-        if (k * 64 + lane < D) y[k * 64 + lane] = Ar<T>::conv(o[k] * inv);
-    if (a.lse && lane == 0) a.lse[b * a.l_b + h * a.l_h + (uint64_t)(s.first + j) * a.l_t] = at_lse(m, l);
+    if (first + (used - 1) * stride >= tile_blocks) return;     // as in the tiles' kernel: starts that decrease
+    at_join<T, false>(a, part, s, b, g, row0, r0, r1, first, stride, used, factors);
 }
 
 template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_device* dev, AttnArgs& a) {
     typedef AtShape<T, DT> S;
     AttnPartial part = {};
-    uint64_t items, rows_all;                                   // blocks per KV head (paged) or per (batch entry, KV head)
+    uint64_t join_tiles, items;                                 // row tiles; blocks per KV head (paged) or per (batch entry, KV head)
     const uint64_t per = PAGED ? a.kv_heads : (uint64_t)a.seqs * a.kv_heads;
-    bool split;
     if (PAGED) {
-        rows_all = (uint64_t)a.tokens * a.heads;
         const uint64_t tiles = ((uint64_t)a.tokens * a.group) / AT_ROWS + a.seqs;
         // sum over the row tiles of ceil(span / piece): at most AT_TARGET / kv_heads + 1 and one for each row tile
-        split = a.cap > AT_LEAST_TILES * S::KT;
-        items = tiles + (split ? AT_TARGET / a.kv_heads + 1 : 0);
+        items = tiles + AT_TARGET / a.kv_heads + 1;
+        part.split = a.cap > AT_LEAST_TILES * S::KT && items * per <= RT_ARRIVALS;
+        if (!part.split) items = tiles;
+        join_tiles = tiles * per;
     } else {
-        rows_all = (uint64_t)a.seqs * a.tokens * a.heads;
         part.row_tiles = (uint32_t)(((uint64_t)a.tokens * a.group + AT_ROWS - 1) / AT_ROWS);
         uint64_t span = (a.cap + S::KT - 1) / S::KT;
         if (a.window != AT_FAR) {
@@ -653,33 +767,37 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
             span = w < span ? w : span;
         }
         uint64_t piece = (span * part.row_tiles * per + AT_TARGET - 1) / AT_TARGET;
+        const uint64_t least = (span + AT_MOST_PIECES - 1) / AT_MOST_PIECES;
         piece = piece < AT_LEAST_TILES ? AT_LEAST_TILES : piece;
+        piece = piece < least ? least : piece;
+        if (part.row_tiles * ((span + piece - 1) / piece) * per > RT_ARRIVALS) piece = span;
         part.piece = (uint32_t)piece;
         part.pieces = (uint32_t)((span + piece - 1) / piece);
-        split = part.pieces > 1;
+        part.split = part.pieces > 1;
         items = (uint64_t)part.row_tiles * part.pieces;
+        join_tiles = part.row_tiles * per;
     }
     const uint64_t blocks = items * per;
-    RT_REQUIRE(blocks <= 0x7fffffffull && (rows_all + AT_WAVES - 1) / AT_WAVES <= 0x7fffffffull, RT_ERR_SIZE, "attention: too many rows");
-    part.blocks = (uint32_t)blocks;
-    const size_t row_count = split ? (size_t)blocks * AT_ROWS : 0;
+    RT_REQUIRE(blocks <= 0x7fffffffull, RT_ERR_SIZE, "attention: too many rows");
+    const size_t row_count = part.split ? (size_t)blocks * AT_ROWS : 0;
     void* p = nullptr;
     int rc = at_workspace(dev, a, row_count * ((size_t)a.dim + 2) * sizeof(float), &p);
     if (rc) return rc;
     part.ml = (float*)p;
     part.o = part.ml + 2 * row_count;
-    const auto kernel = attention_tile_kernel<T, DT, EXACT, PAGED>;
-    const size_t lds = S::LDS;
-    static_assert(S::LDS <= 160 * 1024, "LDS");
-    static bool raised[16] = {};                                // per GPU; setting it twice does no harm
-    if (lds > 64 * 1024 && !(dev->ordinal < 16 && raised[dev->ordinal])) {
-        RT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        if (dev->ordinal < 16) raised[dev->ordinal] = true;
+    part.arrivals = dev->arrivals;
+    const bool few = part.split && (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
+    const auto kernel = few ? attention_tile_kernel<T, DT, EXACT, PAGED, true> : attention_tile_kernel<T, DT, EXACT, PAGED, false>;
+    static_assert(S::LDS <= 160 * 1024 && AT_MOST_PIECES * AT_ROWS * 4 <= S::LDS - 16, "LDS");
+    static bool raised[2][16] = {};                             // per GPU; setting it twice does no harm
+    if (S::LDS > 64 * 1024 && !(dev->ordinal < 16 && raised[few][dev->ordinal])) {
+        RT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
+        if (dev->ordinal < 16) raised[few][dev->ordinal] = true;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(AT_BLOCK), lds, dev->stream, a, part);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(AT_BLOCK), S::LDS, dev->stream, a, part);
     RT_CHECK_LAUNCH("attention_tile_kernel");
-    if (split) {
-        hipLaunchKernelGGL((attention_join_kernel<T, S::KT, PAGED>), dim3((unsigned)((rows_all + AT_WAVES - 1) / AT_WAVES)), dim3(AT_BLOCK), 0, dev->stream, a, part, rows_all);
+    if (part.split && !few) {
+        hipLaunchKernelGGL((attention_join_kernel<T, S::KT, PAGED>), dim3((unsigned)join_tiles, AT_ROWS / AT_JOIN_ROWS), dim3(AT_BLOCK), 0, dev->stream, a, part, (uint32_t)blocks);
         RT_CHECK_LAUNCH("attention_join_kernel");
     }
     return RT_OK;

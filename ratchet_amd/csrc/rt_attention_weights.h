@@ -36,7 +36,7 @@ template <typename T, int DT, bool EXACT>
 __global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : 2) attention_weights_kernel(AttnArgs a, const float* weights, float* out) {
     typedef AtShape<T, DT> S;
     constexpr int CE = S::CE;
-    extern __shared__ unsigned char smem[];
+    extern __shared__ __align__(16) unsigned char smem[];
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
     const uint32_t D = EXACT ? DT : a.dim, chunks = D / CE, pitch = D * sizeof(T);
     constexpr uint32_t PART = (32 * S::CHUNKS * 16 + 1023) / 1024 * 1024;       // a wave's keys in LDS

@@ -209,12 +209,21 @@ int rt_device_create(int ordinal, rt_device** out) {
         e = hipMemset(dev->sm_mask_tiles, 0xff, RT_SM_TILES_HEAD * sizeof(uint32_t));
         if (e != hipSuccess) (void)hipFree(dev->sm_mask_tiles);
     }
+    if (e == hipSuccess) {
+        e = hipMalloc((void**)&dev->arrivals, RT_ARRIVALS * sizeof(uint32_t));
+        if (e == hipSuccess) {
+            e = hipMemset(dev->arrivals, 0, RT_ARRIVALS * sizeof(uint32_t));
+            if (e == hipSuccess) e = hipStreamSynchronize(nullptr);              // the device's stream does not wait for the one the fill ran on
+            if (e != hipSuccess) (void)hipFree(dev->arrivals);
+        }
+        if (e != hipSuccess) (void)hipFree(dev->sm_mask_tiles);
+    }
     if (e != hipSuccess) {
         (void)hipFree(dev->gn_scratch);
         (void)hipStreamDestroy(dev->stream);
         delete dev->pool;
         delete dev;
-        return rt_fail_hip(e, "hipMalloc(mask tiles)");
+        return rt_fail_hip(e, "hipMalloc(mask tiles, arrivals)");
     }
     int rc = rt_norm_device_init(dev);
     if (rc == RT_OK && hipHostMalloc(&dev->pool->host, RT_HOST_BYTES, hipHostMallocDefault) != hipSuccess) {
@@ -222,6 +231,7 @@ int rt_device_create(int ordinal, rt_device** out) {
         dev->pool->host = nullptr;
     }
     if (rc) {
+        (void)hipFree(dev->arrivals);
         (void)hipFree(dev->sm_mask_tiles);
         (void)hipFree(dev->gn_scratch);
         (void)hipStreamDestroy(dev->stream);
@@ -246,6 +256,7 @@ int rt_device_destroy(rt_device* dev) {
         }
     if (dev->gn_scratch) (void)hipFree(dev->gn_scratch);
     if (dev->sm_mask_tiles) (void)hipFree(dev->sm_mask_tiles);
+    if (dev->arrivals) (void)hipFree(dev->arrivals);
     if (dev->scratch) (void)hipFree(dev->scratch);
     while (dev->retired) {
         rt_retired* next = dev->retired->next;

@@ -20,6 +20,8 @@ constexpr size_t RT_SM_TILES_HEAD = 16;         // entries in front of them that
 // L2 at all ([1,32,4096,4096] 338 against 440 us, [1,8,6144,6144] 206 against 244).
 constexpr uint64_t RT_XCD_ORDER_MIN_BYTES = 28ull << 20;
 
+constexpr uint32_t RT_ARRIVALS = 1u << 16;
+
 struct rt_device {
     int ordinal;
     hipStream_t stream;
@@ -56,6 +58,7 @@ struct rt_device {
     int scratch_recorded;          // a recorded graph uses this block: it is not freed before the device
     int capture_used_scratch;      // the capture that is running has asked for it
     struct rt_retired* retired;    // outgrown blocks that graphs still use
+    uint32_t* arrivals;            // RT_ARRIVALS counters, 0 between the calls: the blocks that share a result count themselves in, and the last one sets 0 again
 };
 
 struct rt_event {
