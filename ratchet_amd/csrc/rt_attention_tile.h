@@ -142,9 +142,10 @@ template <> struct AtMma<bf16_t> {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, k), __builtin_bit_cast(v8b, q), s, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
-        uint32_t r;
-        asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
-        return r;
+        // not written as an instruction: one that reads an exponential has to keep a state away from it, which the compiler sees to only for its own
+        typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{x, y}), v2b));
     }
     static constexpr uint32_t SIGNS = 0x80008000u;
 };
@@ -165,10 +166,13 @@ __device__ __forceinline__ float at_lds4(const lds_byte* at) { return *(const __
 __device__ __forceinline__ v2u at_lds_turned(const lds_byte* at) {
     return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)const_cast<lds_byte*>(at)));
 }
-// 16 bytes a lane from memory to LDS: lane i's to at + 16 i
+// 16 bytes a lane from memory to LDS, lane i's to at + 16 i (at: the same in all lanes).  Whoever reads them waits for vmcnt(0) first.  Written as an instruction, which
+// has no result the compiler could misplace: after the builtin the compiler holds every LDS read for a possible flat access in flight, and waits
+// for all reads where it needs one (s_waitcnt lgkmcnt(0) before each product).
 __device__ __forceinline__ void at_to_lds(const void* from, lds_byte* at) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)from, (__attribute__((address_space(3))) void*)at, 16, 0, 0);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"((uint32_t)(uintptr_t)at) : "memory");
 }
+__device__ __forceinline__ void at_wait_memory() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // x and the other half's value of the same column
 __device__ __forceinline__ float at_other(float x) {
     typedef unsigned int v2 __attribute__((ext_vector_type(2)));
@@ -189,6 +193,7 @@ template <typename T, int DT> struct AtShape {
     // a wave's last load of a tile may reach beyond it, and so may the transposed reads of the last block of columns
     static constexpr int TILE = (KT * CHUNKS * 16 + 1023) / 1024 * 1024;
     static constexpr int LDS = 4 * TILE + 256;
+    static constexpr int WAVES = DT > 128 ? 1 : 2;             // of a SIMD: what its registers are shared by
 };
 
 // 16-byte chunks of a row are rotated by an amount that goes by the row, so that what the lanes of one access read spreads over the banks: keys are read a
@@ -202,6 +207,10 @@ template <typename T> __device__ __forceinline__ uint32_t at_turn_v(uint32_t row
     const uint32_t z = chunks % 16 == 0 ? 3 : chunks % 8 == 0 ? 2 : chunks % 4 == 0 ? 1 : 0;
     return 2 * ((row & 7) >> (3 - z));
 }
+
+// Left to itself the compiler reads an operand from LDS, waits for it and multiplies, one at a time.  A step is therefore written in the order it runs in: reads
+// some products in front of their uses, the next keys' exponentials between the products of the last, and a fence for the scheduler after each product.
+__device__ __forceinline__ void at_in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // One row over the keys of tiles [tile0, tile1) of a walk, a lane to a key for the scores and to columns for the result: visible keys alone are touched.
 template <typename T, int DT, bool PAGED, int KT>
@@ -289,7 +298,7 @@ __device__ __forceinline__ void at_take(const float* from, float& x, float& y) {
 
 // Called by all threads of a block that has left its part.  True in the block that comes last of `used`.
 __device__ __forceinline__ bool at_last(uint32_t* arrivals, uint32_t used, volatile uint32_t* shared) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // this wave's part is where the others will read it
+    at_wait_memory();                                              // this wave's part is where the others will read it
     __syncthreads();
     if (threadIdx.x == 0) {
         const bool last = __hip_atomic_fetch_add(arrivals, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == used - 1;
@@ -393,7 +402,7 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
 
 // FEW: pieces are joined by the block that comes last
 template <typename T, int DT, bool EXACT, bool PAGED, bool FEW>
-__global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) attention_tile_kernel(AttnArgs a, AttnPartial part) {
+__global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES, AtShape<T, DT>::WAVES))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
     typedef AtShape<T, DT> S;
     constexpr int KT = S::KT, CE = S::CE;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -536,31 +545,46 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) 
     for (int i = 0; i < S::BLOCKS; i++) o[i] = v16f{0};
     float m = -INFINITY, l = 0.0f;                              // l: of this lane's half of the keys
 
-    int32_t page = 0;
-    uint32_t slot = 0;
-    uint64_t there = ~0ull;                                     // keys of the tile at hand that have a page
+    int32_t page = 0, page2 = 0;                                // of the next tile, and of the one after it
+    uint32_t slot = 0, slot2 = 0;
+    uint64_t there = ~0ull, there2 = ~0ull;                     // keys of the tile at hand that have a page, and of the next
     if (tile0 < tile1) {
-        if (PAGED) page = look(tile0, slot);
+        if (PAGED) {
+            page = look(tile0, slot);
+            there2 = __ballot(page >= 0);
+        }
         fetch(tile0, lds, page, slot);
+        if (PAGED && tile0 + 1 < tile1) page = look(tile0 + 1, slot);
     }
-    // One tile: the loads of the next one go into `next` while this one is read from `cur`.  The two never overlap, which is what lets the compiler
-    // leave the loads in flight: the wait for them stands at the top of the next step.
-    auto step = [&](uint32_t n, lds_byte* __restrict next, const lds_byte* __restrict cur) __attribute__((always_inline)) {
+    // One tile: the loads of the next one go into `next` while this one is read from `cur`.  The wait for them stands at the top of the next step.
+    auto step = [&](uint32_t n, lds_byte* next, const lds_byte* cur) __attribute__((always_inline)) {
         if (n + 1 < tile1) fetch(n + 1, next, page, slot);
+        if (PAGED && n + 2 < tile1) page2 = look(n + 2, slot2);                 // arrives while this tile is worked on
         const int32_t t0 = start_of(n);
         if (!busy || t0 > limit_z || (t0 >= a.sinks && p_a - (t0 + KT - 1) >= a.window)) return;
 
+        constexpr int N = S::STEPS * S::HALVES, AHEAD = N < 4 ? N : 4;
         v16f x[S::HALVES];
 #pragma unroll
-        for (int kk = 0; kk < S::HALVES; kk++) {
-            x[kk] = v16f{0};
+        for (int kk = 0; kk < S::HALVES; kk++) x[kk] = v16f{0};
+        v4u k[N];
+        auto read_k = [&](int at) __attribute__((always_inline)) {              // product `at`: step at / HALVES of half at % HALVES
+            const int i = at / S::HALVES, kk = at % S::HALVES;
+            if (!EXACT && (uint32_t)(2 * i * CE) >= D) return;
+            k[at] = at_lds16(cur + (k_at[i] + kk * 32 * pitch));
+        };
 #pragma unroll
-            for (int i = 0; i < S::STEPS; i++) {
-                if (!EXACT && (uint32_t)(2 * i * CE) >= D) break;
-                v4u k = at_lds16(cur + (k_at[i] + kk * 32 * pitch));
-                if ((EXACT ? DT % (2 * CE) != 0 : true) && (2 * i + 2) * CE > (int)D && half) k = v4u{0, 0, 0, 0};
-                x[kk] = AtMma<T>::qk(k, q[i], x[kk]);
+        for (int at = 0; at < AHEAD; at++) read_k(at);
+        at_in_order();
+#pragma unroll
+        for (int at = 0; at < N; at++) {
+            const int i = at / S::HALVES, kk = at % S::HALVES;
+            if (EXACT || (uint32_t)(2 * i * CE) < D) {
+                if ((EXACT ? DT % (2 * CE) != 0 : true) && (2 * i + 2) * CE > (int)D && half) k[at] = v4u{0, 0, 0, 0};
+                x[kk] = AtMma<T>::qk(k[at], q[i], x[kk]);
             }
+            if (at + AHEAD < N) read_k(at + AHEAD);
+            at_in_order();
         }
         if (t0 + KT - 1 > limit_a || (t0 + KT > a.sinks && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
             // key 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile
@@ -591,52 +615,75 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 && sizeof(T) == 4 ? 1 : 2) 
                 for (int e = 0; e < 16; e++) o[i][e] *= old;
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f;
+        if constexpr (sizeof(T) == 2) {
+            constexpr int GROUPS = 2 * S::HALVES, P = GROUPS * S::BLOCKS, FRONT = 4;           // groups of 16 keys
+            v4u v[P], w[GROUPS];
+            auto read_v = [&](int at) __attribute__((always_inline)) {          // product `at`: columns at % BLOCKS of group at / BLOCKS
+                const int i = at % S::BLOCKS, u = at / S::BLOCKS;
+                if (!EXACT && (uint32_t)(32 * i) >= D) return;
+                const uint32_t from = v_at[i] + 16 * u * pitch;
+                const v2u lo = at_lds_turned(cur + from), hi = at_lds_turned(cur + (from + 8 * pitch));
+                v[at] = v4u{lo[0], lo[1], hi[0], hi[1]};
+            };
+            auto weigh = [&](int u, int e) __attribute__((always_inline)) {     // weights 2e, 2e + 1 of group u's 8 in this lane
+                const float w0 = at_exp2(__builtin_fmaf(x[u / 2][8 * (u % 2) + 2 * e], c, -base)), w1 = at_exp2(__builtin_fmaf(x[u / 2][8 * (u % 2) + 2 * e + 1], c, -base));
+                l += w0 + w1;
+                w[u][e] = AtMma<T>::pack(w0, w1);
+            };
 #pragma unroll
-        for (int kk = 0; kk < S::HALVES; kk++)
+            for (int at = 0; at < FRONT; at++) read_v(at);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                x[kk][e] = at_exp2(__builtin_fmaf(x[kk][e], c, -base));
-                sum += x[kk][e];
+            for (int e = 0; e < 4; e++) weigh(0, e);
+            at_in_order();
+#pragma unroll
+            for (int at = 0; at < P; at++) {
+                const int i = at % S::BLOCKS, u = at / S::BLOCKS;
+                if (EXACT || (uint32_t)(32 * i) < D) o[i] = AtMma<T>::qk(v[at], w[u], o[i]);
+                if (at + FRONT < P) read_v(at + FRONT);
+                if (u + 1 < GROUPS)
+#pragma unroll
+                    for (int e = 4 * i / S::BLOCKS; e < 4 * (i + 1) / S::BLOCKS; e++) weigh(u + 1, e);
+                at_in_order();
             }
-        l += sum;
+        } else {
+            constexpr int P = 16 * S::HALVES * S::BLOCKS, FRONT = 8;
+            float v[P], w[16 * S::HALVES];
+            auto read_v = [&](int at) __attribute__((always_inline)) {          // product `at`: columns at % BLOCKS of the two keys of register at / BLOCKS
+                const int i = at % S::BLOCKS, e = at / S::BLOCKS;
+                if (!EXACT && (uint32_t)(32 * i) >= D) return;
+                v[at] = at_lds4(cur + (v_at[i] + (32 * (e / 16) + e % 4 + 8 * (e % 16 / 4)) * pitch));
+            };
+            auto weigh = [&](int e) __attribute__((always_inline)) {
+                w[e] = at_exp2(__builtin_fmaf(x[e / 16][e % 16], c, -base));
+                l += w[e];
+            };
 #pragma unroll
-        for (int kk = 0; kk < S::HALVES; kk++) {
-            if constexpr (sizeof(T) == 2) {
+            for (int at = 0; at < FRONT; at++) read_v(at);
+            weigh(0);
+            at_in_order();
 #pragma unroll
-                for (int u = 0; u < 2; u++) {                   // 16 keys at a time
-                    v4u w8;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w8[e] = AtMma<T>::pack(x[kk][8 * u + 2 * e], x[kk][8 * u + 2 * e + 1]);
-#pragma unroll
-                    for (int i = 0; i < S::BLOCKS; i++) {
-                        if (!EXACT && (uint32_t)(32 * i) >= D) break;
-                        const uint32_t at = v_at[i] + (32 * kk + 16 * u) * pitch;
-                        const v2u lo = at_lds_turned(cur + at), hi = at_lds_turned(cur + (at + 8 * pitch));
-                        o[i] = AtMma<T>::qk(v4u{lo[0], lo[1], hi[0], hi[1]}, w8, o[i]);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-#pragma unroll
-                    for (int i = 0; i < S::BLOCKS; i++) {
-                        if (!EXACT && (uint32_t)(32 * i) >= D) break;
-                        const float v = at_lds4(cur + (v_at[i] + (32 * kk + e % 4 + 8 * (e / 4)) * pitch));
-                        o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x[kk][e], o[i], 0, 0, 0);
-                    }
+            for (int at = 0; at < P; at++) {
+                const int i = at % S::BLOCKS, e = at / S::BLOCKS;
+                if (EXACT || (uint32_t)(32 * i) < D) o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[at], w[e], o[i], 0, 0, 0);
+                if (at + FRONT < P) read_v(at + FRONT);
+                if (i == 0 && e + 1 < 16 * S::HALVES) weigh(e + 1);
+                at_in_order();
             }
         }
     };
     for (uint32_t n = tile0; n < tile1; n++) {
+        at_wait_memory();                                          // this wave's loads have arrived
         if (PAGED) {
-            there = __ballot(page >= 0);
-            if (n + 1 < tile1) page = look(n + 1, slot);
+            there = there2;
+            there2 = __ballot(page >= 0);
         }
-        __builtin_amdgcn_s_waitcnt(0x0f70);                     // vmcnt(0): this wave's loads have arrived
         __syncthreads();                                        // and everyone's; and everyone is done with the other stage
         const uint32_t stage = (n - tile0) & 1;
         step(n, lds + (stage ^ 1) * 2 * S::TILE, lds + stage * 2 * S::TILE);
+        if (PAGED) {
+            page = page2;
+            slot = slot2;
+        }
     }
 
     // ---- result: lane's columns of d are 32 i + 8 (e / 4) + 4 half + e % 4

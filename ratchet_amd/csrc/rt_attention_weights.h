@@ -95,8 +95,7 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : 2) attention_weights_
         float lse = 0.0f, lse2 = 0.0f;
         uint32_t j = 0, j2 = 0;
         if (r0 < r1) load(r0, q, lse, j);
-        __builtin_amdgcn_s_waitcnt(0x0f70);                     // vmcnt(0): the keys are in LDS
-        asm volatile("" ::: "memory");
+        at_wait_memory();                                       // the keys are in LDS
 #pragma unroll
         for (int i = 0; i < S::STEPS; i++) {
             uint32_t cc = 2 * i + half;
