@@ -21,6 +21,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t AT_ROWS = 128, AT_WAVES = 4, AT_BLOCK = 64 * AT_WAVES;
+constexpr float AT_SLACK = 8.0f;                 // powers of two that a row's weights may lie above its m
 constexpr uint32_t AT_TARGET = 1024;             // work items that fill the chip: two blocks on each of 256 CUs, twice
 constexpr uint32_t AT_LEAST_TILES = 4;           // tiles that a piece of the keys is worth
 constexpr uint32_t AT_MOST_PIECES = 60;          // of a row tile: their factors for its 128 rows fit the LDS of the smallest tiles
@@ -172,6 +173,10 @@ __device__ __forceinline__ v2u at_lds_turned(const lds_byte* at) {
 __device__ __forceinline__ void at_to_lds(const void* from, lds_byte* at) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"((uint32_t)(uintptr_t)at) : "memory");
 }
+// The same with a base that all lanes share.  s_nop 4: a scalar register that a vector instruction wrote (v_readlane) may be read five states later.
+__device__ __forceinline__ void at_to_lds(const void* base, uint32_t offset, lds_byte* at) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"((uint32_t)(uintptr_t)at) : "memory");
+}
 __device__ __forceinline__ void at_wait_memory() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // x and the other half's value of the same column
 __device__ __forceinline__ float at_other(float x) {
@@ -193,7 +198,7 @@ template <typename T, int DT> struct AtShape {
     // a wave's last load of a tile may reach beyond it, and so may the transposed reads of the last block of columns
     static constexpr int TILE = (KT * CHUNKS * 16 + 1023) / 1024 * 1024;
     static constexpr int LDS = 4 * TILE + 256;
-    static constexpr int WAVES = DT > 128 ? 1 : 2;             // of a SIMD: what its registers are shared by
+    static constexpr int WAVES = DT > 128 ? 1 : DT > 96 ? 2 : 3;             // of a SIMD: what its registers are shared by
 };
 
 // 16-byte chunks of a row are rotated by an amount that goes by the row, so that what the lanes of one access read spreads over the banks: keys are read a
@@ -493,27 +498,44 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         t = t < s.keys ? t : s.keys - 1;
         return at_page(a, b, (uint32_t)t, slot);
     };
+    // contiguous: offsets of this lane's chunks from a whole tile's first key
+    uint32_t k_off[S::LOADS], v_off[S::LOADS];
+#pragma unroll
+    for (int i = 0; i < S::LOADS; i++) {
+        k_off[i] = l_row[i] * k_row + l_k[i];
+        v_off[i] = l_row[i] * v_row + l_v[i];
+    }
     auto fetch = [&](uint32_t n, lds_byte* to, int32_t page, uint32_t slot) __attribute__((always_inline)) {
         const int32_t t0 = start_of(n);
+        to += wave * 1024;
+        if (PAGED) {
 #pragma unroll
-        for (int i = 0; i < S::LOADS; i++) {
-            if (i * AT_WAVES + wave >= loads) break;
-            lds_byte* const at = to + (i * AT_WAVES + wave) * 1024;
-            uint64_t k_off, v_off;
-            if (PAGED) {
+            for (int i = 0; i < S::LOADS; i++) {
+                if (i * AT_WAVES + wave >= loads) break;
                 int32_t pg = __shfl(page, (int)l_row[i]);
                 const uint32_t sl = (uint32_t)__shfl((int)slot, (int)l_row[i]);
                 pg = pg < 0 ? 0 : pg;
-                k_off = (uint64_t)(uint32_t)pg * k_page + sl * (uint64_t)k_row;
-                v_off = k_off;
-            } else {
-                int32_t t = t0 + (int32_t)l_row[i];
-                t = t < s.keys ? t : s.keys - 1;
-                k_off = (uint64_t)(uint32_t)t * k_row;
-                v_off = (uint64_t)(uint32_t)t * v_row;
+                const uint64_t at = (uint64_t)(uint32_t)pg * k_page + sl * k_row;
+                at_to_lds(kb + at + l_k[i], to + i * AT_WAVES * 1024);
+                at_to_lds(vb + at + l_v[i], to + i * AT_WAVES * 1024 + S::TILE);
             }
-            at_to_lds(kb + k_off + l_k[i], at);
-            at_to_lds(vb + v_off + l_v[i], at + S::TILE);
+            return;
+        }
+        // Offsets within a tile fit 32 bits (the caller saw to it), its first key's need not.  The last tile's rows beyond the last key are that key's.
+        const unsigned char* k0 = kb + (uint64_t)(uint32_t)t0 * k_row;
+        const unsigned char* v0 = vb + (uint64_t)(uint32_t)t0 * v_row;
+        const bool cut = t0 + KT > s.keys;
+#pragma unroll
+        for (int i = 0; i < S::LOADS; i++) {
+            if (i * AT_WAVES + wave >= loads) break;
+            uint32_t ko = k_off[i], vo = v_off[i];
+            if (cut && t0 + (int32_t)l_row[i] >= s.keys) {
+                const uint32_t rr = (uint32_t)(s.keys - 1 - t0);
+                ko = rr * k_row + l_k[i];
+                vo = rr * v_row + l_v[i];
+            }
+            at_to_lds(k0, ko, to + i * AT_WAVES * 1024);
+            at_to_lds(v0, vo, to + i * AT_WAVES * 1024 + S::TILE);
         }
     };
 
@@ -605,7 +627,8 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
 #pragma unroll
             for (int e = 0; e < 16; e++) top = fmaxf(top, x[kk][e]);
         top = fmaxf(top, at_other(top)) * c;
-        if (__ballot(top > m)) {
+        // m follows the maximum at a distance: a weight of up to 2^AT_SLACK loses nothing in f32, f16 or bf16, and of 32 rows one has a new maximum in nearly every tile
+        if (__ballot(top > m + AT_SLACK)) {
             const float m_new = fmaxf(m, top), old = at_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
             m = m_new;
             l *= old;
@@ -671,19 +694,22 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
             }
         }
     };
-    for (uint32_t n = tile0; n < tile1; n++) {
-        at_wait_memory();                                          // this wave's loads have arrived
+    auto turn = [&](uint32_t n, lds_byte* next, const lds_byte* cur) __attribute__((always_inline)) {
+        at_wait_memory();                                       // this wave's loads have arrived
         if (PAGED) {
             there = there2;
             there2 = __ballot(page >= 0);
         }
         __syncthreads();                                        // and everyone's; and everyone is done with the other stage
-        const uint32_t stage = (n - tile0) & 1;
-        step(n, lds + (stage ^ 1) * 2 * S::TILE, lds + stage * 2 * S::TILE);
+        step(n, next, cur);
         if (PAGED) {
             page = page2;
             slot = slot2;
         }
+    };
+    for (uint32_t n = tile0; n < tile1; n += 2) {               // two at a time: the stages' addresses are then constants
+        turn(n, lds + 2 * S::TILE, lds);
+        if (n + 1 < tile1) turn(n + 1, lds, lds + 2 * S::TILE);
     }
 
     // ---- result: lane's columns of d are 32 i + 8 (e / 4) + 4 half + e % 4
@@ -851,10 +877,10 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
 }
 
 template <typename T> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool paged, bool* done) {
-    // rows of whole 16-byte chunks on 16-byte boundaries, 32-bit offsets of rows in a page and of pages
-    const uint64_t e = sizeof(T), most = 0xffffffffull / e;
+    // rows of whole 16-byte chunks on 16-byte boundaries; 32-bit offsets of the rows of a tile, or in a page, and of pages
+    const uint64_t e = sizeof(T), most = 0xffffffffull / e, far = (1ull << 31) / 64 / e;
     const uint64_t strides[] = {a.dim, a.q_b, a.q_h, a.q_t, a.k_b, a.k_h, a.k_t, a.v_b, a.v_h, a.v_t, a.y_b, a.y_h, a.y_t};
-    bool fits = rt_aligned(a.q, 16) && rt_aligned(a.k, 16) && rt_aligned(a.v, 16) && rt_aligned(a.y, 16) && a.k_t <= most && a.v_t <= most && (!paged || a.k_b <= most) &&
+    bool fits = rt_aligned(a.q, 16) && rt_aligned(a.k, 16) && rt_aligned(a.v, 16) && rt_aligned(a.y, 16) && a.k_t <= far && a.v_t <= far && (!paged || a.k_b <= most) &&
                 (uint64_t)a.tokens * a.group <= 0x7fffffffull && a.dim <= 256;
     for (uint64_t x : strides) fits = fits && x * e % 16 == 0;
     *done = fits;
