@@ -36,7 +36,13 @@ struct AttnArgs {
     float c;                       // scale * log2(e)
     int32_t causal, window, sinks;
     size_t own_lse;                // bytes of lse that the call itself needs and keeps at the front of the workspace
+    float* scores;                 // NULL, or [tokens, heads, score_pitch]: c q.k of each row and key, -inf where hidden, left for the received weights
+    uint32_t score_pitch;
+    bool want_scores;              // the caller has use for them
 };
+
+// Scores of up to this size are kept between the attention of few rows and the sum of its weights; 64 bytes of q and k a score is what it would take to have them again
+constexpr size_t AT_MOST_SCORES = 256u << 20;
 
 // The device's workspace with room for lse, if it is the call's own (a.lse is then set), and `bytes` behind it
 static inline int at_workspace(rt_device* dev, AttnArgs& a, size_t bytes, void** rest) {

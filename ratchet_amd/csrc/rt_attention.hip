@@ -304,6 +304,7 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
     a.table_len = kv->table_len;
     a.page_div = make_fastdiv(kv->page_len);
     a.causal = 1;
+    a.want_scores = weights_out != nullptr;
     a.own_lse = weights_out && !lse ? (size_t)tokens * heads * sizeof(float) : 0;
     return dispatch(dev, dt, a, true, weights, weights_out);
 }

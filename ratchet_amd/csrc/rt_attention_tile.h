@@ -405,7 +405,7 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
     }
 }
 
-// FEW: pieces are joined by the block that comes last
+// FEW: pieces are joined by the block that comes last, and scores are left where they are wanted
 template <typename T, int DT, bool EXACT, bool PAGED, bool FEW>
 __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES, AtShape<T, DT>::WAVES))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
     typedef AtShape<T, DT> S;
@@ -620,6 +620,14 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
                     const bool seen = t <= lim && (near - t < a.window || t < sink) && (!PAGED || (have >> t) & 1);
                     x[kk][e] = seen ? x[kk][e] : -INFINITY;
                 }
+        }
+        if (FEW && a.scores && r < rows) {
+            typedef float v4f __attribute__((ext_vector_type(4)));
+            float* to = a.scores + ((uint64_t)(s.first + j) * a.heads + h) * a.score_pitch + (uint32_t)t0 + 4 * half;
+#pragma unroll
+            for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) *(v4f*)(to + 32 * kk + 8 * (e / 4)) = v4f{x[kk][e] * c, x[kk][e + 1] * c, x[kk][e + 2] * c, x[kk][e + 3] * c};
         }
         float top = x[0][0];
 #pragma unroll
@@ -852,14 +860,18 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
     }
     const uint64_t blocks = items * per;
     RT_REQUIRE(blocks <= 0x7fffffffull, RT_ERR_SIZE, "attention: too many rows");
+    const bool few = (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
     const size_t row_count = part.split ? (size_t)blocks * AT_ROWS : 0;
+    a.score_pitch = (a.cap + 63) / 64 * 64;
+    size_t score_bytes = PAGED && few && a.want_scores ? (size_t)a.tokens * a.heads * a.score_pitch * sizeof(float) : 0;
+    if (score_bytes > AT_MOST_SCORES) score_bytes = 0;
     void* p = nullptr;
-    int rc = at_workspace(dev, a, row_count * ((size_t)a.dim + 2) * sizeof(float), &p);
+    int rc = at_workspace(dev, a, row_count * ((size_t)a.dim + 2) * sizeof(float) + score_bytes, &p);
     if (rc) return rc;
     part.ml = (float*)p;
     part.o = part.ml + 2 * row_count;
+    a.scores = score_bytes ? part.o + row_count * a.dim : nullptr;
     part.arrivals = dev->arrivals;
-    const bool few = part.split && (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
     const auto kernel = few ? attention_tile_kernel<T, DT, EXACT, PAGED, true> : attention_tile_kernel<T, DT, EXACT, PAGED, false>;
     static_assert(S::LDS <= 160 * 1024 && AT_MOST_PIECES * AT_ROWS * 4 <= S::LDS - 16, "LDS");
     static bool raised[2][16] = {};                             // per GPU; setting it twice does no harm

@@ -113,13 +113,20 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : 2) attention_weights_
             }
             const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
             const bool real = r + col < r1;
-            const int32_t lim = real ? limit - t0 - 4 * (int32_t)half : -1, near = p - t0 - 4 * (int32_t)half, sink = a.sinks - t0 - 4 * (int32_t)half;
-            const uint32_t have = there >> (4 * half);
+            // whether every row sees every key of the 32: nearly all tiles of a prompt
+            const bool clear = real && t0 + 31 <= limit && (p - t0 < a.window || t0 + 31 < a.sinks) && there == ~0u;
+            if (__ballot(clear) == ~0ull) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int32_t t = e % 4 + 8 * (e / 4);
-                const bool seen = t <= lim && (near - t < a.window || t < sink) && (have >> t) & 1;
-                sum[e] += seen ? at_exp2(__builtin_fmaf(x[e], c, lse)) : 0.0f;
+                for (int e = 0; e < 16; e++) sum[e] += at_exp2(__builtin_fmaf(x[e], c, lse));
+            } else {
+                const int32_t lim = real ? limit - t0 - 4 * (int32_t)half : -1, near = p - t0 - 4 * (int32_t)half, sink = a.sinks - t0 - 4 * (int32_t)half;
+                const uint32_t have = there >> (4 * half);
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int32_t t = e % 4 + 8 * (e / 4);
+                    const bool seen = t <= lim && (near - t < a.window || t < sink) && (have >> t) & 1;
+                    sum[e] += seen ? at_exp2(__builtin_fmaf(x[e], c, lse)) : 0.0f;
+                }
             }
 #pragma unroll
             for (int i = 0; i < S::STEPS; i++) q[i] = q2[i];
@@ -142,6 +149,26 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : 2) attention_weights_
     }
 }
 
+// The same from scores that the attention left (few rows): a thread to a key, its rows one after the other.  Reads a score a row and key, coalesced.
+constexpr uint32_t AW_SCORE_BLOCK = 128;
+static __global__ void __launch_bounds__(AW_SCORE_BLOCK) attention_weights_of_scores_kernel(AttnArgs a, const float* weights, float* out) {
+    const uint32_t g = blockIdx.y, b = blockIdx.z;
+    const AttnSeq s = at_seq<true>(a, b);
+    const int32_t t = (int32_t)(blockIdx.x * AW_SCORE_BLOCK + threadIdx.x);
+    if (t >= s.keys) return;
+    const uint64_t at = ((uint64_t)b * a.kv_heads + g) * a.cap + (uint32_t)t;
+    float sum = t < s.shift ? weights[at] : 0.0f;
+    for (uint32_t j = 0; j < s.count; j++) {
+        if (!at_visible(a, t, at_limit(a, s, j), at_position(s, j))) continue;                 // its score may never have been written
+        const uint64_t row = (uint64_t)(s.first + j) * a.heads + g * a.group;
+        for (uint32_t h = 0; h < a.group; h++) {
+            const float x = a.scores[(row + h) * a.score_pitch + (uint32_t)t];
+            sum += x == -INFINITY ? 0.0f : at_exp2(__builtin_fmaf(a.lse[row + h], -1.4426950408889634f, x));
+        }
+    }
+    out[at] = sum;
+}
+
 template <typename T, int DT, bool EXACT> int aw_launch(rt_device* dev, const AttnArgs& a, const float* weights, float* out) {
     typedef AtShape<T, DT> S;
     const uint64_t items = (uint64_t)a.seqs * ((a.cap + AW_KEYS - 1) / AW_KEYS) * a.kv_heads;
@@ -159,6 +186,12 @@ template <typename T, int DT, bool EXACT> int aw_launch(rt_device* dev, const At
 }
 
 template <typename T> int aw_dispatch(rt_device* dev, const AttnArgs& a, const float* weights, float* out) {
+    if (a.scores) {
+        const dim3 grid((a.cap + AW_SCORE_BLOCK - 1) / AW_SCORE_BLOCK, a.kv_heads, a.seqs);
+        hipLaunchKernelGGL(attention_weights_of_scores_kernel, grid, dim3(AW_SCORE_BLOCK), 0, dev->stream, a, weights, out);
+        RT_CHECK_LAUNCH("attention_weights_of_scores_kernel");
+        return RT_OK;
+    }
     if (a.dim == 64) return aw_launch<T, 64, true>(dev, a, weights, out);
     if (sizeof(T) == 2 && a.dim == 80) return aw_launch<T, 80, true>(dev, a, weights, out);
     if (sizeof(T) == 2 && a.dim == 96) return aw_launch<T, 96, true>(dev, a, weights, out);
