@@ -1,7 +1,7 @@
 // The attention weight that cached tokens receive from a call's queries, from the finished statistics of its rows:
 //     out[t] = (t is new ? 0 : weights[t]) + sum over the rows that see t of 2^(c q.k_t - lse / ln 2)
-// A wave owns 32 keys of a KV head. They are the rows of the 32 x 32 products S^T = K Q^T and stay in registers while the queries that may see
-// them go by, 32 at a time; each lane adds up the weights of its own query column, and the columns are summed once at the end: no atomics, one order.
+// A wave owns 32 keys of a KV head.  They are the rows of the 32 x 32 products S^T = K Q^T and stay in registers while the queries that may see
+// them go by, 64 at a time; each lane adds up the weights of its own query column, and the columns are summed once at the end: no atomics, one order.
 #ifndef RT_ATTENTION_WEIGHTS_H
 #define RT_ATTENTION_WEIGHTS_H
 
@@ -32,106 +32,164 @@ __device__ __forceinline__ uint32_t aw_locate(const AttnArgs& a, uint32_t& at) {
     return a.seqs;
 }
 
-template <typename T, int DT, bool EXACT>
-__global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : 2) attention_weights_kernel(AttnArgs a, const float* weights, float* out) {
+constexpr int AW_ROWS = 64;                      // queries to a stage
+
+template <typename T, int DT, bool EXACT> struct AwShape : AtShape<T, DT> {
     typedef AtShape<T, DT> S;
+    static constexpr int PART = (32 * S::CHUNKS * 16 + 1023) / 1024 * 1024;     // a wave's keys in LDS, on their way to registers
+    static constexpr int ROWS_AT = (AW_ROWS * S::CHUNKS * 16 + 1023) / 1024 * 1024;            // where a stage keeps its rows' lse
+    static constexpr int STAGE = ROWS_AT + AW_ROWS * 4;
+    static constexpr int STAGES = 3 * STAGE <= 160 * 1024 ? 3 : 2;              // of queries in LDS
+    static constexpr int LDS = STAGES * STAGE > AT_WAVES * PART ? STAGES * STAGE : AT_WAVES * PART;
+    static constexpr int LOADS = (AW_ROWS * S::CHUNKS + AT_BLOCK - 1) / AT_BLOCK;               // of a stage's rows, by each wave, at most
+    // of the youngest stage, those that every wave has issued: what may still be in flight when the one before it is needed
+    static constexpr int LEAST = EXACT && STAGES == 3 ? AW_ROWS * S::CHUNKS / AT_BLOCK : 0;
+};
+
+// 4 bytes a lane from memory to LDS, lane i's to at + 4 i
+__device__ __forceinline__ void aw_to_lds4(const void* from, lds_byte* at) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "{m0}"((uint32_t)(uintptr_t)at) : "memory");
+}
+template <int N> __device__ __forceinline__ void aw_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// The block's four waves share the queries, which go through stages of LDS, two on their way while one is worked on (one where rows are too wide for three).  Bound by the exponentials for prompts.
+template <typename T, int DT, bool EXACT>
+__global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : DT > 96 ? 2 : 3) attention_weights_kernel(AttnArgs a, const float* weights, float* out) {
+    typedef AwShape<T, DT, EXACT> S;
     constexpr int CE = S::CE;
     extern __shared__ __align__(16) unsigned char smem[];
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
     const uint32_t D = EXACT ? DT : a.dim, chunks = D / CE, pitch = D * sizeof(T);
-    constexpr uint32_t PART = (32 * S::CHUNKS * 16 + 1023) / 1024 * 1024;       // a wave's keys in LDS
-    lds_byte* const lds = (lds_byte*)smem + wave * PART;
+    lds_byte* const lds = (lds_byte*)smem;
     const float c = a.c;
+    uint32_t k_at[S::STEPS];                                    // chunk 2 i + half of row col: keys and queries alike
+#pragma unroll
+    for (int i = 0; i < S::STEPS; i++) {
+        uint32_t cc = 2 * i + half;
+        cc = (cc < chunks ? cc : 0) + at_turn_k(col, chunks);
+        k_at[i] = col * pitch + (cc >= chunks ? cc - chunks : cc) * 16;
+    }
     for (uint32_t item = blockIdx.x;; item += gridDim.x) {
         const uint32_t g = item % a.kv_heads;
         uint32_t at = item / a.kv_heads;
         const uint32_t b = __builtin_amdgcn_readfirstlane(aw_locate(a, at));
         if (b >= a.seqs) return;
         const AttnSeq s = at_seq<true>(a, b);
-        const int32_t t0 = (int32_t)(__builtin_amdgcn_readfirstlane(at) * AW_KEYS + wave * 32);
-        if (t0 >= s.keys) continue;
+        const int32_t tb = (int32_t)(__builtin_amdgcn_readfirstlane(at) * AW_KEYS), t0 = tb + (int32_t)wave * 32;
+        const bool busy = t0 < s.keys;
 
-        uint32_t slot;
-        const int32_t mine = t0 + (int32_t)col, page = at_page(a, b, (uint32_t)(mine < s.keys ? mine : s.keys - 1), slot);
+        // ---- this wave's keys, through LDS to registers
+        const int32_t mine = t0 + (int32_t)col;
+        uint32_t slot = 0;
+        const int32_t page = at_page(a, b, (uint32_t)(mine < s.keys ? mine : s.keys - 1), slot);
         const uint64_t w_at = ((uint64_t)b * a.kv_heads + g) * a.cap;
         const float before = mine < s.keys && mine < s.shift ? weights[w_at + (uint32_t)mine] : 0.0f;
         const uint32_t there = (uint32_t)__ballot(page >= 0);   // both halves say the same
         const unsigned char* kb = (const unsigned char*)a.k + g * a.k_h * sizeof(T);
         const uint32_t slots = 32 * chunks;
+        __syncthreads();                                        // the item before this one is done with LDS
         for (uint32_t i = 0; i < (slots + 63) / 64; i++) {
             uint32_t at_slot = i * 64 + lane;
             at_slot = at_slot < slots ? at_slot : slots - 1;
             const uint32_t rr = at_slot / chunks, cc = at_slot - rr * chunks, tk = at_turn_k(rr, chunks);
             const int32_t pg = __shfl(page, (int)rr);
             const uint64_t off = (uint64_t)(pg < 0 ? 0 : pg) * (a.k_b * sizeof(T)) + (uint32_t)__shfl((int)slot, (int)rr) * (uint64_t)pitch;
-            at_to_lds(kb + off + (cc >= tk ? cc - tk : cc + chunks - tk) * 16, lds + i * 1024);
+            at_to_lds(kb + off + (cc >= tk ? cc - tk : cc + chunks - tk) * 16, lds + wave * S::PART + i * 1024);
         }
+        v4u k[S::STEPS];
+        at_wait_memory();
+#pragma unroll
+        for (int i = 0; i < S::STEPS; i++) {
+            k[i] = at_lds16(lds + (wave * S::PART + k_at[i]));
+            if ((2 * i + half) >= chunks) k[i] = v4u{0, 0, 0, 0};
+        }
+        __syncthreads();
 
-        // the rows that may see one of these keys: positions from t0 on and, where no sink is among them, up to the last key's window
-        int64_t j0 = (int64_t)t0 - s.shift, j1 = s.count;
-        if (a.window != AT_FAR && t0 >= a.sinks) {
-            const int64_t x = (int64_t)t0 + 31 + a.window - s.shift;
+        // ---- the rows that may see one of the block's keys: positions from the first key on and, where no sink is among them, up to the last key's window
+        int64_t j0 = (int64_t)tb - s.shift, j1 = s.count;
+        if (a.window != AT_FAR && tb >= a.sinks) {
+            const int64_t x = (int64_t)tb + AW_KEYS - 1 + a.window - s.shift;
             j1 = x < j1 ? x : j1;
         }
         j0 = j0 < 0 ? 0 : j0;
         const uint32_t r0 = j0 < j1 ? (uint32_t)j0 * a.group : 0, r1 = j0 < j1 ? (uint32_t)j1 * a.group : 0;
-
-        auto load = [&](uint32_t r, v4u (&q)[S::STEPS], float& lse, uint32_t& j) __attribute__((always_inline)) {
-            const uint32_t row = r + col < r1 ? r + col : r1 - 1;
-            j = fd_div(row, a.group_div);
-            const uint32_t h = g * a.group + (row - j * a.group);
-            const T* from = (const T*)a.q + h * a.q_h + (uint64_t)(s.first + j) * a.q_t;
+        const uint32_t stages = (r1 - r0 + AW_ROWS - 1) / AW_ROWS, loads = (AW_ROWS * chunks + 63) / 64;
+        auto fetch = [&](uint32_t n, uint32_t stage) __attribute__((always_inline)) {
+            lds_byte* const to = lds + stage * S::STAGE;
 #pragma unroll
-            for (int i = 0; i < S::STEPS; i++) {
-                q[i] = v4u{0, 0, 0, 0};
-                if ((2 * i + half) * CE < D) q[i] = *(const v4u*)(from + (2 * i + half) * CE);
+            for (int i = 0; i < S::LOADS; i++) {
+                if (i * AT_WAVES + wave >= loads) break;
+                uint32_t at_slot = (i * AT_WAVES + wave) * 64 + lane;
+                at_slot = at_slot < AW_ROWS * chunks ? at_slot : AW_ROWS * chunks - 1;
+                const uint32_t rr = at_slot / chunks, cc = at_slot - rr * chunks, tk = at_turn_k(rr, chunks);
+                uint32_t row = r0 + n * AW_ROWS + rr;
+                row = row < r1 ? row : r1 - 1;
+                const uint32_t j = fd_div(row, a.group_div), h = g * a.group + (row - j * a.group);
+                const unsigned char* from = (const unsigned char*)a.q + (h * a.q_h + (uint64_t)(s.first + j) * a.q_t) * sizeof(T);
+                at_to_lds(from + (cc >= tk ? cc - tk : cc + chunks - tk) * 16, to + (i * AT_WAVES + wave) * 1024);
             }
-            lse = a.lse[h * a.l_h + (uint64_t)(s.first + j) * a.l_t] * -1.4426950408889634f;
+            if (wave == AT_WAVES - 1) {
+                uint32_t row = r0 + n * AW_ROWS + lane;
+                row = row < r1 ? row : r1 - 1;
+                const uint32_t j = fd_div(row, a.group_div), h = g * a.group + (row - j * a.group);
+                aw_to_lds4(a.lse + h * a.l_h + (uint64_t)(s.first + j) * a.l_t, to + S::ROWS_AT);
+            }
         };
         float sum[16];
 #pragma unroll
         for (int e = 0; e < 16; e++) sum[e] = 0.0f;
-        v4u k[S::STEPS], q[S::STEPS], q2[S::STEPS];
-        float lse = 0.0f, lse2 = 0.0f;
-        uint32_t j = 0, j2 = 0;
-        if (r0 < r1) load(r0, q, lse, j);
-        at_wait_memory();                                       // the keys are in LDS
+        if (stages > 0) fetch(0, 0);
+        if (S::STAGES == 3 && stages > 1) fetch(1, 1);
+        uint32_t stage = 0;
+        for (uint32_t n = 0; n < stages; n++) {
+            if (n + 1 < stages) aw_wait<S::LEAST>();
+            else aw_wait<0>();
+            __syncthreads();                                    // this stage is there, and everyone is done with the one before
+            if (n + S::STAGES - 1 < stages) fetch(n + S::STAGES - 1, stage == 0 ? S::STAGES - 1 : stage - 1);
+            const lds_byte* const cur = lds + stage * S::STAGE;
+            stage = stage == S::STAGES - 1 ? 0 : stage + 1;
+            if (!busy) continue;
+            constexpr int N = 2 * S::STEPS, AHEAD = N < 4 ? N : 4;
+            v16f x[2] = {v16f{0}, v16f{0}};
+            v4u q[N];
+            auto read_q = [&](int p) __attribute__((always_inline)) {
+                if (!EXACT && (uint32_t)(p / 2 * 2 * CE) >= D) return;
+                q[p] = at_lds16(cur + (k_at[p / 2] + p % 2 * 32 * pitch));
+            };
 #pragma unroll
-        for (int i = 0; i < S::STEPS; i++) {
-            uint32_t cc = 2 * i + half;
-            const bool in = cc < chunks;
-            cc = (in ? cc : 0) + at_turn_k(col, chunks);
-            k[i] = at_lds16(lds + (col * pitch + (cc >= chunks ? cc - chunks : cc) * 16));
-            if (!in) k[i] = v4u{0, 0, 0, 0};
-        }
-        for (uint32_t r = r0; r < r1; r += 32) {
-            if (r + 32 < r1) load(r + 32, q2, lse2, j2);
-            v16f x = {0};
+            for (int p = 0; p < AHEAD; p++) read_q(p);
+            const float lse[2] = {at_lds4(cur + S::ROWS_AT + col * 4) * -1.4426950408889634f, at_lds4(cur + S::ROWS_AT + (col + 32) * 4) * -1.4426950408889634f};
+            at_in_order();
 #pragma unroll
-            for (int i = 0; i < S::STEPS; i++) {
-                if (EXACT || (uint32_t)(2 * i * CE) < D) x = AtMma<T>::qk(k[i], q[i], x);
+            for (int p = 0; p < N; p++) {
+                // where the row ends in a half chunk, both operands' other half holds what is not theirs: k's is 0 and q's has to be
+                if ((EXACT ? DT % (2 * CE) != 0 : true) && (p / 2 * 2 + 2) * CE > (int)D && half) q[p] = v4u{0, 0, 0, 0};
+                if (EXACT || (uint32_t)(p / 2 * 2 * CE) < D) x[p % 2] = AtMma<T>::qk(k[p / 2], q[p], x[p % 2]);
+                if (p + AHEAD < N) read_q(p + AHEAD);
+                at_in_order();
             }
-            const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
-            const bool real = r + col < r1;
-            // whether every row sees every key of the 32: nearly all tiles of a prompt
-            const bool clear = real && t0 + 31 <= limit && (p - t0 < a.window || t0 + 31 < a.sinks) && there == ~0u;
-            if (__ballot(clear) == ~0ull) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) sum[e] += at_exp2(__builtin_fmaf(x[e], c, lse));
-            } else {
-                const int32_t lim = real ? limit - t0 - 4 * (int32_t)half : -1, near = p - t0 - 4 * (int32_t)half, sink = a.sinks - t0 - 4 * (int32_t)half;
-                const uint32_t have = there >> (4 * half);
+            for (int y = 0; y < 2; y++) {
+                const uint32_t row = r0 + n * AW_ROWS + 32 * y + col;
+                const bool real = row < r1;
+                const uint32_t j = fd_div(real ? row : r1 - 1, a.group_div);
+                const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
+                // whether every row sees every key of the 32: nearly all tiles of a prompt
+                const bool clear = real && t0 + 31 <= limit && (p - t0 < a.window || t0 + 31 < a.sinks) && there == ~0u;
+                if (__ballot(clear) == ~0ull) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int32_t t = e % 4 + 8 * (e / 4);
-                    const bool seen = t <= lim && (near - t < a.window || t < sink) && (have >> t) & 1;
-                    sum[e] += seen ? at_exp2(__builtin_fmaf(x[e], c, lse)) : 0.0f;
+                    for (int e = 0; e < 16; e++) sum[e] += at_exp2(__builtin_fmaf(x[y][e], c, lse[y]));
+                } else {
+                    const int32_t lim = real ? limit - t0 - 4 * (int32_t)half : -1, near = p - t0 - 4 * (int32_t)half, sink = a.sinks - t0 - 4 * (int32_t)half;
+                    const uint32_t have = there >> (4 * half);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int32_t t = e % 4 + 8 * (e / 4);
+                        const bool seen = t <= lim && (near - t < a.window || t < sink) && (have >> t) & 1;
+                        sum[e] += seen ? at_exp2(__builtin_fmaf(x[y][e], c, lse[y])) : 0.0f;
+                    }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < S::STEPS; i++) q[i] = q2[i];
-            lse = lse2;
-            j = j2;
         }
         // over the 32 columns; the lane with column n keeps key n: element e of half h is key e % 4 + 8 (e / 4) + 4 h
         float total = 0.0f;
@@ -170,10 +228,11 @@ static __global__ void __launch_bounds__(AW_SCORE_BLOCK) attention_weights_of_sc
 }
 
 template <typename T, int DT, bool EXACT> int aw_launch(rt_device* dev, const AttnArgs& a, const float* weights, float* out) {
-    typedef AtShape<T, DT> S;
+    typedef AwShape<T, DT, EXACT> S;
     const uint64_t items = (uint64_t)a.seqs * ((a.cap + AW_KEYS - 1) / AW_KEYS) * a.kv_heads;
     const unsigned blocks = items < AW_MOST_BLOCKS ? (unsigned)items : (AW_MOST_BLOCKS + a.kv_heads - 1) / a.kv_heads * a.kv_heads;
-    constexpr int LDS = AT_WAVES * ((32 * S::CHUNKS * 16 + 1023) / 1024 * 1024);
+    static_assert(S::LDS <= 160 * 1024, "LDS");
+    constexpr int LDS = S::LDS;
     const auto kernel = attention_weights_kernel<T, DT, EXACT>;
     static bool raised[16] = {};
     if (LDS > 64 * 1024 && !(dev->ordinal < 16 && raised[dev->ordinal])) {
