@@ -51,17 +51,19 @@ template <int KT> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a
     uint64_t work = 0;
     for (uint32_t b = __lane_id(); b < a.seqs; b += 64) {
         const AttnSeq s = at_seq<true>(a, b);
-        work += (uint64_t)at_row_tiles(a, s) * at_span<KT>(a, s);
+        const uint32_t span = at_span<KT>(a, s), less = s.count / (2 * KT);      // causal: the middle row of the new ones lacks half of them
+        work += (uint64_t)at_row_tiles(a, s) * (span > 2 * less ? span - less : (span + 1) / 2);
     }
     work = at_wave_sum(work) * a.kv_heads;
     const uint64_t n = (work + AT_TARGET - 1) / AT_TARGET;
     return n < AT_LEAST_TILES ? AT_LEAST_TILES : n > 0x7fffffffu ? 0x7fffffffu : (uint32_t)n;
 }
 
-// ... and in a piece of this sequence's
-__device__ __forceinline__ uint32_t at_piece_of(uint32_t piece, uint32_t span) {
-    const uint32_t least = (span + AT_MOST_PIECES - 1) / AT_MOST_PIECES;
-    return piece > least ? piece : least;
+// ... and in a piece of this sequence's: pieces of the same size
+__host__ __device__ __forceinline__ uint32_t at_piece_of(uint32_t piece, uint32_t span) {
+    uint32_t n = (span + piece - 1) / piece;
+    n = n < AT_MOST_PIECES ? n : AT_MOST_PIECES;
+    return (span + n - 1) / n;
 }
 
 // Sequence b's items are numbered row tile by row tile, at_items of them, after those of the sequences before it.
@@ -505,19 +507,26 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         k_off[i] = l_row[i] * k_row + l_k[i];
         v_off[i] = l_row[i] * v_row + l_v[i];
     }
-    auto fetch = [&](uint32_t n, lds_byte* to, int32_t page, uint32_t slot) __attribute__((always_inline)) {
+    // paged: offsets of the rows of this lane's chunks of the next tile, worked out from its pages before the loads can be issued
+    uint64_t next_off[S::LOADS];
+    auto prepare = [&](int32_t page, uint32_t slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < S::LOADS; i++) {
+            int32_t pg = __shfl(page, (int)l_row[i]);
+            const uint32_t sl = (uint32_t)__shfl((int)slot, (int)l_row[i]);
+            pg = pg < 0 ? 0 : pg;
+            next_off[i] = (uint64_t)(uint32_t)pg * k_page + sl * k_row;
+        }
+    };
+    auto fetch = [&](uint32_t n, lds_byte* to) __attribute__((always_inline)) {
         const int32_t t0 = start_of(n);
         to += wave * 1024;
         if (PAGED) {
 #pragma unroll
             for (int i = 0; i < S::LOADS; i++) {
                 if (i * AT_WAVES + wave >= loads) break;
-                int32_t pg = __shfl(page, (int)l_row[i]);
-                const uint32_t sl = (uint32_t)__shfl((int)slot, (int)l_row[i]);
-                pg = pg < 0 ? 0 : pg;
-                const uint64_t at = (uint64_t)(uint32_t)pg * k_page + sl * k_row;
-                at_to_lds(kb + at + l_k[i], to + i * AT_WAVES * 1024);
-                at_to_lds(vb + at + l_v[i], to + i * AT_WAVES * 1024 + S::TILE);
+                at_to_lds(kb + next_off[i] + l_k[i], to + i * AT_WAVES * 1024);
+                at_to_lds(vb + next_off[i] + l_v[i], to + i * AT_WAVES * 1024 + S::TILE);
             }
             return;
         }
@@ -567,21 +576,22 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
     for (int i = 0; i < S::BLOCKS; i++) o[i] = v16f{0};
     float m = -INFINITY, l = 0.0f;                              // l: of this lane's half of the keys
 
-    int32_t page = 0, page2 = 0;                                // of the next tile, and of the one after it
-    uint32_t slot = 0, slot2 = 0;
-    uint64_t there = ~0ull, there2 = ~0ull;                     // keys of the tile at hand that have a page, and of the next
+    int32_t page = 0;                                           // of this lane's key of the tile after next
+    uint32_t slot = 0;
+    uint64_t there = ~0ull, there1 = ~0ull;                     // keys of the tile at hand that have a page, and of the next
     if (tile0 < tile1) {
         if (PAGED) {
             page = look(tile0, slot);
-            there2 = __ballot(page >= 0);
+            there1 = __ballot(page >= 0);
+            prepare(page, slot);
         }
-        fetch(tile0, lds, page, slot);
+        fetch(tile0, lds);
         if (PAGED && tile0 + 1 < tile1) page = look(tile0 + 1, slot);
     }
     // One tile: the loads of the next one go into `next` while this one is read from `cur`.  The wait for them stands at the top of the next step.
     auto step = [&](uint32_t n, lds_byte* next, const lds_byte* cur) __attribute__((always_inline)) {
-        if (n + 1 < tile1) fetch(n + 1, next, page, slot);
-        if (PAGED && n + 2 < tile1) page2 = look(n + 2, slot2);                 // arrives while this tile is worked on
+        if (n + 1 < tile1) fetch(n + 1, next);
+        if (PAGED && n + 2 < tile1) page = look(n + 2, slot);                   // arrives while this tile is worked on
         const int32_t t0 = start_of(n);
         if (!busy || t0 > limit_z || (t0 >= a.sinks && p_a - (t0 + KT - 1) >= a.window)) return;
 
@@ -703,17 +713,14 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         }
     };
     auto turn = [&](uint32_t n, lds_byte* next, const lds_byte* cur) __attribute__((always_inline)) {
-        at_wait_memory();                                       // this wave's loads have arrived
         if (PAGED) {
-            there = there2;
-            there2 = __ballot(page >= 0);
+            there = there1;
+            there1 = __ballot(page >= 0);
+            prepare(page, slot);
         }
+        at_wait_memory();                                       // this wave's loads have arrived
         __syncthreads();                                        // and everyone's; and everyone is done with the other stage
         step(n, next, cur);
-        if (PAGED) {
-            page = page2;
-            slot = slot2;
-        }
     };
     for (uint32_t n = tile0; n < tile1; n += 2) {               // two at a time: the stages' addresses are then constants
         turn(n, lds + 2 * S::TILE, lds);
@@ -847,10 +854,10 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
             const uint64_t w = ((uint64_t)a.window + AT_ROWS) / S::KT + 2 + ((uint64_t)a.sinks + S::KT - 1) / S::KT;
             span = w < span ? w : span;
         }
-        uint64_t piece = (span * part.row_tiles * per + AT_TARGET - 1) / AT_TARGET;
-        const uint64_t least = (span + AT_MOST_PIECES - 1) / AT_MOST_PIECES;
-        piece = piece < AT_LEAST_TILES ? AT_LEAST_TILES : piece;
-        piece = piece < least ? least : piece;
+        const uint64_t less = a.causal ? a.tokens / (2 * S::KT) : 0, mean = span > 2 * less ? span - less : (span + 1) / 2;
+        uint64_t piece = (mean * part.row_tiles * per + AT_TARGET - 1) / AT_TARGET;
+        piece = piece < AT_LEAST_TILES ? AT_LEAST_TILES : piece > span ? span : piece;
+        piece = at_piece_of((uint32_t)piece, (uint32_t)span);
         if (part.row_tiles * ((span + piece - 1) / piece) * per > RT_ARRIVALS) piece = span;
         part.piece = (uint32_t)piece;
         part.pieces = (uint32_t)((span + piece - 1) / piece);
