@@ -22,8 +22,12 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t AT_ROWS = 128, AT_WAVES = 4, AT_BLOCK = 64 * AT_WAVES;
 constexpr float AT_SLACK = 8.0f;                 // powers of two that a row's weights may lie above its m
-constexpr uint32_t AT_TARGET = 1024;             // work items that fill the chip: two blocks on each of 256 CUs, twice
-constexpr uint32_t AT_LEAST_TILES = 4;           // tiles that a piece of the keys is worth
+// How far the keys of row tiles are shared out over blocks.  Single tokens (FEW): to AT_TARGET_FEW items, in pieces of no fewer than two tiles, which costs little as
+// their parts are small (one token's 2051 keys 17.9 us, with four tiles at least 19.3; 16 tokens 53 us at 1024 items, 61 at 512, 58 at 2048; 64 ragged
+// ones 255, 277, 251).  Others leave and join 64 KB a row tile and piece: only where the row tiles do not fill the chip by themselves (AT_ENOUGH), and to
+// AT_TARGET items (Phi-2 prompt, 512 row tiles: 45 us whole, 55 to 57 shared out; chunks, about 100 row tiles: 152 us at 256 items, 125 at 768, 142 at 1536;
+// encoder, 288: 202, 149, 140).
+constexpr uint32_t AT_TARGET_FEW = 1024, AT_TARGET = 768, AT_ENOUGH = 512, AT_LEAST_TILES_FEW = 2, AT_LEAST_TILES = 4;
 constexpr uint32_t AT_MOST_PIECES = 60;          // of a row tile: their factors for its 128 rows fit the LDS of the smallest tiles
 constexpr uint32_t AT_FEW_ROWS = 16;             // rows of a sequence and KV head, on average, up to which a launch joins its own pieces
 constexpr uint32_t AT_JOIN_ROWS = 16;            // rows to a block of the joining kernel
@@ -46,19 +50,25 @@ template <typename T> __device__ __forceinline__ T at_wave_sum(T x) {
     return x;
 }
 
-// Tiles in a piece of the keys: as many as give AT_TARGET work items in all, and no fewer than AT_LEAST_TILES.  The same in every wave.
-template <int KT> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a) {
+// Tiles in a piece of the keys, for `tiles` row tiles in all that have `work` tiles of keys to walk
+template <bool FEW> __host__ __device__ __forceinline__ uint32_t at_piece_for(uint64_t tiles, uint64_t work) {
+    if (!FEW && tiles >= AT_ENOUGH) return 0x7fffffffu;
+    constexpr uint32_t target = FEW ? AT_TARGET_FEW : AT_TARGET, least = FEW ? AT_LEAST_TILES_FEW : AT_LEAST_TILES;
+    const uint64_t n = (work + target - 1) / target;
+    return n < least ? least : n > 0x7fffffffu ? 0x7fffffffu : (uint32_t)n;
+}
+// The same from the device's lengths; the same in every wave.
+template <int KT, bool FEW> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a) {
     uint64_t work = 0;
+    uint32_t tiles = 0;
     for (uint32_t b = __lane_id(); b < a.seqs; b += 64) {
         const AttnSeq s = at_seq<true>(a, b);
-        const uint32_t span = at_span<KT>(a, s), less = s.count / (2 * KT);      // causal: the middle row of the new ones lacks half of them
+        const uint32_t span = at_span<KT>(a, s), less = FEW ? 0 : s.count / (2 * KT);           // causal: the middle row of the new ones lacks half of them
         work += (uint64_t)at_row_tiles(a, s) * (span > 2 * less ? span - less : (span + 1) / 2);
+        tiles += at_row_tiles(a, s);
     }
-    work = at_wave_sum(work) * a.kv_heads;
-    const uint64_t n = (work + AT_TARGET - 1) / AT_TARGET;
-    return n < AT_LEAST_TILES ? AT_LEAST_TILES : n > 0x7fffffffu ? 0x7fffffffu : (uint32_t)n;
+    return at_piece_for<FEW>((uint64_t)at_wave_sum(tiles) * a.kv_heads, at_wave_sum(work) * a.kv_heads);
 }
-
 // ... and in a piece of this sequence's: pieces of the same size
 __host__ __device__ __forceinline__ uint32_t at_piece_of(uint32_t piece, uint32_t span) {
     uint32_t n = (span + piece - 1) / piece;
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         stride = a.kv_heads;
         g = blockIdx.x % a.kv_heads;
         uint32_t at = blockIdx.x / a.kv_heads;
-        piece = part.split ? __builtin_amdgcn_readfirstlane(at_piece<KT>(a)) : 0x7fffffffu;
+        piece = part.split ? __builtin_amdgcn_readfirstlane(at_piece<KT, FEW>(a)) : 0x7fffffffu;
         b = __builtin_amdgcn_readfirstlane(at_locate<KT>(a, piece, at));
         if (b >= a.seqs) return;
         tile = __builtin_amdgcn_readfirstlane(at);
@@ -810,7 +820,7 @@ template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_B
         if (b >= a.seqs) return;
         s = at_seq<true>(a, b);
         tile = __builtin_amdgcn_readfirstlane(at);
-        const uint32_t span = at_span<KT>(a, s), all = __builtin_amdgcn_readfirstlane(at_piece<KT>(a));
+        const uint32_t span = at_span<KT>(a, s), all = __builtin_amdgcn_readfirstlane(at_piece<KT, false>(a));
         piece = at_piece_of(all, span);
         pieces = (span + piece - 1) / piece;
         if (pieces == 1) return;
@@ -838,13 +848,15 @@ template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_B
 template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_device* dev, AttnArgs& a) {
     typedef AtShape<T, DT> S;
     AttnPartial part = {};
+    const bool few = (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
     uint64_t join_tiles, items;                                 // row tiles; blocks per KV head (paged) or per (batch entry, KV head)
     const uint64_t per = PAGED ? a.kv_heads : (uint64_t)a.seqs * a.kv_heads;
     if (PAGED) {
         const uint64_t tiles = ((uint64_t)a.tokens * a.group) / AT_ROWS + a.seqs;
-        // sum over the row tiles of ceil(span / piece): at most AT_TARGET / kv_heads + 1 and one for each row tile
-        items = tiles + AT_TARGET / a.kv_heads + 1;
-        part.split = a.cap > AT_LEAST_TILES * S::KT && items * per <= RT_ARRIVALS;
+        // sum over the row tiles of ceil(span / piece): no more than work / piece, which is at most the target, and one for each row tile
+        const uint32_t target = few ? AT_TARGET_FEW : AT_TARGET, least = few ? AT_LEAST_TILES_FEW : AT_LEAST_TILES;
+        items = tiles + (few ? 1 : 2) * target / a.kv_heads + 1;                // (twice where the work is a causal mean, at least half of the spans)
+        part.split = a.cap > least * S::KT && items * per <= RT_ARRIVALS;
         if (!part.split) items = tiles;
         join_tiles = tiles * per;
     } else {
@@ -855,9 +867,9 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
             span = w < span ? w : span;
         }
         const uint64_t less = a.causal ? a.tokens / (2 * S::KT) : 0, mean = span > 2 * less ? span - less : (span + 1) / 2;
-        uint64_t piece = (mean * part.row_tiles * per + AT_TARGET - 1) / AT_TARGET;
-        piece = piece < AT_LEAST_TILES ? AT_LEAST_TILES : piece > span ? span : piece;
-        piece = at_piece_of((uint32_t)piece, (uint32_t)span);
+        const uint64_t tiles = part.row_tiles * per;
+        uint64_t piece = few ? at_piece_for<true>(tiles, mean * tiles) : at_piece_for<false>(tiles, mean * tiles);
+        piece = at_piece_of((uint32_t)(piece > span ? span : piece), (uint32_t)span);
         if (part.row_tiles * ((span + piece - 1) / piece) * per > RT_ARRIVALS) piece = span;
         part.piece = (uint32_t)piece;
         part.pieces = (uint32_t)((span + piece - 1) / piece);
@@ -867,7 +879,6 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
     }
     const uint64_t blocks = items * per;
     RT_REQUIRE(blocks <= 0x7fffffffull, RT_ERR_SIZE, "attention: too many rows");
-    const bool few = (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
     const size_t row_count = part.split ? (size_t)blocks * AT_ROWS : 0;
     a.score_pitch = (a.cap + 63) / 64 * 64;
     size_t score_bytes = PAGED && few && a.want_scores ? (size_t)a.tokens * a.heads * a.score_pitch * sizeof(float) : 0;
