@@ -301,7 +301,16 @@ struct AttnPartial {
     uint32_t pieces;               // contiguous: pieces of the keys a row tile is split into, `piece` tiles each
     uint32_t piece;
     uint32_t row_tiles;            // contiguous: of each batch entry
+    uint32_t round;                // see at_turned
 };
+
+// Contiguous: which row tile, counted from the last, has place `at` in the launch.  A launch that the chip holds at once is not balanced by blocks that come later: where
+// a CU gets one block of each `round` tiles, every other round runs backwards, so that a long causal walk shares its CU with a short one.
+__device__ __forceinline__ uint32_t at_turned(const AttnPartial& part, uint32_t at) {
+    if (part.round == 0) return at;
+    const uint32_t n = at / part.round, first = n * part.round, count = part.row_tiles - first < part.round ? part.row_tiles - first : part.round;
+    return n & 1 ? first + count - 1 - (at - first) : at;
+}
 
 __device__ __forceinline__ void at_leave(float* to, float x, float y) {
     const uint64_t both = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
@@ -443,7 +452,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         b = pair / a.kv_heads;
         g = pair - b * a.kv_heads;
         piece = part.piece;
-        tile = part.row_tiles - 1 - at / part.pieces;                           // the longest walks first
+        tile = part.row_tiles - 1 - at_turned(part, at / part.pieces);          // the longest walks first
         piece_at = at % part.pieces;
     }
     const AttnSeq s = at_seq<PAGED>(a, b);
@@ -856,7 +865,8 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
         // sum over the row tiles of ceil(span / piece): no more than work / piece, which is at most the target, and one for each row tile
         const uint32_t target = few ? AT_TARGET_FEW : AT_TARGET, least = few ? AT_LEAST_TILES_FEW : AT_LEAST_TILES;
         items = tiles + (few ? 1 : 2) * target / a.kv_heads + 1;                // (twice where the work is a causal mean, at least half of the spans)
-        part.split = a.cap > least * S::KT && items * per <= RT_ARRIVALS;
+        const bool enough = !few && ((uint64_t)a.tokens * a.group + AT_ROWS - 1) / AT_ROWS * per >= AT_ENOUGH;                // at least so many row tiles
+        part.split = a.cap > least * S::KT && items * per <= RT_ARRIVALS && !enough;
         if (!part.split) items = tiles;
         join_tiles = tiles * per;
     } else {
@@ -875,6 +885,7 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
         part.pieces = (uint32_t)((span + piece - 1) / piece);
         part.split = part.pieces > 1;
         items = (uint64_t)part.row_tiles * part.pieces;
+        if (a.causal && part.pieces == 1 && tiles > (uint64_t)dev->num_cus && tiles <= 3ull * dev->num_cus) part.round = (uint32_t)(dev->num_cus / per);
         join_tiles = part.row_tiles * per;
     }
     const uint64_t blocks = items * per;
