@@ -558,9 +558,9 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
             if (i * AT_WAVES + wave >= loads) break;
             uint32_t ko = k_off[i], vo = v_off[i];
             if (cut && t0 + (int32_t)l_row[i] >= s.keys) {
-                const uint32_t rr = (uint32_t)(s.keys - 1 - t0);
-                ko = rr * k_row + l_k[i];
-                vo = rr * v_row + l_v[i];
+                const uint32_t beyond = (uint32_t)(t0 + (int32_t)l_row[i] - (s.keys - 1));
+                ko -= beyond * k_row;
+                vo -= beyond * v_row;
             }
             at_to_lds(k0, ko, to + i * AT_WAVES * 1024);
             at_to_lds(v0, vo, to + i * AT_WAVES * 1024 + S::TILE);
@@ -638,15 +638,16 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
             at_in_order();
         }
         if (t0 + KT - 1 > limit_a || (t0 + KT > a.sinks && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
-            // key 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile
-            const int32_t lim = limit - t0 - 4 * (int32_t)half, near = p - t0 - 4 * (int32_t)half, sink = a.sinks - t0 - 4 * (int32_t)half;
+            // key t = 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile: p - t < window as t > p - window, which saturates where there is no window
+            int32_t lim = limit - t0 - 4 * (int32_t)half, from = __builtin_elementwise_sub_sat(p - t0 - 4 * (int32_t)half, a.window), sink = a.sinks - t0 - 4 * (int32_t)half;
+            asm volatile("" : "+v"(lim), "+v"(from), "+v"(sink));               // nothing of this is worth registers outside of masked tiles
             const uint64_t have = there >> (4 * half);
 #pragma unroll
             for (int kk = 0; kk < S::HALVES; kk++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int32_t t = 32 * kk + e % 4 + 8 * (e / 4);
-                    const bool seen = t <= lim && (near - t < a.window || t < sink) && (!PAGED || (have >> t) & 1);
+                    const bool seen = t <= lim && (t > from || t < sink) && (!PAGED || (have >> t) & 1);
                     x[kk][e] = seen ? x[kk][e] : -INFINITY;
                 }
         }
@@ -685,15 +686,24 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
                 const v2u lo = at_lds_turned(cur + from), hi = at_lds_turned(cur + (from + 8 * pitch));
                 v[at] = v4u{lo[0], lo[1], hi[0], hi[1]};
             };
-            auto weigh = [&](int u, int e) __attribute__((always_inline)) {     // weights 2e, 2e + 1 of group u's 8 in this lane
-                const float w0 = at_exp2(__builtin_fmaf(x[u / 2][8 * (u % 2) + 2 * e], c, -base)), w1 = at_exp2(__builtin_fmaf(x[u / 2][8 * (u % 2) + 2 * e + 1], c, -base));
-                l += w0 + w1;
-                w[u][e] = AtMma<T>::pack(w0, w1);
+            // the exponentials of weights 2e, 2e + 1 of group u's 8 in this lane, and, later, what is made of them: a wave would wait for an exponential it uses at once
+            auto weigh = [&](int u, int e) __attribute__((always_inline)) {
+                x[u / 2][8 * (u % 2) + 2 * e] = at_exp2(__builtin_fmaf(x[u / 2][8 * (u % 2) + 2 * e], c, -base));
+                x[u / 2][8 * (u % 2) + 2 * e + 1] = at_exp2(__builtin_fmaf(x[u / 2][8 * (u % 2) + 2 * e + 1], c, -base));
+            };
+            auto finish = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float w0 = x[u / 2][8 * (u % 2) + 2 * e], w1 = x[u / 2][8 * (u % 2) + 2 * e + 1];
+                    l += w0 + w1;
+                    w[u][e] = AtMma<T>::pack(w0, w1);
+                }
             };
 #pragma unroll
             for (int at = 0; at < FRONT; at++) read_v(at);
 #pragma unroll
             for (int e = 0; e < 4; e++) weigh(0, e);
+            finish(0);
             at_in_order();
 #pragma unroll
             for (int at = 0; at < P; at++) {
@@ -703,6 +713,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
                 if (u + 1 < GROUPS)
 #pragma unroll
                     for (int e = 4 * i / S::BLOCKS; e < 4 * (i + 1) / S::BLOCKS; e++) weigh(u + 1, e);
+                if (i == S::BLOCKS - 1 && u + 1 < GROUPS) finish(u + 1);
                 at_in_order();
             }
         } else {
