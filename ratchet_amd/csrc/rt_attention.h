@@ -12,6 +12,7 @@
 
 constexpr int AT_MAX_DIM = 512;                  // columns of a head
 constexpr int32_t AT_FAR = 0x7fffffff;           // window of a call without one
+constexpr int32_t AT_MOST_TOKENS = 1 << 30;      // rows, keys and positions lie below it, and their differences in 32 bits
 
 struct AttnArgs {
     const void* q;
@@ -82,7 +83,7 @@ template <bool PAGED> __device__ __forceinline__ AttnSeq at_seq(const AttnArgs& 
         lo = lo < 0 ? 0 : lo > top ? top : lo;
         hi = hi < lo ? lo : hi > top ? top : hi;
         int32_t len = a.lens[b];
-        len = len < 0 ? 0 : len;
+        len = len < 0 ? 0 : len < AT_MOST_TOKENS ? len : AT_MOST_TOKENS;
         s.first = (uint32_t)lo;
         s.count = (uint32_t)(hi - lo);
         s.keys = len < (int32_t)a.cap ? len : (int32_t)a.cap;
@@ -108,7 +109,6 @@ __device__ __forceinline__ int32_t at_limit(const AttnArgs& a, const AttnSeq& s,
 }
 // Position that the window counts from
 __device__ __forceinline__ int32_t at_position(const AttnSeq& s, uint32_t j) { return (int32_t)j + s.shift; }
-// p - t never wraps: both lie in [0, 2^31) wherever t <= limit
 __device__ __forceinline__ bool at_visible(const AttnArgs& a, int32_t t, int32_t limit, int32_t p) {
     return t <= limit && (p - t < a.window || t < a.sinks);
 }

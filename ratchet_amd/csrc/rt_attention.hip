@@ -154,7 +154,7 @@ int dispatch(rt_device* dev, int dt, AttnArgs& a, bool paged, const float* weigh
     }
 }
 
-constexpr uint32_t MOST_TOKENS = 1u << 30;       // positions and their differences stay in 32 bits
+constexpr uint32_t MOST_TOKENS = AT_MOST_TOKENS;
 
 int head_rules(const char* who, int dt, uint32_t heads, uint32_t kv_heads, uint32_t dim, float scale, uint32_t window, uint32_t sinks, AttnArgs& a) {
     RT_REQUIRE(rt_is_float_dt(dt), RT_ERR_DTYPE, "%s: dtype %d is not F32, F16 or BF16", who, dt);
@@ -169,8 +169,8 @@ int head_rules(const char* who, int dt, uint32_t heads, uint32_t kv_heads, uint3
     a.group_div = make_fastdiv(a.group);
     a.dim = dim;
     a.c = scale * 1.4426950408889634f;
-    a.window = window == 0 || window > (uint32_t)AT_FAR ? AT_FAR : (int32_t)window;
-    a.sinks = sinks > (uint32_t)AT_FAR ? AT_FAR : (int32_t)sinks;
+    a.window = window == 0 || window >= MOST_TOKENS ? AT_FAR : (int32_t)window;               // as far as positions go
+    a.sinks = sinks > MOST_TOKENS ? AT_MOST_TOKENS : (int32_t)sinks;
     return RT_OK;
 }
 

@@ -28,6 +28,7 @@ constexpr float AT_SLACK = 8.0f;                 // powers of two that a row's w
 // AT_TARGET items (Phi-2 prompt, 512 row tiles: 45 us whole, 55 to 57 shared out; chunks, about 100 row tiles: 152 us at 256 items, 125 at 768, 142 at 1536;
 // encoder, 288: 202, 149, 140).
 constexpr uint32_t AT_TARGET_FEW = 1024, AT_TARGET = 768, AT_ENOUGH = 512, AT_LEAST_TILES_FEW = 2, AT_LEAST_TILES = 4;
+constexpr size_t AT_MOST_PARTS = 1u << 30;       // bytes of parts; a launch that would leave more shares nothing out
 constexpr uint32_t AT_MOST_PIECES = 60;          // of a row tile: their factors for its 128 rows fit the LDS of the smallest tiles
 constexpr uint32_t AT_FEW_ROWS = 16;             // rows of a sequence and KV head, on average, up to which a launch joins its own pieces
 constexpr uint32_t AT_JOIN_ROWS = 16;            // rows to a block of the joining kernel
@@ -869,6 +870,7 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
     typedef AtShape<T, DT> S;
     AttnPartial part = {};
     const bool few = (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
+    const uint64_t most_blocks = AT_MOST_PARTS / (AT_ROWS * ((uint64_t)a.dim + 2) * sizeof(float));
     uint64_t join_tiles, items;                                 // row tiles; blocks per KV head (paged) or per (batch entry, KV head)
     const uint64_t per = PAGED ? a.kv_heads : (uint64_t)a.seqs * a.kv_heads;
     if (PAGED) {
@@ -877,7 +879,7 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
         const uint32_t target = few ? AT_TARGET_FEW : AT_TARGET, least = few ? AT_LEAST_TILES_FEW : AT_LEAST_TILES;
         items = tiles + (few ? 1 : 2) * target / a.kv_heads + 1;                // (twice where the work is a causal mean, at least half of the spans)
         const bool enough = !few && ((uint64_t)a.tokens * a.group + AT_ROWS - 1) / AT_ROWS * per >= AT_ENOUGH;                // at least so many row tiles
-        part.split = a.cap > least * S::KT && items * per <= RT_ARRIVALS && !enough;
+        part.split = a.cap > least * S::KT && items * per <= RT_ARRIVALS && items * per <= most_blocks && !enough;
         if (!part.split) items = tiles;
         join_tiles = tiles * per;
     } else {
@@ -891,7 +893,7 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
         const uint64_t tiles = part.row_tiles * per;
         uint64_t piece = few ? at_piece_for<true>(tiles, mean * tiles) : at_piece_for<false>(tiles, mean * tiles);
         piece = at_piece_of((uint32_t)(piece > span ? span : piece), (uint32_t)span);
-        if (part.row_tiles * ((span + piece - 1) / piece) * per > RT_ARRIVALS) piece = span;
+        if (part.row_tiles * ((span + piece - 1) / piece) * per > (most_blocks < RT_ARRIVALS ? most_blocks : RT_ARRIVALS)) piece = span;
         part.piece = (uint32_t)piece;
         part.pieces = (uint32_t)((span + piece - 1) / piece);
         part.split = part.pieces > 1;

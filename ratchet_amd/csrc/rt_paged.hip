@@ -27,8 +27,8 @@ template <typename VecT> __global__ void __launch_bounds__(BLOCK) paged_append_k
     hi = hi > top ? top : hi;
     if ((int32_t)token < lo || (int32_t)token >= hi) return;
     int32_t len = a.lens[b];
-    len = len < 0 ? 0 : len;
-    const int32_t t = len - hi + (int32_t)token;               // both below 2^31
+    len = len < 0 ? 0 : len < AT_MOST_TOKENS ? len : AT_MOST_TOKENS;
+    const int32_t t = len - hi + (int32_t)token;
     if (t < 0) return;
     uint32_t at, slot;
     fd_divmod((uint32_t)t, a.page_div, at, slot);

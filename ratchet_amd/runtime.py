@@ -7,6 +7,7 @@ This mirrors the storage/dispatch seam of ratchet-core that the native library r
 Every method enqueues on the device's single stream; Device.sync() / Buffer.to_numpy() block.
 """
 import ctypes
+import functools
 
 import numpy as np
 
@@ -177,22 +178,23 @@ class PagedCache:
         return (self.seqs, self.kv_heads, self.table_len * self.page_len)
 
 
-def _require(ok, what):
-    if not ok:
-        raise ValueError(what)
+@functools.lru_cache(maxsize=4096)
+def _checked_strides(shape, strides, offset, numel):
+    strides = tuple(map(int, strides))
+    if min(strides) < 0:
+        raise ValueError(f"negative stride in {strides}")
+    last = offset + sum((n - 1) * s for n, s in zip(shape, strides)) + (shape[-1] - 1 if len(strides) < len(shape) else 0)
+    if last >= numel:
+        raise ValueError(f"{shape} with strides {strides} reaches beyond its buffer")
+    return strides_array(strides)
 
 
 def _strided(x, strides):
     """what the library takes for `strides` (elements, one for each extent of x but the last where x is a row list), checked against the memory behind x"""
     if strides is None:
         return None
-    strides = tuple(map(int, strides))
     parent = getattr(x, "parent", x)
-    at = (x.ptr.value - parent.ptr.value) // _DT_BYTES[x.dt]
-    _require(min(strides) >= 0, f"negative stride in {strides}")
-    last = at + sum((n - 1) * s for n, s in zip(x.shape, strides)) + (x.shape[-1] - 1 if len(strides) < len(x.shape) else 0)
-    _require(last < parent.numel, f"{x.shape} with strides {strides} reaches beyond its buffer")
-    return strides_array(strides)
+    return _checked_strides(x.shape, tuple(strides), 0 if parent is x else (x.ptr.value - parent.ptr.value) // _DT_BYTES[x.dt], parent.numel)
 
 
 class Device:
@@ -424,11 +426,15 @@ class Device:
         """softmax(scale q k^T over the visible keys) v: q [B, heads, Sq, D], k and v [B, kv_heads, Sk, D]; the strides (elements, one for each extent) say
         where they lie in memory, out's too.  lens: I32 [B], the keys of each entry; the last query is at the last key.  window: a query
         sees that many last keys and the first `sinks`; scale: 1 / sqrt(D) unless given; lse: F32 [B, heads, Sq] for the log of each row's sum."""
-        _require(len(q.shape) == 4 and len(k.shape) == 4 and k.shape == v.shape and q.dt == k.dt == v.dt, f"attention of {q.shape}, {k.shape}, {v.shape}")
-        _require(lens is None or (lens.dt == _lib.I32 and lens.shape == (q.shape[0],)), "lens has to be I32 [B]")
+        if not (len(q.shape) == 4 and len(k.shape) == 4 and k.shape == v.shape and q.dt == k.dt == v.dt):
+            raise ValueError(f"attention of {q.shape}, {k.shape}, {v.shape}")
+        if not (lens is None or (lens.dt == _lib.I32 and lens.shape == (q.shape[0],))):
+            raise ValueError("lens has to be I32 [B]")
         out = out or Buffer(self, q.shape, q.dt)
-        _require(out.dt == q.dt and out.numel == q.numel and (lse is None or (lse.dt == _lib.F32 and lse.numel * q.shape[3] == q.numel)), "out or lse does not fit")
-        _require(out_strides is None or out.shape == q.shape, "out with strides has the shape of q")
+        if not (out.dt == q.dt and out.numel == q.numel and (lse is None or (lse.dt == _lib.F32 and lse.numel * q.shape[3] == q.numel))):
+            raise ValueError("out or lse does not fit")
+        if not (out_strides is None or out.shape == q.shape):
+            raise ValueError("out with strides has the shape of q")
         check(self.lib.rt_attention(self.handle, q.dt, q.ptr, buffer_shape4(q.shape), _strided(q, q_strides), k.ptr, _strided(k, k_strides), v.ptr, _strided(v, v_strides),
                                     buffer_shape4(k.shape), lens.ptr if lens is not None else None, out.ptr, _strided(out, out_strides), lse.ptr if lse is not None else None,
                                     q.shape[3] ** -0.5 if scale is None else scale, 1 if causal else 0, window, sinks))
@@ -440,22 +446,29 @@ class Device:
     def paged_append(self, cache, starts, k, v, k_strides=None, v_strides=None):
         """Rows of k and v [tokens, kv_heads, head_dim] into the cache: rows starts[b] .. starts[b + 1] - 1 are the last tokens that cache.lens counts
         of sequence b.  starts: I32 [seqs + 1]; strides: elements from token to token and from head to head."""
-        _require(k.shape == v.shape and k.shape[1:] == (cache.kv_heads, cache.head_dim) and k.dt == v.dt == cache.dt, f"{k.shape} and {v.shape} do not fit the cache")
-        _require(starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,), "starts has to be I32 [seqs + 1]")
+        if not (k.shape == v.shape and k.shape[1:] == (cache.kv_heads, cache.head_dim) and k.dt == v.dt == cache.dt):
+            raise ValueError(f"{k.shape} and {v.shape} do not fit the cache")
+        if not (starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,)):
+            raise ValueError("starts has to be I32 [seqs + 1]")
         check(self.lib.rt_paged_append(self.handle, _DT_BYTES[cache.dt], cache.ref, starts.ptr, k.shape[0], k.ptr, _strided(k, k_strides), v.ptr, _strided(v, v_strides)))
         return cache
 
     def paged_attention(self, q, cache, starts, window=0, sinks=0, scale=None, q_strides=None, out=None, lse=None, weights=None, weights_out=None):
         """Causal attention of the new tokens q [tokens, heads, head_dim] (starts as in paged_append, whose rows are in the cache already).
         weights: F32 cache.weights_shape, the attention weight each cached token has received, updated in place or into weights_out."""
-        _require(len(q.shape) == 3 and q.shape[2] == cache.head_dim and q.dt == cache.dt, f"{q.shape} does not fit the cache")
-        _require(starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,), "starts has to be I32 [seqs + 1]")
+        if not (len(q.shape) == 3 and q.shape[2] == cache.head_dim and q.dt == cache.dt):
+            raise ValueError(f"{q.shape} does not fit the cache")
+        if not (starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,)):
+            raise ValueError("starts has to be I32 [seqs + 1]")
         out = out or Buffer(self, q.shape, q.dt)
-        _require(out.dt == q.dt and out.numel == q.numel and (lse is None or (lse.dt == _lib.F32 and lse.numel * q.shape[2] == q.numel)), "out or lse does not fit")
-        _require(weights is not None or weights_out is None, "weights_out without weights")
+        if not (out.dt == q.dt and out.numel == q.numel and (lse is None or (lse.dt == _lib.F32 and lse.numel * q.shape[2] == q.numel))):
+            raise ValueError("out or lse does not fit")
+        if not (weights is not None or weights_out is None):
+            raise ValueError("weights_out without weights")
         if weights is not None:
             weights_out = weights if weights_out is None else weights_out
-            _require(weights.dt == weights_out.dt == _lib.F32 and weights.shape == weights_out.shape == cache.weights_shape, f"weights have to be F32 {cache.weights_shape}")
+            if not (weights.dt == weights_out.dt == _lib.F32 and weights.shape == weights_out.shape == cache.weights_shape):
+                raise ValueError(f"weights have to be F32 {cache.weights_shape}")
         check(self.lib.rt_paged_attention(self.handle, q.dt, q.ptr, _strided(q, q_strides), q.shape[0], q.shape[1], cache.ref, starts.ptr, out.ptr,
                                           lse.ptr if lse is not None else None, weights.ptr if weights is not None else None,
                                           weights_out.ptr if weights is not None else None, q.shape[2] ** -0.5 if scale is None else scale, window, sinks))
@@ -466,7 +479,9 @@ class Device:
         on its own, in their order: in place, or into the pages of the table `to` (none of them in use by the cache), lens_out and weights_out.
         Returns the cache with what it then holds."""
         to, lens_out, weights_out = to or cache.table, lens_out or cache.lens, weights_out or weights
-        _require(to.dt == lens_out.dt == _lib.I32 and to.shape == cache.table.shape and lens_out.shape == cache.lens.shape, "to or lens_out does not fit the cache")
-        _require(weights.dt == weights_out.dt == _lib.F32 and weights.shape == weights_out.shape == cache.weights_shape, f"weights have to be F32 {cache.weights_shape}")
+        if not (to.dt == lens_out.dt == _lib.I32 and to.shape == cache.table.shape and lens_out.shape == cache.lens.shape):
+            raise ValueError("to or lens_out does not fit the cache")
+        if not (weights.dt == weights_out.dt == _lib.F32 and weights.shape == weights_out.shape == cache.weights_shape):
+            raise ValueError(f"weights have to be F32 {cache.weights_shape}")
         check(self.lib.rt_paged_evict(self.handle, _DT_BYTES[cache.dt], cache.ref, weights.ptr, keep, first, recent, to.ptr, lens_out.ptr, weights_out.ptr))
         return cache if to is cache.table and lens_out is cache.lens else PagedCache(cache.k_pages, cache.v_pages, to, lens_out)

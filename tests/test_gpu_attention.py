@@ -465,3 +465,118 @@ def test_the_same_call_gives_the_same_bits(dev, dtype):
         out = dev.paged_attention(q, cache, starts, weights=w_in, weights_out=w_out)
         seen.append(out.to_numpy().tobytes() + w_out.to_numpy().tobytes())
     assert len(set(seen)) == 1
+
+
+# ---------------------------------------------------------------------------------------------------- large and odd
+@pytest.mark.parametrize("queries", [1, 70])
+def test_keys_beyond_4_gib(dev, queries):
+    """2^25 keys of 128 bytes; a window over the last ones and two sinks at the other end"""
+    rng = np.random.default_rng(queries)
+    keys, window = 1 << 25, 500
+    k, v = dev.empty((1, 1, keys, 64), _lib.F16), dev.empty((1, 1, keys, 64), _lib.F16)
+    tail = window + queries
+    rows = {}
+    for name, buf in (("k", k), ("v", v)):
+        first, last = ref.rounded(rng.standard_normal((2, 64)), "f16"), ref.rounded(rng.standard_normal((tail, 64)), "f16")
+        buf.view(0, (2, 64)).upload(ref.raw(first, "f16"))
+        buf.view((keys - tail) * 64, (tail, 64)).upload(ref.raw(last, "f16"))
+        rows[name] = np.concatenate([first, last])
+    q = ref.rounded(rng.standard_normal((1, 1, queries, 64)), "f16")
+    got = ref.values(dev.attention(ref.upload(dev, q, "f16"), k, v, window=window, sinks=2).to_numpy(), "f16")
+    p, t = np.arange(queries)[:, None] + keys - queries, np.concatenate([np.arange(2), np.arange(keys - tail, keys)])[None, :]
+    o, _, _, off, _, _ = ref.head(q[0, 0], rows["k"], rows["v"], (t <= p) & ((p - t < window) | (t < 2)), 0.125, "f16")
+    ref.check(got[0, 0], o, off, "o")
+
+
+@pytest.mark.parametrize("new", [[1, 1], [1, 200]])
+def test_pages_beyond_4_gib(dev, new):
+    """append, attention, received weights and eviction on pages on either side of byte 2^32 of the pools"""
+    from test_gpu_paged import host_append, host_evict
+
+    rng = np.random.default_rng(sum(new))
+    p = ref.Paged(rng, "f16", 4, 2, 64, 32, [400, 300], new, spare=1)
+    per = 2 * 32 * 64                                          # elements of a page
+    pages = (1 << 32) // (2 * per) + 40
+    where = np.sort(rng.choice(np.concatenate([np.arange(20), np.arange(pages - 60, pages)]), p.pages, replace=False))
+    kb, vb = dev.empty((pages, 2, 32, 64), _lib.F16), dev.empty((pages, 2, 32, 64), _lib.F16)
+    for i, at in enumerate(where):
+        kb.view(int(at) * per, (per,)).upload(ref.raw(p.k[i], "f16").ravel())
+        vb.view(int(at) * per, (per,)).upload(ref.raw(p.v[i], "f16").ravel())
+    table = np.where(p.table >= 0, where[np.maximum(p.table, 0)], -1).astype(np.int32)
+    cache = dev.paged_cache(kb, vb, dev.upload(table), dev.upload(p.lens.astype(np.int32)))
+    k, v = (ref.rounded(rng.standard_normal((p.tokens, 2, 64)), "f16") for _ in range(2))
+    starts, w = dev.upload(p.starts), rng.random((2, 2, p.cap), dtype=np.float32)
+    w_dev = dev.upload(w)
+    dev.paged_append(cache, starts, ref.upload(dev, k, "f16"), ref.upload(dev, v, "f16"))
+    host_append(p, k, v)
+    got = ref.values(dev.paged_attention(ref.upload(dev, p.q, "f16"), cache, starts, weights=w_dev).to_numpy(), "f16")
+    o, _, received, off, _, r_off = p.attention(0.125, weights=w)
+    ref.check(got, o, off, "o")
+    there = np.arange(p.cap)[None, None] < p.lens[:, None, None] + np.zeros((1, 2, 1), int)
+    now = w_dev.to_numpy()
+    ref.check(now[there], received[there], r_off[there], "weights")
+    dev.paged_evict(cache, w_dev, 100, first=4, recent=20)
+    host_evict(p, now, 100, 4, 20)
+    for i, at in enumerate(where):
+        assert np.array_equal(ref.values(kb.view(int(at) * per, (2, 32, 64)).to_numpy(), "f16"), p.k[i]), i
+        assert np.array_equal(ref.values(vb.view(int(at) * per, (2, 32, 64)).to_numpy(), "f16"), p.v[i]), i
+
+
+@pytest.mark.parametrize("seqs, cap_pages", [(200, 300), (3, 40000)])
+def test_more_room_than_blocks(dev, seqs, cap_pages):
+    """weights of chunks where the table has room for far more keys than there are"""
+    rng = np.random.default_rng(seqs)
+    lens = rng.integers(1, 300, seqs)
+    p = ref.Paged(rng, "f16", 2, 1, 32, 16, lens, np.minimum(rng.integers(10, 60, seqs), lens), spare=cap_pages)
+    paged(dev, p, weights=rng.random((seqs, 1, p.cap), dtype=np.float32))
+
+
+def test_many_ragged_chunks(dev):
+    """row tiles of many lengths, whose pieces add up to the most that a launch has room for"""
+    for seed in range(4):
+        rng = np.random.default_rng(seed)
+        lens = rng.integers(1, 1500, 20)
+        new = np.maximum(1, (lens * rng.random(20) ** 2).astype(int))
+        paged(dev, ref.Paged(rng, "bf16", 4, 2, 64, 16, lens, new))
+    rng = np.random.default_rng(9)
+    lens = np.array([9000] + [300] * 12)                        # one long walk among short ones
+    paged(dev, ref.Paged(rng, "bf16", 8, 1, 64, 16, lens, [140] + [129] * 12))
+
+
+@pytest.mark.parametrize("queries", [1, 140])
+@pytest.mark.parametrize("window", [1 << 30, (1 << 31) - 2, 1 << 31])
+def test_windows_wider_than_any_position(dev, queries, window):
+    dense(dev, np.random.default_rng(1), "f16", 1, 2, 1, queries, 100, 64, window=window, sinks=1)
+
+
+def test_lens_far_beyond_the_table(dev):
+    """tokens that there is no room for: the queries sit behind all keys, and a window has passed those that are there"""
+    rng = np.random.default_rng(2)
+    for window, sinks in ((0, 0), (10, 0), (10, 3)):
+        p = ref.Paged(rng, "f16", 4, 2, 64, 16, np.array([60, 20]), np.array([1, 40]), spare=0)
+        p.lens = np.array([(1 << 30) - 1, 1000])
+        paged(dev, p, window=window, sinks=sinks, weights=rng.random((2, 2, p.cap), dtype=np.float32))
+
+
+def test_two_devices_at_once():
+    """two rt_devices of one GPU have their own streams and workspaces: calls that overlap do not meet"""
+    from ratchet_amd import Device
+
+    devs = [Device(0), Device(0)]
+    rng = np.random.default_rng(3)
+    runs = []
+    for d in devs:
+        p = ref.Paged(rng, "bf16", 8, 2, 128, 16, [3000, 900, 12], [1, 1, 1])
+        w = rng.random((3, 2, p.cap), dtype=np.float32)
+        cache = d.paged_cache(ref.upload(d, p.k, "bf16"), ref.upload(d, p.v, "bf16"), d.upload(p.table), d.upload(p.lens.astype(np.int32)))
+        args = ref.upload(d, p.q, "bf16"), cache, d.upload(p.starts)
+        out, w_in, w_out = d.empty(p.q.shape, _lib.BF16), d.upload(w), d.upload(np.zeros_like(w))
+        d.paged_attention(*args, out=out, weights=w_in, weights_out=w_out)
+        runs.append((d, args, out, w_in, w_out, out.to_numpy(), w_out.to_numpy()))
+    for _ in range(20):
+        for d, args, out, w_in, w_out, *_ in runs:
+            d.paged_attention(*args, out=out, weights=w_in, weights_out=w_out)
+    for d, _, out, _, w_out, want, want_w in runs:
+        assert np.array_equal(out.to_numpy(), want) and np.array_equal(w_out.to_numpy(), want_w)
+    for d in devs:
+        d.close()
