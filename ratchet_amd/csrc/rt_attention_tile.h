@@ -183,8 +183,9 @@ __device__ __forceinline__ v2u at_lds_turned(const lds_byte* at) {
 // 16 bytes a lane from memory to LDS, lane i's to at + 16 i (at: the same in all lanes).  Whoever reads them waits for vmcnt(0) first.  Written as an instruction, which
 // has no result the compiler could misplace: after the builtin the compiler holds every LDS read for a possible flat access in flight, and waits
 // for all reads where it needs one (s_waitcnt lgkmcnt(0) before each product).
-__device__ __forceinline__ void at_to_lds(const void* from, lds_byte* at) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"((uint32_t)(uintptr_t)at) : "memory");
+template <bool ONCE = false> __device__ __forceinline__ void at_to_lds(const void* from, lds_byte* at) {
+    if (ONCE) asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(from), "{m0}"((uint32_t)(uintptr_t)at) : "memory");
+    else asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"((uint32_t)(uintptr_t)at) : "memory");
 }
 // The same with a base that all lanes share.  s_nop 4: a scalar register that a vector instruction wrote (v_readlane) may be read five states later.
 __device__ __forceinline__ void at_to_lds(const void* base, uint32_t offset, lds_byte* at) {
@@ -545,8 +546,8 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
 #pragma unroll
             for (int i = 0; i < S::LOADS; i++) {
                 if (i * AT_WAVES + wave >= loads) break;
-                at_to_lds(kb + next_off[i] + l_k[i], to + i * AT_WAVES * 1024);
-                at_to_lds(vb + next_off[i] + l_v[i], to + i * AT_WAVES * 1024 + S::TILE);
+                at_to_lds<FEW>(kb + next_off[i] + l_k[i], to + i * AT_WAVES * 1024);
+                at_to_lds<FEW>(vb + next_off[i] + l_v[i], to + i * AT_WAVES * 1024 + S::TILE);
             }
             return;
         }
