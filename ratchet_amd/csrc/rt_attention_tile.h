@@ -164,14 +164,29 @@ template <> struct AtMma<bf16_t> {
     static constexpr uint32_t SIGNS = 0x80008000u;
 };
 template <> struct AtMma<float> {
-    static __device__ __forceinline__ v16f qk(v4u k, v4u q, v16f s) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q[e]), s, 0, 0, 0);
-        return s;
+    static __device__ __forceinline__ v16f one(uint32_t k, uint32_t q, v16f s) {
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k), __uint_as_float(q), s, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float, float) { return 0; }
     static constexpr uint32_t SIGNS = 0x80000000u;
 };
+
+// The products of a pair of chunks, added to a score's SUMS sums: s and the others
+template <typename T, int SUMS> __device__ __forceinline__ void at_score(v4u k, v4u q, v16f& s, v16f (&others)[SUMS]) {
+    if constexpr (sizeof(T) == 2) {
+        s = AtMma<T>::qk(k, q, s);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (e % SUMS == 0) s = AtMma<T>::one(k[e], q[e], s);
+            else others[e % SUMS] = AtMma<T>::one(k[e], q[e], others[e % SUMS]);
+        }
+    }
+}
+template <int SUMS> __device__ __forceinline__ void at_join_sums(v16f& s, v16f (&others)[SUMS]) {
+    if constexpr (SUMS == 4) s = (s + others[1]) + (others[2] + others[3]);
+    if constexpr (SUMS == 2) s = s + others[1];
+}
 
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 __device__ __forceinline__ v4u at_lds16(const lds_byte* at) { return *(const __attribute__((address_space(3))) v4u*)at; }
@@ -207,12 +222,14 @@ template <typename T, int DT> struct AtShape {
     static constexpr int BLOCKS = (DT + 31) / 32;              // 32-column blocks of the result
     static constexpr int KT = sizeof(T) == 2 && DT <= 128 ? 64 : 32;
     static constexpr int HALVES = KT / 32;
+    // Sums that a score is kept in while it grows: a f32 product adds two columns at a time, and 128 additions in a row lose twice what 32 do (a 16-bit one adds 16)
+    static constexpr int SUMS = sizeof(T) == 2 || DT <= 64 ? 1 : DT <= 128 ? 2 : 4;
     static constexpr int CHUNKS = DT / CE;                     // of a row, at most
     static constexpr int LOADS = (KT * CHUNKS + AT_BLOCK - 1) / AT_BLOCK;      // of a tile of keys (or values), by each wave
     // a wave's last load of a tile may reach beyond it, and so may the transposed reads of the last block of columns
     static constexpr int TILE = (KT * CHUNKS * 16 + 1023) / 1024 * 1024;
     static constexpr int LDS = 4 * TILE + 256;
-    static constexpr int WAVES = DT > 128 ? 1 : DT > 96 ? 2 : 3;             // of a SIMD: what its registers are shared by
+    static constexpr int WAVES = DT > 128 ? 1 : DT > (sizeof(T) == 2 ? 96 : 64) ? 2 : 3;             // of a SIMD: what its registers are shared by
 };
 
 // 16-byte chunks of a row are rotated by an amount that goes by the row, so that what the lanes of one access read spreads over the banks: keys are read a
@@ -230,6 +247,14 @@ template <typename T> __device__ __forceinline__ uint32_t at_turn_v(uint32_t row
 // Left to itself the compiler reads an operand from LDS, waits for it and multiplies, one at a time.  A step is therefore written in the order it runs in: reads
 // some products in front of their uses, the next keys' exponentials between the products of the last, and a fence for the scheduler after each product.
 __device__ __forceinline__ void at_in_order() { __builtin_amdgcn_sched_barrier(0); }
+// After a chain of products, `sum` being the last one's: reads it in the products' own block, so that the matrix unit is waited for there. Left to the reads behind a
+// branch over a few instructions, the compiler counts the wait states of the longer way only, and what comes the shorter way reads sums that are not there yet (f32
+// rows of 80 columns were off by 4e-2 for it)
+__device__ __forceinline__ void at_settle(const v16f& sum) {
+    at_in_order();
+    asm volatile("" : : "s"(__builtin_amdgcn_readfirstlane(__float_as_uint(sum[15]))));
+    at_in_order();
+}
 
 // One row over the keys of tiles [tile0, tile1) of a walk, a lane to a key for the scores and to columns for the result: visible keys alone are touched.
 template <typename T, int DT, bool PAGED, int KT>
@@ -430,9 +455,10 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
 
 // FEW: pieces are joined by the block that comes last, and scores are left where they are wanted
 template <typename T, int DT, bool EXACT, bool PAGED, bool FEW>
-__global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES, AtShape<T, DT>::WAVES))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
+__global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES + (DT <= 64 && !PAGED && !FEW), AtShape<T, DT>::WAVES + (DT <= 64 && !PAGED && !FEW)))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
     typedef AtShape<T, DT> S;
     constexpr int KT = S::KT, CE = S::CE;
+    constexpr int SUMS = sizeof(T) == 4 && (PAGED || FEW) ? (S::SUMS > 2 ? S::SUMS : 2) : S::SUMS;  // 64 columns have registers for two where three waves share them
     extern __shared__ __align__(16) unsigned char smem[];
     lds_byte* const lds = (lds_byte*)smem;
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 32, half = lane / 32;
@@ -617,9 +643,13 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         if (!busy || t0 > limit_z || (t0 >= a.sinks && p_a - (t0 + KT - 1) >= a.window)) return;
 
         constexpr int N = S::STEPS * S::HALVES, AHEAD = N < 4 ? N : 4;
-        v16f x[S::HALVES];
+        v16f x[S::HALVES], others[S::HALVES][SUMS];
 #pragma unroll
-        for (int kk = 0; kk < S::HALVES; kk++) x[kk] = v16f{0};
+        for (int kk = 0; kk < S::HALVES; kk++) {
+            x[kk] = v16f{0};
+#pragma unroll
+            for (int z = 1; z < SUMS; z++) others[kk][z] = v16f{0};
+        }
         v4u k[N];
         auto read_k = [&](int at) __attribute__((always_inline)) {              // product `at`: step at / HALVES of half at % HALVES
             const int i = at / S::HALVES, kk = at % S::HALVES;
@@ -634,11 +664,14 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
             const int i = at / S::HALVES, kk = at % S::HALVES;
             if (EXACT || (uint32_t)(2 * i * CE) < D) {
                 if ((EXACT ? DT % (2 * CE) != 0 : true) && (2 * i + 2) * CE > (int)D && half) k[at] = v4u{0, 0, 0, 0};
-                x[kk] = AtMma<T>::qk(k[at], q[i], x[kk]);
+                at_score<T>(k[at], q[i], x[kk], others[kk]);
             }
             if (at + AHEAD < N) read_k(at + AHEAD);
             at_in_order();
         }
+        at_settle(SUMS == 1 ? x[S::HALVES - 1] : others[S::HALVES - 1][SUMS - 1]);
+#pragma unroll
+        for (int kk = 0; kk < S::HALVES; kk++) at_join_sums(x[kk], others[kk]);
         if (t0 + KT - 1 > limit_a || (t0 + KT > a.sinks && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
             // key t = 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile: p - t < window as t > p - window, which saturates where there is no window
             int32_t lim = limit - t0 - 4 * (int32_t)half, from = __builtin_elementwise_sub_sat(p - t0 - 4 * (int32_t)half, a.window), sink = a.sinks - t0 - 4 * (int32_t)half;
@@ -668,7 +701,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
             for (int e = 0; e < 16; e++) top = fmaxf(top, x[kk][e]);
         top = fmaxf(top, at_other(top)) * c;
         // m follows the maximum at a distance: a weight of up to 2^AT_SLACK loses nothing in f32, f16 or bf16, and of 32 rows one has a new maximum in nearly every tile
-        if (__ballot(top > m + AT_SLACK)) {
+        if (__ballot(top > m + (FEW ? 0.0f : AT_SLACK))) {
             const float m_new = fmaxf(m, top), old = at_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
             m = m_new;
             l *= old;
@@ -760,6 +793,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
     }
 
     // ---- result: lane's columns of d are 32 i + 8 (e / 4) + 4 half + e % 4
+    at_settle(o[S::BLOCKS - 1]);
     l += at_other(l);
     bool fine = __builtin_isfinite(l) && m < INFINITY;
 #pragma unroll
@@ -942,9 +976,9 @@ template <typename T> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool pag
     if (!fits) return RT_OK;
 #define RT_TILE(DT, EXACT) return paged ? at_launch_tile<T, DT, EXACT, true>(dev, a) : at_launch_tile<T, DT, EXACT, false>(dev, a)
     if (a.dim == 64) RT_TILE(64, true);
-    if (sizeof(T) == 2 && a.dim == 80) RT_TILE(80, true);
-    if (sizeof(T) == 2 && a.dim == 96) RT_TILE(96, true);
-    if (sizeof(T) == 2 && a.dim == 128) RT_TILE(128, true);
+    if (a.dim == 80) RT_TILE(80, true);
+    if (a.dim == 96) RT_TILE(96, true);
+    if (a.dim == 128) RT_TILE(128, true);
     if (a.dim <= 128) RT_TILE(128, false);
     RT_TILE(256, false);
 #undef RT_TILE

@@ -54,7 +54,7 @@ template <int N> __device__ __forceinline__ void aw_wait() { asm volatile("s_wai
 
 // The block's four waves share the queries, which go through stages of LDS, two on their way while one is worked on (one where rows are too wide for three).  Bound by the exponentials for prompts.
 template <typename T, int DT, bool EXACT>
-__global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : DT > 96 ? 2 : 3) attention_weights_kernel(AttnArgs a, const float* weights, float* out) {
+__global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : DT > 96 || sizeof(T) == 4 ? 2 : 3) attention_weights_kernel(AttnArgs a, const float* weights, float* out) {
     typedef AwShape<T, DT, EXACT> S;
     constexpr int CE = S::CE;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -150,7 +150,9 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : DT > 96 ? 2 : 3) atte
             stage = stage == S::STAGES - 1 ? 0 : stage + 1;
             if (!busy) continue;
             constexpr int N = 2 * S::STEPS, AHEAD = N < 4 ? N : 4;
-            v16f x[2] = {v16f{0}, v16f{0}};
+            v16f x[2] = {v16f{0}, v16f{0}}, others[2][S::SUMS];
+#pragma unroll
+            for (int z = 1; z < S::SUMS; z++) others[0][z] = others[1][z] = v16f{0};
             v4u q[N];
             auto read_q = [&](int p) __attribute__((always_inline)) {
                 if (!EXACT && (uint32_t)(p / 2 * 2 * CE) >= D) return;
@@ -164,10 +166,13 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : DT > 96 ? 2 : 3) atte
             for (int p = 0; p < N; p++) {
                 // where the row ends in a half chunk, both operands' other half holds what is not theirs: k's is 0 and q's has to be
                 if ((EXACT ? DT % (2 * CE) != 0 : true) && (p / 2 * 2 + 2) * CE > (int)D && half) q[p] = v4u{0, 0, 0, 0};
-                if (EXACT || (uint32_t)(p / 2 * 2 * CE) < D) x[p % 2] = AtMma<T>::qk(k[p / 2], q[p], x[p % 2]);
+                if (EXACT || (uint32_t)(p / 2 * 2 * CE) < D) at_score<T>(k[p / 2], q[p], x[p % 2], others[p % 2]);
                 if (p + AHEAD < N) read_q(p + AHEAD);
                 at_in_order();
             }
+            at_settle(S::SUMS == 1 ? x[1] : others[1][S::SUMS - 1]);
+            at_join_sums(x[0], others[0]);
+            at_join_sums(x[1], others[1]);
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const uint32_t row = r0 + n * AW_ROWS + 32 * y + col;
@@ -252,10 +257,10 @@ template <typename T> int aw_dispatch(rt_device* dev, const AttnArgs& a, const f
         return RT_OK;
     }
     if (a.dim == 64) return aw_launch<T, 64, true>(dev, a, weights, out);
-    if (sizeof(T) == 2 && a.dim == 80) return aw_launch<T, 80, true>(dev, a, weights, out);
-    if (sizeof(T) == 2 && a.dim == 96) return aw_launch<T, 96, true>(dev, a, weights, out);
-    if (sizeof(T) == 2 && a.dim == 128) return aw_launch<T, 128, true>(dev, a, weights, out);
-    if (a.dim <= 128) return aw_launch<T, 128, false>(dev, a, weights, out);
+    if (a.dim == 80) return aw_launch<T, 80, true>(dev, a, weights, out);
+    if (a.dim == 96) return aw_launch<T, 96, true>(dev, a, weights, out);
+    if (a.dim == 128) return aw_launch<T, 128, true>(dev, a, weights, out);
+    if (a.dim < 128) return aw_launch<T, 128, false>(dev, a, weights, out);
     return aw_launch<T, 256, false>(dev, a, weights, out);
 }
 
