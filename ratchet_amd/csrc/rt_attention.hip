@@ -9,6 +9,7 @@ constexpr int WAVES = 4, BLOCK = 64 * WAVES;
 
 // A wave to a (query, head) row.  A lane computes the score of one key of a tile of 64; the tile's weights then go round the wave, key by key, and
 // each lane adds them to its columns.  Hidden keys are skipped there, so nothing they hold is ever multiplied.
+// Simple, and 50 to 800 times slower than the tiles: bound by its scalar dot products and uncoalesced key reads ([4,6,1500,64] f32 14.5 ms, with tiles 0.15)
 template <typename T, bool PAGED>
 __global__ void __launch_bounds__(BLOCK) attention_any_kernel(AttnArgs a, uint64_t rows) {
     const uint32_t lane = threadIdx.x % 64;

@@ -10,6 +10,15 @@
 //
 // What hidden keys hold is kept out of the scores by a select and out of the maxima and sums by that; their values meet a weight of 0, and 0 times
 // what is not finite is NaN, which stays.  So a row tile whose result is not finite is computed again, one row at a time, over the visible keys only.
+//
+// Roundings below f32: the weights of 16-bit types are rounded to the type for the second product, as its operands have to be (their f32 values make the sums);
+// everything else, scores, m, l and O, is f32.  An m that lags by up to AT_SLACK powers of two makes weights up to 2^8: rounded relative to themselves, so nothing
+// is lost, and f16's largest is 2^16.
+//
+// What bounds it, by counters: 8192 tokens of 32 heads of 96 with a window of 2047, bf16: 227 to 236 us, 770 to 800 TFLOP/s of the visible pairs' products; the
+// matrix units are busy 47 % and the vector units (scores to weights: about eight instructions each) 62 % of the time, and three waves of a SIMD have both overlap
+// only in part.  f32, [4,6,1500,64]: 154 us, 79 % of it the matrix units, whose f32 products do an eighth of the 16-bit ones' work.  Single tokens, 64 of about
+// 4600 keys in bf16: 242 us, the keys and values once at 5.0 TB/s; a copy reaches 5.2.
 #ifndef RT_ATTENTION_TILE_H
 #define RT_ATTENTION_TILE_H
 
@@ -28,6 +37,7 @@ constexpr float AT_SLACK = 8.0f;                 // powers of two that a row's w
 // AT_TARGET items (Phi-2 prompt, 512 row tiles: 45 us whole, 55 to 57 shared out; chunks, about 100 row tiles: 152 us at 256 items, 125 at 768, 142 at 1536;
 // encoder, 288: 202, 149, 140).
 constexpr uint32_t AT_TARGET_FEW = 1024, AT_TARGET = 768, AT_ENOUGH = 512, AT_LEAST_TILES_FEW = 2, AT_LEAST_TILES = 4;
+constexpr uint32_t AT_SHORT = 40;                // tiles of keys to a row tile
 constexpr size_t AT_MOST_PARTS = 1u << 30;       // bytes of parts; a launch that would leave more shares nothing out
 constexpr uint32_t AT_MOST_PIECES = 60;          // of a row tile: their factors for its 128 rows fit the LDS of the smallest tiles
 constexpr uint32_t AT_FEW_ROWS = 16;             // rows of a sequence and KV head, on average, up to which a launch joins its own pieces
@@ -453,7 +463,8 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
     }
 }
 
-// FEW: pieces are joined by the block that comes last, and scores are left where they are wanted
+// FEW: pieces are joined by the block that comes last (a joining launch took 10 to 13 us more), and scores are left where they are
+// wanted.  Waves of a SIMD: as many as the registers let, four where the rows have 64 columns and no page table is followed (encoder in f32: 146.5 us a call, with three 148.7)
 template <typename T, int DT, bool EXACT, bool PAGED, bool FEW>
 __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES + (DT <= 64 && !PAGED && !FEW), AtShape<T, DT>::WAVES + (DT <= 64 && !PAGED && !FEW)))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
     typedef AtShape<T, DT> S;
@@ -862,6 +873,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         at_join<T, true>(a, part, s, b, g, row0, 0, rows, first, stride, used, (float*)smem);
 }
 
+// Parts of a row to the row: bound by reading them, 96 KB a row tile and piece in two 64 KB or more (encoder: 10 us, ragged chunks: 16 us with their search).
 // blockIdx.y: which AT_JOIN_ROWS of a row tile.  blockIdx.x: paged: KV head, sequence and row tile of it, a row tile having more than one piece; contiguous: as the tiles' blocks
 template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_BLOCK) attention_join_kernel(AttnArgs a, AttnPartial part, uint32_t tile_blocks) {
     __shared__ float factors[AT_JOIN_ROWS * AT_MOST_PIECES];
@@ -927,6 +939,10 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
         const uint64_t less = a.causal ? a.tokens / (2 * S::KT) : 0, mean = span > 2 * less ? span - less : (span + 1) / 2;
         const uint64_t tiles = part.row_tiles * per;
         uint64_t piece = few ? at_piece_for<true>(tiles, mean * tiles) : at_piece_for<false>(tiles, mean * tiles);
+        // a block to each CU and short walks of 16-bit tiles, one to two microseconds each: parts and their joining cost more than the CUs that end early leave idle.
+        // 32 heads of 64, 96 and 128, whole | shared out, us: causal 1024 tokens 21, 25, 29 | 27, 29, 40; 1024 of 2048 keys, all visible 40, 48, 58 | 40, 51, 71; of
+        // 2560 47, 58, 72 | 46, 58, 82; of 4096 74, 88, 110 | 69, 89, 116; 8 heads, causal 4096 67, 78, 93 | 45, 62, 82.  A f32 tile takes four times as long
+        if (!few && sizeof(T) == 2 && tiles >= (uint64_t)dev->num_cus && span <= AT_SHORT) piece = span;
         piece = at_piece_of((uint32_t)(piece > span ? span : piece), (uint32_t)span);
         if (part.row_tiles * ((span + piece - 1) / piece) * per > (most_blocks < RT_ARRIVALS ? most_blocks : RT_ARRIVALS)) piece = span;
         part.piece = (uint32_t)piece;
