@@ -543,6 +543,15 @@ def test_many_ragged_chunks(dev):
     paged(dev, ref.Paged(rng, "bf16", 8, 1, 64, 16, lens, [140] + [129] * 12))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("batch, heads, kv_heads, queries, keys, lens", [(1, 64, 64, 512, 512, None), (3, 33, 11, 130, 700, [700, 5, 333]), (1, 300, 300, 129, 200, None),
+                                                                         (1, 32, 32, 1030, 1030, None), (1, 64, 16, 260, 2900, None)])
+def test_row_tiles_that_fill_the_chip(dev, dtype, causal, batch, heads, kv_heads, queries, keys, lens):
+    """256 row tiles and more: a block to each, in rounds that pair long walks with short ones, or shared out where the walks are long"""
+    dense(dev, np.random.default_rng(heads), dtype, batch, heads, kv_heads, queries, keys, 32, causal=causal, lens=lens)
+
+
 @pytest.mark.parametrize("queries", [1, 140])
 @pytest.mark.parametrize("window", [1 << 30, (1 << 31) - 2, 1 << 31])
 def test_windows_wider_than_any_position(dev, queries, window):
