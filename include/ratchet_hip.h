@@ -302,8 +302,9 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
  * each KV head on its own, the keep - first - recent others with the largest weights stay (equal weights: the lower
  * token; NaN ranks lowest), in their order, as tokens 0 .. keep - 1; shorter sequences stay whole.  The rows go into the pages of
  * table_out [seqs, table_len], their weights into weights_out, min(len, keep) into lens_out.  Each of the three may be its
- * input, the same pointer (the cache is then compacted in place); otherwise it overlaps no input, and the pages that table_out
- * names are none of table's, none of them named twice.  Rows whose page in table_out is not there are dropped; other rows of the pages stay as they were. */
+ * input, the same pointer (the cache is then compacted in place, and a sequence that is cut shares no page of its tokens with
+ * another); otherwise it overlaps no input, and the pages that table_out names are none of table's, none of them named
+ * twice.  Rows whose page in table_out is not there are dropped; other rows of the pages stay as they were. */
 int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const float* weights, uint32_t keep, uint32_t first, uint32_t recent,
                    const int32_t* table_out, int32_t* lens_out, float* weights_out);
 

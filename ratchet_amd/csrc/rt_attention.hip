@@ -287,6 +287,8 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
     if ((rc = rt_rows_rules(who, "q", tokens, heads, kv->head_dim, q_strides, &a.q_t, &a.q_h))) return rc;
     RT_REQUIRE(q && starts && y, RT_ERR_NULL_POINTER, "%s: NULL operand", who);
     RT_REQUIRE(!weights == !weights_out, RT_ERR_NULL_POINTER, "%s: weights and weights_out go together", who);
+    RT_REQUIRE((uint64_t)tokens * heads <= RT_MAX_NUMEL / kv->head_dim, RT_ERR_SIZE, "%s: y is too large", who);
+    RT_REQUIRE(!weights || (uint64_t)kv->seqs * kv->kv_heads <= RT_MAX_NUMEL / ((uint64_t)kv->table_len * kv->page_len), RT_ERR_SIZE, "%s: weights are too large", who);
     RT_REQUIRE(rt_aligned(q, e) && rt_aligned(y, e) && rt_aligned(starts, 4) && rt_aligned(lse, 4) && rt_aligned(weights, 4) && rt_aligned(weights_out, 4),
                RT_ERR_ALIGN, "%s: misaligned pointer", who);
     rc = rt_enter(dev);

@@ -320,6 +320,7 @@ int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const 
     RT_REQUIRE(weights && table_out && lens_out && weights_out, RT_ERR_NULL_POINTER, "%s: NULL operand", who);
     RT_REQUIRE(rt_aligned(weights, 4) && rt_aligned(table_out, 4) && rt_aligned(lens_out, 4) && rt_aligned(weights_out, 4), RT_ERR_ALIGN, "%s: misaligned pointer", who);
     const uint64_t pairs = (uint64_t)kv->seqs * kv->kv_heads;
+    RT_REQUIRE(pairs <= RT_MAX_NUMEL / cap, RT_ERR_SIZE, "%s: weights are too large", who);
     rc = rt_enter(dev);
     if (rc) return rc;
     int vb = 16;

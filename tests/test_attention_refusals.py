@@ -105,6 +105,18 @@ def test_head_dims_of_paged_attention(lib):
     assert append(lib, cache(head_dim=513)) == OK_BUT_NO_DEVICE                # moving rows has no such limit
 
 
+# sequences x KV heads x keys of 65535 x 65535 x 2^20: no weights can have as many elements, and the sizes that go by them would not fit 64 bits
+WIDE = dict(seqs=65535, kv_heads=65535, page_len=1, pages=1, head_dim=8, table_len=1 << 20)
+
+
+def test_sizes_that_pass_64_bits(lib):
+    assert attend(lib, cache(**WIDE), heads=65535, weights=SOME, weights_out=SOME) == SIZE
+    assert attend(lib, cache(**WIDE), heads=65535) == OK_BUT_NO_DEVICE
+    assert evict(lib, cache(**WIDE)) == SIZE
+    assert attend(lib, cache(), q_strides=s(0, 0), tokens=1 << 30, heads=1 << 31) == SIZE
+    assert attend(lib, cache(), q_strides=s(0, 0), tokens=1 << 20, heads=1 << 10) == OK_BUT_NO_DEVICE
+
+
 class Shape:
     """stands for a buffer: the Python layer looks at its shape and type first"""
 
