@@ -466,7 +466,7 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
 // FEW: pieces are joined by the block that comes last (a joining launch took 10 to 13 us more), and scores are left where they are
 // wanted.  Waves of a SIMD: as many as the registers let, four where the rows have 64 columns and no page table is followed (encoder in f32: 146.5 us a call, with three 148.7)
 template <typename T, int DT, bool EXACT, bool PAGED, bool FEW>
-__global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES + (DT <= 64 && !PAGED && !FEW), AtShape<T, DT>::WAVES + (DT <= 64 && !PAGED && !FEW)))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
+__global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW), AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW)))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
     typedef AtShape<T, DT> S;
     constexpr int KT = S::KT, CE = S::CE;
     constexpr int SUMS = sizeof(T) == 4 && (PAGED || FEW) ? (S::SUMS > 2 ? S::SUMS : 2) : S::SUMS;  // 64 columns have registers for two where three waves share them
@@ -995,7 +995,12 @@ template <typename T> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool pag
     if (a.dim == 80) RT_TILE(80, true);
     if (a.dim == 96) RT_TILE(96, true);
     if (a.dim == 128) RT_TILE(128, true);
-    if (a.dim <= 128) RT_TILE(128, false);
+    if (a.dim == 192) RT_TILE(192, true);
+    if (a.dim == 256) RT_TILE(256, true);
+    // f16, 32 heads, causal 2048 tokens: 40 columns 50 us, in the variant for 128 66; 192 and 256 columns 130 and 160 us,
+    // with each step's columns tested 248 and 262 (f32 603 and 904, 1549 and 2720)
+    if (a.dim < 64) RT_TILE(64, false);
+    if (a.dim < 128) RT_TILE(128, false);
     RT_TILE(256, false);
 #undef RT_TILE
 }

@@ -260,6 +260,9 @@ template <typename T> int aw_dispatch(rt_device* dev, const AttnArgs& a, const f
     if (a.dim == 80) return aw_launch<T, 80, true>(dev, a, weights, out);
     if (a.dim == 96) return aw_launch<T, 96, true>(dev, a, weights, out);
     if (a.dim == 128) return aw_launch<T, 128, true>(dev, a, weights, out);
+    if (a.dim == 192) return aw_launch<T, 192, true>(dev, a, weights, out);
+    if (a.dim == 256) return aw_launch<T, 256, true>(dev, a, weights, out);
+    if (a.dim < 64) return aw_launch<T, 64, false>(dev, a, weights, out);
     if (a.dim < 128) return aw_launch<T, 128, false>(dev, a, weights, out);
     return aw_launch<T, 256, false>(dev, a, weights, out);
 }

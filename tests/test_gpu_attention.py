@@ -229,6 +229,18 @@ def test_paged_head_layouts(dev, dtype, heads, kv_heads, dim):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [8, 16, 32, 48, 56, 72, 104, 120, 136, 160, 192, 200, 248, 256])
+def test_whole_vectors_of_columns(dev, dtype, dim):
+    """every number of columns that the tiles take rows of, in chunks that end anywhere in a step"""
+    rng = np.random.default_rng(dim)
+    dense(dev, rng, dtype, 2, 4, 2, 150, 333, dim, lens=[333, 170])
+    dense(dev, rng, dtype, 1, 2, 2, 200, 200, dim, window=70, sinks=3)
+    for new in ([1, 1, 1], [70, 2, 140]):
+        p = ref.Paged(rng, dtype, 4, 2, dim, 24, [100, 9, 301], new)
+        paged(dev, p, weights=rng.random((3, 2, p.cap), dtype=np.float32))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("window, sinks", [(0, 0), (40, 0), (40, 5), (3, 90)])
 @pytest.mark.parametrize("alias", [False, True])
 def test_received_weights(dev, dtype, window, sinks, alias):
