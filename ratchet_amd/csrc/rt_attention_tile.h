@@ -873,7 +873,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         at_join<T, true>(a, part, s, b, g, row0, 0, rows, first, stride, used, (float*)smem);
 }
 
-// Parts of a row to the row: bound by reading them, 96 KB a row tile and piece in two 64 KB or more (encoder: 10 us, ragged chunks: 16 us with their search).
+// Parts of a row to the row: bound by reading them, 512 bytes a row, piece and 128 columns, and by the launch (encoder: 10 us, ragged chunks: 16 us with their search).
 // blockIdx.y: which AT_JOIN_ROWS of a row tile.  blockIdx.x: paged: KV head, sequence and row tile of it, a row tile having more than one piece; contiguous: as the tiles' blocks
 template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_BLOCK) attention_join_kernel(AttnArgs a, AttnPartial part, uint32_t tile_blocks) {
     __shared__ float factors[AT_JOIN_ROWS * AT_MOST_PIECES];
