@@ -179,22 +179,24 @@ class PagedCache:
 
 
 @functools.lru_cache(maxsize=4096)
-def _checked_strides(shape, strides, offset, numel):
+def _checked_strides(shape, strides, count, offset, numel):
     strides = tuple(map(int, strides))
+    if len(strides) != count:
+        raise ValueError(f"{len(strides)} strides for {shape}, {count} are wanted")
     if min(strides) < 0:
         raise ValueError(f"negative stride in {strides}")
-    last = offset + sum((n - 1) * s for n, s in zip(shape, strides)) + (shape[-1] - 1 if len(strides) < len(shape) else 0)
+    last = offset + sum((n - 1) * s for n, s in zip(shape, strides)) + (shape[-1] - 1 if count < len(shape) else 0)
     if last >= numel:
         raise ValueError(f"{shape} with strides {strides} reaches beyond its buffer")
     return strides_array(strides)
 
 
-def _strided(x, strides):
-    """what the library takes for `strides` (elements, one for each extent of x but the last where x is a row list), checked against the memory behind x"""
+def _strided(x, strides, count):
+    """what the library takes for `strides` (elements; it reads `count` of them: one for each extent of x, but the last where x is a row list), checked against the memory behind x"""
     if strides is None:
         return None
     parent = getattr(x, "parent", x)
-    return _checked_strides(x.shape, tuple(strides), 0 if parent is x else (x.ptr.value - parent.ptr.value) // _DT_BYTES[x.dt], parent.numel)
+    return _checked_strides(x.shape, tuple(strides), count, 0 if parent is x else (x.ptr.value - parent.ptr.value) // _DT_BYTES[x.dt], parent.numel)
 
 
 class Device:
@@ -435,8 +437,8 @@ class Device:
             raise ValueError("out or lse does not fit")
         if not (out_strides is None or out.shape == q.shape):
             raise ValueError("out with strides has the shape of q")
-        check(self.lib.rt_attention(self.handle, q.dt, q.ptr, buffer_shape4(q.shape), _strided(q, q_strides), k.ptr, _strided(k, k_strides), v.ptr, _strided(v, v_strides),
-                                    buffer_shape4(k.shape), lens.ptr if lens is not None else None, out.ptr, _strided(out, out_strides), lse.ptr if lse is not None else None,
+        check(self.lib.rt_attention(self.handle, q.dt, q.ptr, buffer_shape4(q.shape), _strided(q, q_strides, 4), k.ptr, _strided(k, k_strides, 4), v.ptr, _strided(v, v_strides, 4),
+                                    buffer_shape4(k.shape), lens.ptr if lens is not None else None, out.ptr, _strided(out, out_strides, 4), lse.ptr if lse is not None else None,
                                     q.shape[3] ** -0.5 if scale is None else scale, 1 if causal else 0, window, sinks))
         return out
 
@@ -450,7 +452,7 @@ class Device:
             raise ValueError(f"{k.shape} and {v.shape} do not fit the cache")
         if not (starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,)):
             raise ValueError("starts has to be I32 [seqs + 1]")
-        check(self.lib.rt_paged_append(self.handle, _DT_BYTES[cache.dt], cache.ref, starts.ptr, k.shape[0], k.ptr, _strided(k, k_strides), v.ptr, _strided(v, v_strides)))
+        check(self.lib.rt_paged_append(self.handle, _DT_BYTES[cache.dt], cache.ref, starts.ptr, k.shape[0], k.ptr, _strided(k, k_strides, 2), v.ptr, _strided(v, v_strides, 2)))
         return cache
 
     def paged_attention(self, q, cache, starts, window=0, sinks=0, scale=None, q_strides=None, out=None, lse=None, weights=None, weights_out=None):
@@ -469,7 +471,7 @@ class Device:
             weights_out = weights if weights_out is None else weights_out
             if not (weights.dt == weights_out.dt == _lib.F32 and weights.shape == weights_out.shape == cache.weights_shape):
                 raise ValueError(f"weights have to be F32 {cache.weights_shape}")
-        check(self.lib.rt_paged_attention(self.handle, q.dt, q.ptr, _strided(q, q_strides), q.shape[0], q.shape[1], cache.ref, starts.ptr, out.ptr,
+        check(self.lib.rt_paged_attention(self.handle, q.dt, q.ptr, _strided(q, q_strides, 2), q.shape[0], q.shape[1], cache.ref, starts.ptr, out.ptr,
                                           lse.ptr if lse is not None else None, weights.ptr if weights is not None else None,
                                           weights_out.ptr if weights is not None else None, q.shape[2] ** -0.5 if scale is None else scale, window, sinks))
         return out
