@@ -199,6 +199,13 @@ def _strided(x, strides, count):
     return _checked_strides(x.shape, tuple(strides), count, 0 if parent is x else (x.ptr.value - parent.ptr.value) // _DT_BYTES[x.dt], parent.numel)
 
 
+def _counts(**counts):
+    """the library takes each modulo 2^32"""
+    for name, n in counts.items():
+        if not 0 <= n < 2 ** 32:
+            raise ValueError(f"{name} is {n}")
+
+
 class Device:
     """One GPU: its storage pool, and the ops, which are enqueued on a stream of the device's own and return at once.  No other
     stream is ordered with that one, torch's current stream included: who fills a buffer or reads a result through torch (or
@@ -432,6 +439,7 @@ class Device:
             raise ValueError(f"attention of {q.shape}, {k.shape}, {v.shape}")
         if not (lens is None or (lens.dt == _lib.I32 and lens.shape == (q.shape[0],))):
             raise ValueError("lens has to be I32 [B]")
+        _counts(window=window, sinks=sinks)
         out = out or Buffer(self, q.shape, q.dt)
         if not (out.dt == q.dt and out.numel == q.numel and (lse is None or (lse.dt == _lib.F32 and lse.numel * q.shape[3] == q.numel))):
             raise ValueError("out or lse does not fit")
@@ -462,6 +470,7 @@ class Device:
             raise ValueError(f"{q.shape} does not fit the cache")
         if not (starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,)):
             raise ValueError("starts has to be I32 [seqs + 1]")
+        _counts(window=window, sinks=sinks)
         out = out or Buffer(self, q.shape, q.dt)
         if not (out.dt == q.dt and out.numel == q.numel and (lse is None or (lse.dt == _lib.F32 and lse.numel * q.shape[2] == q.numel))):
             raise ValueError("out or lse does not fit")
@@ -480,6 +489,7 @@ class Device:
         """Cuts every sequence of more than `keep` tokens to its first `first`, its last `recent` and the others with the largest weights, each KV head
         on its own, in their order: in place, or into the pages of the table `to` (none of them in use by the cache), lens_out and weights_out.
         Returns the cache with what it then holds."""
+        _counts(keep=keep, first=first, recent=recent)
         to, lens_out, weights_out = to or cache.table, lens_out or cache.lens, weights_out or weights
         if not (to.dt == lens_out.dt == _lib.I32 and to.shape == cache.table.shape and lens_out.shape == cache.lens.shape):
             raise ValueError("to or lens_out does not fit the cache")

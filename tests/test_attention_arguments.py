@@ -69,3 +69,25 @@ def test_another_number_of_strides_than_the_library_reads(dev, call, name, strid
     with pytest.raises(ValueError, match="strides"):
         call(dev, **{name: strides})
     assert dev.lib.calls == 0
+
+
+def evict(dev, **change):
+    return dev.paged_evict(CACHE, **{**dict(weights=WEIGHTS, keep=40), **change})
+
+
+@pytest.mark.parametrize("call, name, value", [
+    *[(call, name, v) for call in (attention, paged) for name in ("window", "sinks") for v in (-1, -5, 2 ** 32, 2 ** 32 + 7)],
+    *[(evict, name, v) for name in ("keep", "first", "recent") for v in (-1, -(2 ** 32) + 3, 2 ** 32, 2 ** 32 + 7)],
+])
+def test_counts_that_32_bits_do_not_hold(dev, call, name, value):
+    """taken modulo 2^32 they would be other counts: -1 sinks all keys, 2^32 + 7 a window of 7"""
+    with pytest.raises(ValueError, match=name):
+        call(dev, **{name: value})
+    assert dev.lib.calls == 0
+
+
+def test_counts_that_32_bits_hold(dev):
+    attention(dev, window=2 ** 32 - 1, sinks=2 ** 32 - 1)
+    paged(dev, window=2 ** 32 - 1, sinks=0)
+    evict(dev, keep=80, first=0, recent=80)
+    assert dev.lib.calls == 3
