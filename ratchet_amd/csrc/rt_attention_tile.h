@@ -12,8 +12,10 @@
 // what is not finite is NaN, which stays.  So a row tile whose result is not finite is computed again, one row at a time, over the visible keys only.
 //
 // Roundings below f32: the weights of 16-bit types are rounded to the type for the second product, as its operands have to be (their f32 values make the sums);
-// everything else, scores, m, l and O, is f32.  An m that lags by up to AT_SLACK powers of two makes weights up to 2^8: rounded relative to themselves, so nothing
-// is lost, and f16's largest is 2^16.
+// everything else, scores, m, l and O, is f32.  An m that lags by up to AT_SLACK powers of two makes weights up to 2^8: rounded relative to themselves.  f16's small numbers
+// are not: they end at 2^-24, and thousands of keys below that against the row's largest can be most of a result.  f16 weights are therefore held 2^AT_LIFT larger,
+// to 2^14 at most (f16's largest is 2^16; scores beyond 2^24, whose own rounding may pass that, make a row that is computed again): relative to the largest they
+// go down to 2^-30 at least, where rows are few to 2^-38.  l and O carry the same factor until the row is finished or its part is left.
 //
 // What bounds it, by counters: 8192 tokens of 32 heads of 96 with a window of 2047, bf16: 227 to 236 us, 770 to 800 TFLOP/s of the visible pairs' products; the
 // matrix units are busy 47 % and the vector units (scores to weights: about eight instructions each) 62 % of the time, and three waves of a SIMD have both overlap
@@ -30,7 +32,10 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t AT_ROWS = 128, AT_WAVES = 4, AT_BLOCK = 64 * AT_WAVES;
-constexpr float AT_SLACK = 8.0f;                 // powers of two that a row's weights may lie above its m
+constexpr int AT_SLACK = 8;                      // powers of two that a row's weights may lie above its m
+template <typename T, bool FEW> constexpr int AT_LIFT = 0;
+template <> inline constexpr int AT_LIFT<half_t, false> = 14 - AT_SLACK;
+template <> inline constexpr int AT_LIFT<half_t, true> = 14;
 // How far the keys of row tiles are shared out over blocks.  Single tokens (FEW): to AT_TARGET_FEW items, in pieces of no fewer than two tiles, which costs little as
 // their parts are small (one token's 2051 keys 17.9 us, with four tiles at least 19.3; 16 tokens 53 us at 1024 items, 61 at 512, 58 at 2048; 64 ragged
 // ones 255, 277, 251).  Others leave and join 64 KB a row tile and piece: only where the row tiles do not fill the chip by themselves (AT_ENOUGH), and to
@@ -469,6 +474,7 @@ template <typename T, int DT, bool EXACT, bool PAGED, bool FEW>
 __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW), AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW)))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
     typedef AtShape<T, DT> S;
     constexpr int KT = S::KT, CE = S::CE;
+    constexpr float LIFT = AT_LIFT<T, FEW>, LOWER = 1.0f / (1 << AT_LIFT<T, FEW>);              // the weights' factor is 2^LIFT, 1 / LOWER
     constexpr int SUMS = sizeof(T) == 4 && (PAGED || FEW) ? (S::SUMS > 2 ? S::SUMS : 2) : S::SUMS;  // 64 columns have registers for two where three waves share them
     extern __shared__ __align__(16) unsigned char smem[];
     lds_byte* const lds = (lds_byte*)smem;
@@ -712,7 +718,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
             for (int e = 0; e < 16; e++) top = fmaxf(top, x[kk][e]);
         top = fmaxf(top, at_other(top)) * c;
         // m follows the maximum at a distance: a weight of up to 2^AT_SLACK loses nothing in f32, f16 or bf16, and of 32 rows one has a new maximum in nearly every tile
-        if (__ballot(top > m + (FEW ? 0.0f : AT_SLACK))) {
+        if (__ballot(top > m + (FEW ? 0.0f : (float)AT_SLACK))) {
             const float m_new = fmaxf(m, top), old = at_exp2(m - (m_new == -INFINITY ? 0.0f : m_new));
             m = m_new;
             l *= old;
@@ -721,7 +727,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[i][e] *= old;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float base = m == -INFINITY ? 0.0f : m - LIFT;
         if constexpr (sizeof(T) == 2) {
             constexpr int GROUPS = 2 * S::HALVES, P = GROUPS * S::BLOCKS, FRONT = 4;           // groups of 16 keys
             v4u v[P], w[GROUPS];
@@ -848,7 +854,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
                     *(v4f*)(y + d) = v4f{o[i][e] * inv, o[i][e + 1] * inv, o[i][e + 2] * inv, o[i][e + 3] * inv};
                 }
             }
-        if (a.lse && half == 0) a.lse[b * a.l_b + h * a.l_h + (uint64_t)(s.first + j) * a.l_t] = at_lse(m, l);
+        if (a.lse && half == 0) a.lse[b * a.l_b + h * a.l_h + (uint64_t)(s.first + j) * a.l_t] = at_lse(m, l * LOWER);
     } else if (r < rows) {
         const uint64_t part_at = (uint64_t)blockIdx.x * AT_ROWS + r;
 #pragma unroll
@@ -858,14 +864,14 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
                 const uint32_t d = 32 * i + 8 * (e / 4) + 4 * half;
                 if (d >= D) continue;
                 if (FEW) {
-                    at_leave(part.o + part_at * D + d, o[i][e], o[i][e + 1]);
-                    at_leave(part.o + part_at * D + d + 2, o[i][e + 2], o[i][e + 3]);
+                    at_leave(part.o + part_at * D + d, o[i][e] * LOWER, o[i][e + 1] * LOWER);
+                    at_leave(part.o + part_at * D + d + 2, o[i][e + 2] * LOWER, o[i][e + 3] * LOWER);
                 } else {
                     typedef float v4f __attribute__((ext_vector_type(4)));
-                    *(v4f*)(part.o + part_at * D + d) = v4f{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+                    *(v4f*)(part.o + part_at * D + d) = v4f{o[i][e] * LOWER, o[i][e + 1] * LOWER, o[i][e + 2] * LOWER, o[i][e + 3] * LOWER};
                 }
             }
-        if (half == 0) at_put<FEW>(part.ml + 2 * part_at, m, l);
+        if (half == 0) at_put<FEW>(part.ml + 2 * part_at, m, l * LOWER);
     }
     if (!FEW || whole) return;
     const uint32_t used = (w.tiles + piece - 1) / piece, first = blockIdx.x - piece_at * stride;
