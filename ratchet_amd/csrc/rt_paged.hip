@@ -17,8 +17,11 @@ struct AppendArgs {
 
 // A block to a token: the wave finds the token's sequence, then the block's threads move the vectors of all its heads, keys and values alike.
 // Moves each row once; bound by memory for prompts (157 MB in f16: 31.7 us, 5.0 TB/s) and by the chain starts -> lens and table -> store for single tokens (64: 2.8 us).
+constexpr uint32_t APPEND_ROW = 1u << 22;           // blocks to a row of the grid: an extent of a launch has fewer than 2^32 threads
+
 template <typename VecT> __global__ void __launch_bounds__(BLOCK) paged_append_kernel(AppendArgs a) {
-    const uint32_t token = blockIdx.x;
+    const uint32_t token = blockIdx.y * APPEND_ROW + blockIdx.x;
+    if (token >= a.tokens) return;
     const uint32_t b = at_find(a.starts, a.seqs, token);
     if (b == a.seqs) return;
     const int32_t top = (int32_t)a.tokens;
@@ -298,7 +301,7 @@ int rt_paged_append(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const
     a.tokens = tokens;
     a.page_div = make_fastdiv(kv->page_len);
     a.row_div = make_fastdiv(a.row_v);
-    const dim3 grid(tokens), block(BLOCK);
+    const dim3 grid(tokens < APPEND_ROW ? tokens : APPEND_ROW, (tokens + APPEND_ROW - 1) / APPEND_ROW), block(BLOCK);
     if (vb == 16) hipLaunchKernelGGL((paged_append_kernel<v4u>), grid, block, 0, dev->stream, a);
     else if (vb == 8) hipLaunchKernelGGL((paged_append_kernel<v2u>), grid, block, 0, dev->stream, a);
     else if (vb == 4) hipLaunchKernelGGL((paged_append_kernel<uint32_t>), grid, block, 0, dev->stream, a);
