@@ -57,7 +57,7 @@ static inline int at_workspace(rt_device* dev, AttnArgs& a, size_t bytes, void**
     return RT_OK;
 }
 
-// The matrix-unit kernels (rt_attention_tile.h), a source to each element type.  RT_OK with *done = false where the operands are not laid out for them
+// The matrix-unit kernels (rt_attention_tile.h), a source to each element type.  RT_OK with *done = false where the operands are not laid out for them, or are too many rows for a launch
 int rt_attention_tile_f32(rt_device* dev, AttnArgs& a, bool paged, bool* done);
 int rt_attention_tile_f16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
 int rt_attention_tile_bf16(rt_device* dev, AttnArgs& a, bool paged, bool* done);

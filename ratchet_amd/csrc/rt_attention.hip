@@ -6,6 +6,7 @@
 namespace {
 
 constexpr int WAVES = 4, BLOCK = 64 * WAVES;
+constexpr uint32_t GRID_ROW = 1u << 22;          // blocks to a row of the grid: an extent of a launch has fewer than 2^32 threads
 
 // A wave to a (query, head) row.  A lane computes the score of one key of a tile of 64; the tile's weights then go round the wave, key by key, and
 // each lane adds them to its columns.  Hidden keys are skipped there, so nothing they hold is ever multiplied.
@@ -13,7 +14,7 @@ constexpr int WAVES = 4, BLOCK = 64 * WAVES;
 template <typename T, bool PAGED>
 __global__ void __launch_bounds__(BLOCK) attention_any_kernel(AttnArgs a, uint64_t rows) {
     const uint32_t lane = threadIdx.x % 64;
-    const uint64_t row = (uint64_t)blockIdx.x * WAVES + threadIdx.x / 64;
+    const uint64_t row = ((uint64_t)blockIdx.y * GRID_ROW + blockIdx.x) * WAVES + threadIdx.x / 64;
     if (row >= rows) return;
     const uint32_t h = (uint32_t)(row % a.heads);
     uint64_t at = row / a.heads;
@@ -124,9 +125,10 @@ __global__ void __launch_bounds__(64) attention_weights_any_kernel(AttnArgs a, c
 
 template <typename T> int launch_any(rt_device* dev, const AttnArgs& a, bool paged, const float* weights, float* weights_out) {
     const uint64_t rows = (uint64_t)(paged ? 1 : a.seqs) * a.tokens * a.heads, blocks = (rows + WAVES - 1) / WAVES;
-    RT_REQUIRE(blocks <= 0x7fffffffull, RT_ERR_SIZE, "attention: too many rows");
-    if (paged) hipLaunchKernelGGL((attention_any_kernel<T, true>), dim3((unsigned)blocks), dim3(BLOCK), 0, dev->stream, a, rows);
-    else hipLaunchKernelGGL((attention_any_kernel<T, false>), dim3((unsigned)blocks), dim3(BLOCK), 0, dev->stream, a, rows);
+    RT_REQUIRE(blocks <= 65535ull * GRID_ROW, RT_ERR_SIZE, "attention: too many rows");
+    const dim3 grid((unsigned)(blocks < GRID_ROW ? blocks : GRID_ROW), (unsigned)((blocks + GRID_ROW - 1) / GRID_ROW));
+    if (paged) hipLaunchKernelGGL((attention_any_kernel<T, true>), grid, dim3(BLOCK), 0, dev->stream, a, rows);
+    else hipLaunchKernelGGL((attention_any_kernel<T, false>), grid, dim3(BLOCK), 0, dev->stream, a, rows);
     RT_CHECK_LAUNCH("attention_any_kernel");
     if (weights_out) {
         hipLaunchKernelGGL((attention_weights_any_kernel<T>), dim3((a.cap + 63) / 64, a.kv_heads, a.seqs), dim3(64), 0, dev->stream, a, weights, weights_out);

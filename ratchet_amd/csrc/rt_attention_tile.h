@@ -47,6 +47,7 @@ constexpr size_t AT_MOST_PARTS = 1u << 30;       // bytes of parts; a launch tha
 constexpr uint32_t AT_MOST_PIECES = 60;          // of a row tile: their factors for its 128 rows fit the LDS of the smallest tiles
 constexpr uint32_t AT_FEW_ROWS = 16;             // rows of a sequence and KV head, on average, up to which a launch joins its own pieces
 constexpr uint32_t AT_JOIN_ROWS = 16;            // rows to a block of the joining kernel
+constexpr uint64_t AT_MOST_BLOCKS = (1u << 24) - 1;   // of a launch, which has fewer than 2^32 threads; more rows go to the kernel for any
 
 // ------------------------------------------------------------------------------------------------- who does what
 // Tiles of KT keys that a tile of rows of sequence s may see at most; 1 where there are no keys, for the block that writes the zeros
@@ -919,7 +920,7 @@ template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_B
     at_join<T, false>(a, part, s, b, g, row0, r0, r1, first, stride, used, factors);
 }
 
-template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_device* dev, AttnArgs& a) {
+template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_device* dev, AttnArgs& a, bool* done) {
     typedef AtShape<T, DT> S;
     AttnPartial part = {};
     const bool few = (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
@@ -959,7 +960,8 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
         join_tiles = part.row_tiles * per;
     }
     const uint64_t blocks = items * per;
-    RT_REQUIRE(blocks <= 0x7fffffffull, RT_ERR_SIZE, "attention: too many rows");
+    *done = blocks <= AT_MOST_BLOCKS;
+    if (!*done) return RT_OK;
     const size_t row_count = part.split ? (size_t)blocks * AT_ROWS : 0;
     a.score_pitch = (a.cap + 63) / 64 * 64;
     size_t score_bytes = PAGED && few && a.want_scores ? (size_t)a.tokens * a.heads * a.score_pitch * sizeof(float) : 0;
@@ -996,7 +998,7 @@ template <typename T> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool pag
     for (uint64_t x : strides) fits = fits && x * e % 16 == 0;
     *done = fits;
     if (!fits) return RT_OK;
-#define RT_TILE(DT, EXACT) return paged ? at_launch_tile<T, DT, EXACT, true>(dev, a) : at_launch_tile<T, DT, EXACT, false>(dev, a)
+#define RT_TILE(DT, EXACT) return paged ? at_launch_tile<T, DT, EXACT, true>(dev, a, done) : at_launch_tile<T, DT, EXACT, false>(dev, a, done)
     if (a.dim == 64) RT_TILE(64, true);
     if (a.dim == 80) RT_TILE(80, true);
     if (a.dim == 96) RT_TILE(96, true);

@@ -30,3 +30,22 @@ def test_append_of_more_than_2_to_the_24_tokens(dev):
         want[:tokens] = x.view(np.uint16).ravel()
         got = buf.to_numpy().view(np.uint16).reshape(pages, page)
         assert np.array_equal(got[order], want.reshape(pages, page))
+
+
+def test_attention_of_more_than_2_to_the_26_rows(dev):
+    """one key, so that every row is that key's value"""
+    rows = (1 << 26) + 5
+    q = dev.empty((1, 1, rows, 1), _lib.F16).zero_()
+    k, v = dev.upload(np.full((1, 1, 1, 1), 2.0, np.float16)), dev.upload(np.full((1, 1, 1, 1), 3.5, np.float16))
+    out = dev.empty(q.shape, _lib.F16).zero_()
+    dev.attention(q, k, v, causal=False, out=out)
+    assert (out.to_numpy() == 3.5).all()
+
+
+def test_attention_of_more_than_2_to_the_24_heads(dev):
+    """of whole vectors of columns, each with one query and one key of its own"""
+    shape = (65535, 257, 1, 8)
+    rng = np.random.default_rng(1)
+    x = rng.integers(0, 1000, shape, dtype=np.int16).astype(np.float16)
+    v = dev.upload(x)
+    assert np.array_equal(dev.attention(v, v, v).to_numpy(), x)
