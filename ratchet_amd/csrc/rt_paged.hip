@@ -324,11 +324,17 @@ int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const 
     RT_REQUIRE(rt_aligned(weights, 4) && rt_aligned(table_out, 4) && rt_aligned(lens_out, 4) && rt_aligned(weights_out, 4), RT_ERR_ALIGN, "%s: misaligned pointer", who);
     const uint64_t pairs = (uint64_t)kv->seqs * kv->kv_heads;
     RT_REQUIRE(pairs <= RT_MAX_NUMEL / cap, RT_ERR_SIZE, "%s: weights are too large", who);
-    rc = rt_enter(dev);
-    if (rc) return rc;
     int vb = 16;
     for (; vb > elem_bytes; vb >>= 1)
         if ((uint64_t)kv->head_dim * elem_bytes % vb == 0 && rt_aligned(kv->k, (size_t)vb) && rt_aligned(kv->v, (size_t)vb)) break;
+    MoveArgs m;
+    m.row_v = (uint32_t)((uint64_t)kv->head_dim * elem_bytes / vb);
+    m.slice_v = m.row_v < (uint32_t)BLOCK ? m.row_v : BLOCK;
+    // an extent of a launch has fewer than 2^32 threads (narrower slices, below, make no more than 8 blocks a CU)
+    RT_REQUIRE(pairs * 2 * ((m.row_v + m.slice_v - 1) / m.slice_v) < (1ull << 32) / BLOCK, RT_ERR_SIZE, "%s: %u sequences, %u KV heads of %u columns", who, kv->seqs, kv->kv_heads,
+               kv->head_dim);
+    rc = rt_enter(dev);
+    if (rc) return rc;
     void* scratch;
     if ((rc = rt_scratch(dev, (size_t)(pairs * (1 + (uint64_t)keep)) * sizeof(uint32_t), &scratch))) return rc;
     EvictArgs e;
@@ -339,16 +345,13 @@ int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const 
     e.kv_heads = kv->kv_heads; e.cap = cap; e.keep = keep; e.first = first; e.recent = recent;
     hipLaunchKernelGGL(evict_select_kernel, dim3(kv->kv_heads, kv->seqs), dim3(SELECT_BLOCK), 0, dev->stream, e);
     RT_CHECK_LAUNCH("evict_select_kernel");
-    MoveArgs m;
     m.pages[0] = kv->k; m.pages[1] = kv->v;
     m.table = kv->table; m.table_out = table_out; m.lens_out = lens_out;
     m.kept = e.kept; m.counts = e.counts;
     m.n_pages = kv->pages; m.kv_heads = kv->kv_heads; m.page_len = kv->page_len; m.seqs = kv->seqs; m.table_len = kv->table_len; m.keep = keep;
-    m.row_v = (uint32_t)((uint64_t)kv->head_dim * elem_bytes / vb);
     // Elsewhere: whole rows.  In place the rows of a pair cannot be shared out, but their columns can: slices of 64 bytes at least, as many
     // as give four blocks a CU.
     const bool in_place = table_out == kv->table;
-    m.slice_v = m.row_v < (uint32_t)BLOCK ? m.row_v : BLOCK;
     if (in_place)
         while (m.slice_v > 4 && pairs * 2 * ((m.row_v + m.slice_v - 1) / m.slice_v) < 4ull * dev->num_cus) m.slice_v = (m.slice_v + 1) / 2;
     m.slices = (m.row_v + m.slice_v - 1) / m.slice_v;
@@ -359,9 +362,7 @@ int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const 
     const uint64_t wanted = pairs * 2 * m.slices * keep / (8ull * dev->num_cus);
     if (wanted > m.rows) m.rows = (uint32_t)((wanted + one_step - 1) / one_step * one_step);
     if (in_place) m.rows = keep;
-    const uint64_t blocks = pairs * 2 * m.slices, chunks = (keep + m.rows - 1) / m.rows;
-    RT_REQUIRE(blocks <= 0x7fffffffull && chunks <= 65535, RT_ERR_SIZE, "%s: too many rows", who);
-    const dim3 grid((unsigned)blocks, (unsigned)chunks), block(BLOCK);
+    const dim3 grid((unsigned)(pairs * 2 * m.slices), (keep + m.rows - 1) / m.rows), block(BLOCK);
     if (vb == 16) hipLaunchKernelGGL((evict_move_kernel<v4u>), grid, block, 0, dev->stream, m);
     else if (vb == 8) hipLaunchKernelGGL((evict_move_kernel<v2u>), grid, block, 0, dev->stream, m);
     else if (vb == 4) hipLaunchKernelGGL((evict_move_kernel<uint32_t>), grid, block, 0, dev->stream, m);
