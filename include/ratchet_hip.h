@@ -216,7 +216,7 @@ int rt_softmax_masked(rt_device* dev, int dt, const void* x, const uint32_t x_sh
  * rt_h2d, rt_d2h, rt_pool_trim, event calls, an rt_malloc the pool cannot serve, and the first use of an op that builds
  * a lookup table or grows scratch (run the sequence once eagerly first).  A graph holds raw pointers: every buffer it
  * touches must stay allocated while the graph is in use.  One that holds an attention or eviction call uses the recording
- * device's scratch: rt_graph_launch takes it on that rt_device only, and it is not launched after that device is destroyed. */
+ * device's scratch: rt_graph_launch takes it on that rt_device only, and refuses it once that device is destroyed. */
 typedef struct rt_graph rt_graph;
 int rt_capture_begin(rt_device* dev);
 int rt_capture_end(rt_device* dev, rt_graph** out);

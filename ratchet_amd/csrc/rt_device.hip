@@ -1,6 +1,7 @@
 // Device, storage and timing entry points of the C ABI: hipMalloc'd storage and one in-order stream take the place
 // of ratchet-core's wgpu device, buffer pool and queue (gpu/device.rs, gpu/pools/buffer_pool.rs,
 // storage/gpu_buffer.rs in crates/ratchet-core/src).
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -15,7 +16,7 @@ struct rt_graph {
     hipGraph_t graph;
     hipGraphExec_t exec;
     int ordinal;
-    rt_device* scratch_owner;      // the device whose workspace the recorded calls use, NULL if they use none
+    uint64_t scratch_owner;        // serial of the device whose workspace the recorded calls use, 0 if they use none
 };
 
 struct rt_retired {
@@ -183,6 +184,8 @@ int rt_device_create(int ordinal, rt_device** out) {
     memset(dev, 0, sizeof(*dev));
     dev->pool = new rt_pool();
     dev->ordinal = ordinal;
+    static std::atomic<uint64_t> devices{0};
+    dev->serial = ++devices;
     dev->num_cus = prop.multiProcessorCount;
     {
         int khz = 0;
@@ -529,7 +532,7 @@ int rt_capture_end(rt_device* dev, rt_graph** out) {
     g->graph = graph;
     g->exec = exec;
     g->ordinal = dev->ordinal;
-    g->scratch_owner = dev->capture_used_scratch ? dev : nullptr;
+    g->scratch_owner = dev->capture_used_scratch ? dev->serial : 0;
     *out = g;
     return RT_OK;
 }
@@ -540,7 +543,7 @@ int rt_graph_launch(rt_device* dev, rt_graph* graph) {
     if (rc) return rc;
     RT_NO_CAPTURE(dev, "rt_graph_launch");
     RT_REQUIRE(graph->ordinal == dev->ordinal, RT_ERR_ARG, "rt_graph_launch: the graph was captured on device %d", graph->ordinal);
-    RT_REQUIRE(!graph->scratch_owner || graph->scratch_owner == dev, RT_ERR_ARG,
+    RT_REQUIRE(!graph->scratch_owner || graph->scratch_owner == dev->serial, RT_ERR_ARG,
                "rt_graph_launch: the graph uses the workspace of the rt_device that recorded it");
     RT_HIP(hipGraphLaunch(graph->exec, dev->stream));
     return RT_OK;

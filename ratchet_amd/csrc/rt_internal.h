@@ -24,6 +24,7 @@ constexpr uint32_t RT_ARRIVALS = 1u << 16;
 
 struct rt_device {
     int ordinal;
+    uint64_t serial;        // 1, 2, ... in the order devices are made: an address can be a later device's too
     hipStream_t stream;
     int num_cus;
     double wall_clock_hz;   // rate of the device's constant-frequency wall clock (s_memrealtime), 100 MHz on this chip
