@@ -255,7 +255,7 @@ int rt_gated_mul_via_f32(rt_device* dev, int op, int io_dt, const void* gate, ui
  * cache.  Query head h reads KV head h / (heads / kv_heads).  Scores, softmax statistics and the sums over the keys are
  * f32; the result is rounded once to the element type (F32, F16, BF16).  With p the position of a query and len the
  * keys there are, key t is visible iff t < len and, where causal, 0 <= t <= p and (window == 0 or p - t < window or t < sinks):
- * a sliding window, and `sinks` first keys that stay in sight.  A query that sees no key yields 0 and an lse of -inf;
+ * a sliding window, and `sinks` first keys that stay in sight.  A query that sees no key, or none with a score above -inf, yields 0 and an lse of -inf;
  * what hidden keys and values hold, infinities and NaN included, does not matter.  y and lse overlap no input. */
 
 /* q [B, heads, Sq, D], k and v [B, kv_heads, Sk, D], y as q; strides in elements (NULL: contiguous), the last one 1 where D > 1,

@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(64) attention_weights_any_kernel(AttnArgs a, c
         for (uint32_t h = g * a.group; h < (g + 1) * a.group; h++) {
             const T* q = (const T*)a.q + h * a.q_h + (uint64_t)(s.first + j) * a.q_t;
             const float lse = a.lse[h * a.l_h + (uint64_t)(s.first + j) * a.l_t];
-            if (!seen) continue;
+            if (!seen || lse == -INFINITY) continue;           // a row whose scores are all -inf weighs nothing
             float dot = 0.0f;
             for (uint32_t d = 0; d < a.dim; d++) dot = __builtin_fmaf(Ar<T>::widen(q[d]), Ar<T>::widen(k[d]), dot);
             sum += at_exp2(__builtin_fmaf(lse, -1.4426950408889634f, dot * a.c));

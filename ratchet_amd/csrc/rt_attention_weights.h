@@ -160,7 +160,9 @@ __global__ void __launch_bounds__(AT_BLOCK, DT > 128 ? 1 : DT > 96 || sizeof(T) 
             };
 #pragma unroll
             for (int p = 0; p < AHEAD; p++) read_q(p);
-            const float lse[2] = {at_lds4(cur + S::ROWS_AT + col * 4) * -1.4426950408889634f, at_lds4(cur + S::ROWS_AT + (col + 32) * 4) * -1.4426950408889634f};
+            float lse[2] = {at_lds4(cur + S::ROWS_AT + col * 4) * -1.4426950408889634f, at_lds4(cur + S::ROWS_AT + (col + 32) * 4) * -1.4426950408889634f};
+#pragma unroll
+            for (int y = 0; y < 2; y++) lse[y] = lse[y] == INFINITY ? -INFINITY : lse[y];       // a row whose scores are all -inf weighs nothing
             at_in_order();
 #pragma unroll
             for (int p = 0; p < N; p++) {

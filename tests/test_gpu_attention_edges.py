@@ -1,0 +1,54 @@
+"""Edges of attention: scores of minus infinity, lengths of a padded batch over many keys, strides of extents of one."""
+import numpy as np
+import pytest
+
+import attention_ref as ref
+from test_gpu_attention import DTYPES, dense, paged
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    from ratchet_amd import Device
+
+    d = Device(0)
+    yield d
+    d.close()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [7, 40, 64, 80, 256])
+@pytest.mark.parametrize("new", [[1, 1, 1], [90, 1, 200]])
+def test_rows_whose_visible_scores_are_all_minus_infinity(dev, dtype, dim, new):
+    """they weigh nothing, as keys out of sight do: a result of 0, an lse of -inf, and nothing received from them"""
+    rng = np.random.default_rng(dim)
+    p = ref.Paged(rng, dtype, 4, 2, dim, 16, [300, 80, 250], new)
+    p.q[..., 0] = np.abs(p.q[..., 0]) + 1.0
+    p.q = ref.rounded(p.q, dtype)
+    t = np.arange(300)
+    p.k[p.table[0, t // 16], :, t % 16, 0] = -np.inf            # all of sequence 0
+    t = np.arange(0, 250, 3)
+    p.k[p.table[2, t // 16], :, t % 16, 0] = -np.inf            # every third key of sequence 2
+    w = rng.random((3, 2, p.cap), dtype=np.float32)
+    lse, w_out = dev.upload(np.zeros(p.q.shape[:2], np.float32)), dev.upload(np.zeros(w.shape, np.float32))
+    cache = dev.paged_cache(ref.upload(dev, p.k, dtype), ref.upload(dev, p.v, dtype), dev.upload(p.table), dev.upload(p.lens.astype(np.int32)))
+    out = dev.paged_attention(ref.upload(dev, p.q, dtype), cache, dev.upload(p.starts), scale=0.125, lse=lse, weights=dev.upload(w), weights_out=w_out)
+    got, got_lse, got_w = ref.values(out.to_numpy(), dtype), lse.to_numpy(), w_out.to_numpy()
+    for b in range(3):
+        lo, hi, n = p.starts[b], p.starts[b + 1], int(p.lens[b])
+        k, _ = p.rows(p.k, b)
+        v, _ = p.rows(p.v, b)
+        shift = n - (hi - lo)
+        for g in range(2):
+            total, off = np.where(np.arange(n) < shift, w[b, g, :n].astype(np.float64), 0.0), np.zeros(n)
+            gone = np.isinf(k[g, :, 0])
+            clean = np.where(gone[:, None], 0.0, k[g])
+            see = ref.visible(hi - lo, n, shift, True, 0, 0, gone)
+            for h in (2 * g, 2 * g + 1):
+                o, want_lse, x, o_off, lse_off, factor = ref.head(p.q[lo:hi, h], clean, v[g], see, 0.125, dtype)
+                ref.check(got[lo:hi, h], o, o_off, ("o", b, h))
+                ref.check(got_lse[lo:hi, h], want_lse, lse_off, ("lse", b, h))
+                total += x.sum(axis=0)
+                off += (x * factor[:, None]).sum(axis=0)
+            ref.check(got_w[b, g, :n], total, off + (2 * (hi - lo) + 1) * ref.U * np.abs(total), ("weights", b, g))
