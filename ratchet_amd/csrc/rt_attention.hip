@@ -177,12 +177,12 @@ int head_rules(const char* who, int dt, uint32_t heads, uint32_t kv_heads, uint3
     return RT_OK;
 }
 
-// The last extent's stride is 1; elements of one tensor lie below 2^40
+// The last extent's stride is 1; elements of one tensor lie below 2^40.  A stride of an extent of 1 is never taken, so it does not decide about the layout: 0.
 int stride_rules(const char* who, const char* what, const uint32_t shape[4], const uint64_t* strides, uint64_t out[4]) {
     unsigned __int128 dense = 1, last = 0;
     for (int i = 3; i >= 0; i--) {
         RT_REQUIRE(strides || dense <= RT_MAX_NUMEL, RT_ERR_SIZE, "%s: %s is too large", who, what);
-        out[i] = strides ? strides[i] : (uint64_t)dense;
+        out[i] = shape[i] == 1 ? 0 : strides ? strides[i] : (uint64_t)dense;
         dense *= shape[i];
         last += (unsigned __int128)(shape[i] - 1) * out[i];
     }
@@ -228,8 +228,8 @@ int rt_paged_rules(const char* who, const rt_paged_kv* kv, size_t elem_bytes) {
 }
 
 int rt_rows_rules(const char* who, const char* what, uint32_t tokens, uint32_t heads, uint32_t dim, const uint64_t strides[2], uint64_t* token, uint64_t* head) {
-    *token = strides ? strides[0] : (uint64_t)heads * dim;
-    *head = strides ? strides[1] : dim;
+    *token = tokens == 1 ? 0 : strides ? strides[0] : (uint64_t)heads * dim;                  // of an extent of 1: as in stride_rules
+    *head = heads == 1 ? 0 : strides ? strides[1] : dim;
     RT_REQUIRE(tokens > 0, RT_ERR_SHAPE, "%s: no tokens", who);
     RT_REQUIRE(tokens <= MOST_TOKENS, RT_ERR_SIZE, "%s: %u tokens", who, tokens);
     RT_REQUIRE(*token < RT_MAX_NUMEL / tokens && *head < RT_MAX_NUMEL / heads, RT_ERR_SIZE, "%s: %s is too large", who, what);

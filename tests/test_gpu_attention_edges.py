@@ -52,3 +52,34 @@ def test_rows_whose_visible_scores_are_all_minus_infinity(dev, dtype, dim, new):
                 total += x.sum(axis=0)
                 off += (x * factor[:, None]).sum(axis=0)
             ref.check(got_w[b, g, :n], total, off + (2 * (hi - lo) + 1) * ref.U * np.abs(total), ("weights", b, g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 104])
+@pytest.mark.parametrize("causal, window, sinks", [(True, 0, 0), (True, 700, 0), (True, 700, 9), (False, 0, 0)])
+@pytest.mark.parametrize("queries", [1, 16, 150])
+def test_lens_of_a_padded_batch_over_many_keys(dev, dtype, dim, causal, window, sinks, queries):
+    """entries whose keys are shared out over blocks next to those with none, and with fewer keys than queries"""
+    dense(dev, np.random.default_rng(queries), dtype, 6, 2, 1, queries, 3000, dim, causal=causal, window=window, sinks=sinks, lens=[0, 1, 5, 2999, 3000, 1400])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries, keys, heads, kv_heads", [(1, 90, 4, 1), (40, 40, 1, 1), (1, 1, 2, 2)])
+def test_strides_of_extents_of_one(dev, dtype, queries, keys, heads, kv_heads):
+    """nothing is ever that far away, so they change nothing: the same bits"""
+    rng = np.random.default_rng(keys)
+    q, k, v = (ref.upload(dev, ref.rounded(rng.standard_normal(s), dtype), dtype) for s in ((1, heads, queries, 64), (1, kv_heads, keys, 64), (1, kv_heads, keys, 64)))
+
+    def odd(shape):
+        dense_strides = (shape[1] * shape[2] * 64, shape[2] * 64, 64, 1)
+        return tuple(s if n > 1 else 7 + 2 * i for i, (n, s) in enumerate(zip(shape, dense_strides)))
+
+    want = dev.attention(q, k, v).to_numpy()
+    got = dev.attention(q, k, v, q_strides=odd(q.shape), k_strides=odd(k.shape), v_strides=odd(v.shape), out=dev.empty(q.shape, q.dt), out_strides=odd(q.shape)).to_numpy()
+    assert np.array_equal(got.view(np.uint8), want.view(np.uint8))
+    # one token, one KV head over pages
+    p = ref.Paged(rng, dtype, 1, 1, 64, 16, [80], [1])
+    cache = dev.paged_cache(ref.upload(dev, p.k, dtype), ref.upload(dev, p.v, dtype), dev.upload(p.table), dev.upload(p.lens.astype(np.int32)))
+    x, starts = ref.upload(dev, p.q, dtype), dev.upload(p.starts)
+    want = dev.paged_attention(x, cache, starts).to_numpy()
+    assert np.array_equal(dev.paged_attention(x, cache, starts, q_strides=(65, 67)).to_numpy().view(np.uint8), want.view(np.uint8))
