@@ -50,7 +50,7 @@ template <typename VecT> __global__ void __launch_bounds__(BLOCK) paged_append_k
 
 // -------------------------------------------------------------------------------------------------- eviction
 struct EvictArgs {
-    const int32_t *table, *lens;
+    const int32_t* lens;
     const float* weights;
     float* weights_out;
     uint32_t* kept;                // scratch: [seqs, kv_heads, keep] tokens that stay, in order
@@ -203,7 +203,7 @@ struct MoveArgs {
     const int32_t *table, *table_out;
     int32_t* lens_out;
     const uint32_t *kept, *counts;
-    uint32_t n_pages, kv_heads, page_len, row_v, seqs, table_len, keep, slices, slice_v, rows;   // rows: of each block
+    uint32_t n_pages, kv_heads, page_len, row_v, table_len, keep, slices, slice_v, rows;   // rows: of each block
     FastDiv page_div, slice_div;
 };
 
@@ -338,7 +338,7 @@ int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const 
     void* scratch;
     if ((rc = rt_scratch(dev, (size_t)(pairs * (1 + (uint64_t)keep)) * sizeof(uint32_t), &scratch))) return rc;
     EvictArgs e;
-    e.table = kv->table; e.lens = kv->lens;
+    e.lens = kv->lens;
     e.weights = weights; e.weights_out = weights_out;
     e.counts = (uint32_t*)scratch;
     e.kept = e.counts + pairs;
@@ -348,7 +348,7 @@ int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const 
     m.pages[0] = kv->k; m.pages[1] = kv->v;
     m.table = kv->table; m.table_out = table_out; m.lens_out = lens_out;
     m.kept = e.kept; m.counts = e.counts;
-    m.n_pages = kv->pages; m.kv_heads = kv->kv_heads; m.page_len = kv->page_len; m.seqs = kv->seqs; m.table_len = kv->table_len; m.keep = keep;
+    m.n_pages = kv->pages; m.kv_heads = kv->kv_heads; m.page_len = kv->page_len; m.table_len = kv->table_len; m.keep = keep;
     // Elsewhere: whole rows.  In place the rows of a pair cannot be shared out, but their columns can: slices of 64 bytes at least, as many
     // as give four blocks a CU.
     const bool in_place = table_out == kv->table;
