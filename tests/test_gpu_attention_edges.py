@@ -83,3 +83,35 @@ def test_strides_of_extents_of_one(dev, dtype, queries, keys, heads, kv_heads):
     x, starts = ref.upload(dev, p.q, dtype), dev.upload(p.starts)
     want = dev.paged_attention(x, cache, starts).to_numpy()
     assert np.array_equal(dev.paged_attention(x, cache, starts, q_strides=(65, 67)).to_numpy().view(np.uint8), want.view(np.uint8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [4, 12, 28, 60, 76, 100, 132, 252])
+def test_whole_vectors_of_f32_columns(dev, dtype, dim):
+    """a multiple of 4 is whole vectors in f32 and not in 16 bits; 4 columns are one"""
+    rng = np.random.default_rng(dim)
+    dense(dev, rng, dtype, 2, 4, 2, 140, 300, dim, lens=[300, 170])
+    for new in ([1, 1, 1], [70, 2, 140]):
+        p = ref.Paged(rng, dtype, 4, 2, dim, 24, [100, 9, 301], new)
+        paged(dev, p, weights=rng.random((3, 2, p.cap), dtype=np.float32))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, kv_heads", [(130, 1), (400, 2), (129, 3)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 20]])
+def test_more_heads_to_a_kv_head_than_rows_to_a_tile(dev, dtype, heads, kv_heads, new):
+    rng = np.random.default_rng(heads)
+    p = ref.Paged(rng, dtype, heads, kv_heads, 64, 16, [900, 33, 300], new)
+    weights = rng.random((3, kv_heads, p.cap), dtype=np.float32)
+    paged(dev, p, weights=weights)
+    paged(dev, p, window=100, sinks=3, weights=weights)
+    dense(dev, rng, dtype, 2, heads, kv_heads, new[0], 200, 64, lens=[200, 5])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, kv_heads, new", [(8, 2, [1] * 5), (6, 2, [1, 90, 7, 1, 33]), (32, 4, [2, 1, 1, 300, 1])])
+@pytest.mark.parametrize("window, sinks", [(1, 0), (17, 40), (64, 1), (129, 0), (500, 200)])
+def test_windows_of_shared_heads_over_pages(dev, dtype, heads, kv_heads, new, window, sinks):
+    rng = np.random.default_rng(window)
+    p = ref.Paged(rng, dtype, heads, kv_heads, 48, 24, [1500, 400, 7, 300, 64], new, holes=[(0, 3), (1, 16)])
+    paged(dev, p, window=window, sinks=sinks, weights=rng.random((5, kv_heads, p.cap), dtype=np.float32))
