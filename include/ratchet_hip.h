@@ -253,7 +253,9 @@ int rt_gated_mul_via_f32(rt_device* dev, int op, int io_dt, const void* gate, ui
  * What the models build from a product, scale, mask, softmax and a second product (phi2/attn.rs:113-153,
  * phi3/attn.rs:143-153, whisper/mha.rs:115-124) without the scores ever reaching memory; the reference has no such op and no paged
  * cache.  Query head h reads KV head h / (heads / kv_heads).  Scores, softmax statistics and the sums over the keys are
- * f32; the result is rounded once to the element type (F32, F16, BF16).  With p the position of a query and len the
+ * f32, and the result is rounded to the element type (F32, F16, BF16).  Softmax weights of F16 and BF16 calls are rounded to the type as well, for
+ * their product with the values, where rows are whole 16-byte vectors of up to 256 columns on 16-byte boundaries; elsewhere they stay f32, so that the same
+ * row may differ by such roundings there.  With p the position of a query and len the
  * keys there are, key t is visible iff t < len and, where causal, 0 <= t <= p and (window == 0 or p - t < window or t < sinks):
  * a sliding window, and `sinks` first keys that stay in sight.  A query that sees no key, or none with a score above -inf, yields 0 and an lse of -inf;
  * what hidden keys and values hold, infinities and NaN included, does not matter.  y and lse overlap no input. */
@@ -303,7 +305,7 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
  * token; NaN ranks lowest), in their order, as tokens 0 .. keep - 1; shorter sequences stay whole.  The rows go into the pages of
  * table_out [seqs, table_len], their weights into weights_out, min(len, keep) into lens_out.  Each of the three may be its
  * input, the same pointer (the cache is then compacted in place, and a sequence that is cut shares no page of its tokens with
- * another); otherwise it overlaps no input, and the pages that table_out names are none of table's, none of them named
+ * another, nor names one twice); otherwise it overlaps no input, and the pages that table_out names are none of table's, none of them named
  * twice.  Rows whose page in table_out is not there are dropped; other rows of the pages stay as they were. */
 int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const float* weights, uint32_t keep, uint32_t first, uint32_t recent,
                    const int32_t* table_out, int32_t* lens_out, float* weights_out);

@@ -17,8 +17,8 @@
 // to 2^14 at most (f16's largest is 2^16; scores beyond 2^24, whose own rounding may pass that, make a row that is computed again): relative to the largest they
 // go down to 2^-30 at least, where rows are few to 2^-38.  l and O carry the same factor until the row is finished or its part is left.
 //
-// What bounds it, by counters: 8192 tokens of 32 heads of 96 with a window of 2047, bf16: 227 to 236 us, 770 to 800 TFLOP/s of the visible pairs' products; the
-// matrix units are busy 47 % and the vector units (scores to weights: about eight instructions each) 62 % of the time, and three waves of a SIMD have both overlap
+// What bounds it, by counters: 8192 tokens of 32 heads of 96 with a window of 2047, bf16: 227 to 244 us, 745 to 800 TFLOP/s of the visible pairs' products; the
+// matrix units are busy 47 % and the vector units (scores to weights: six to seven instructions each, by the counters) 62 % of the time, and three waves of a SIMD have both overlap
 // only in part.  f32, [4,6,1500,64]: 154 us, 79 % of it the matrix units, whose f32 products do an eighth of the 16-bit ones' work.  Single tokens, 64 of about
 // 4600 keys in bf16: 242 us, the keys and values once at 5.0 TB/s; a copy reaches 5.2.
 #ifndef RT_ATTENTION_TILE_H
@@ -39,13 +39,17 @@ template <> inline constexpr int AT_LIFT<half_t, true> = 14;
 // How far the keys of row tiles are shared out over blocks.  Single tokens (FEW): to AT_TARGET_FEW items, in pieces of no fewer than two tiles, which costs little as
 // their parts are small (one token's 2051 keys 17.9 us, with four tiles at least 19.3; 16 tokens 53 us at 1024 items, 61 at 512, 58 at 2048; 64 ragged
 // ones 255, 277, 251).  Others leave and join 64 KB a row tile and piece: only where the row tiles do not fill the chip by themselves (AT_ENOUGH), and to
-// AT_TARGET items (Phi-2 prompt, 512 row tiles: 45 us whole, 55 to 57 shared out; chunks, about 100 row tiles: 152 us at 256 items, 125 at 768, 142 at 1536;
+// AT_TARGET items (Phi-2 prompt, 512 row tiles: 45 us whole, 55 to 57 shared out; chunks, 320 row tiles: 152 us at 256 items, 125 at 768, 142 at 1536;
 // encoder, 288: 202, 149, 140).
 constexpr uint32_t AT_TARGET_FEW = 1024, AT_TARGET = 768, AT_ENOUGH = 512, AT_LEAST_TILES_FEW = 2, AT_LEAST_TILES = 4;
 constexpr uint32_t AT_SHORT = 40;                // tiles of keys to a row tile
 constexpr size_t AT_MOST_PARTS = 1u << 30;       // bytes of parts; a launch that would leave more shares nothing out
 constexpr uint32_t AT_MOST_PIECES = 60;          // of a row tile: their factors for its 128 rows fit the LDS of the smallest tiles
-constexpr uint32_t AT_FEW_ROWS = 16;             // rows of a sequence and KV head, on average, up to which a launch joins its own pieces
+// Rows of a sequence and KV head, on average, up to which a launch joins its own pieces.  The average, as the rows of each are known on the device alone: a step of 60 tokens
+// and one piece of a prompt is then few rows as well.  It is the faster for it (us, as few rows | as many: bf16, 32 heads on 8 of 128, up to 8000 keys, a piece of 60 tokens
+// 219 | 225, of 180 231 | 281; f32, up to 4000 keys, 180 487 | 760; 32 heads of 80, up to 2000 keys, 700 171 | 198) but for short caches (up to 400 keys, 180 42 | 36; 8
+// sequences, 25 64 | 55) and received weights, whose scores are then added up row after row (180 395 | 327; 700 563 | 412).
+constexpr uint32_t AT_FEW_ROWS = 16;
 constexpr uint32_t AT_JOIN_ROWS = 16;            // rows to a block of the joining kernel
 constexpr uint64_t AT_MOST_BLOCKS = (1u << 24) - 1;   // of a launch, which has fewer than 2^32 threads; more rows go to the kernel for any
 
@@ -335,7 +339,7 @@ __device__ __forceinline__ void at_row_again(const AttnArgs& a, uint32_t b, uint
 //   few rows (single tokens): the block that comes last.  Each counts itself in when its part is written, which for few rows is a few hundred bytes; parts then travel
 //       between blocks of one launch, and each XCD has an L2 of its own, so they are written and read as agent-scope atomics, which go past it, and a
 //       block counts itself in only when its writes have been acknowledged.
-//   many rows: a launch of its own, 16 rows to a block.  The last block alone would read a whole row tile's parts (64 KB each) through one CU.
+//   many rows: a launch of its own, 16 rows to a block.  The last block alone would read a whole row tile's parts (64 KB each) through one CU (see AT_FEW_ROWS for what is few).
 struct AttnPartial {
     float* o;                      // [blocks][AT_ROWS][dim], unnormalised
     float* ml;                     // [blocks][AT_ROWS][2]: m (of scaled scores, base 2), l
