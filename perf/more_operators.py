@@ -280,7 +280,7 @@ def prepare(case, seed):
     dev, both = _device(), {k: _buffer(v) for k, v in t.items()}
     b, s["seen"] = {k: v[0] for k, v in both.items()}, {k: v[1] for k, v in both.items()}
     if "rotary" in c:
-        s["table"] = dev.rope_table(c["rotary"], 10000.0, _divisors(c))
+        s["turns"] = dev.rope_table(c["rotary"], 10000.0, _divisors(c))
     s.update(b)
     if c["kind"] == "sample":
         s["logits"], s["stride"] = b["logits"].view(0, (c["rows"], c["vocab"])), c["vocab"] + c["padding"]
@@ -327,7 +327,7 @@ def _rotate(x, positions, frequencies, factor, interleaved, dtype):
 
 def _rope(s, c):
     if own:
-        _device().rope_tokens(s["qk"], s["positions"], s["table"], factor=s["factor"], interleaved=c["interleaved"], strides=s["strides"], out=s["o"])
+        _device().rope_tokens(s["qk"], s["positions"], s["turns"], factor=s["factor"], interleaved=c["interleaved"], strides=s["strides"], out=s["o"])
         return s["seen"]["o"]
     t = s["t"]
     return _rotate(t["qkv"][:, :c["heads"] + c["kv_heads"]], t["positions"], t["frequencies"], s["factor"], c["interleaved"], TORCH[c["dtype"]])
@@ -335,7 +335,7 @@ def _rope(s, c):
 
 def _rope_append(s, c):
     if own:
-        _device().paged_rope_append(s["cache"], s["starts"], s["q"], s["k"], s["v"], s["table"], factor=s["factor"], interleaved=c["interleaved"], q_strides=s["strides"],
+        _device().paged_rope_append(s["cache"], s["starts"], s["q"], s["k"], s["v"], s["turns"], factor=s["factor"], interleaved=c["interleaved"], q_strides=s["strides"],
                                     k_strides=s["strides"], v_strides=s["strides"], out=s["o"])
         return [s["seen"][k] for k in ("o", "k_pages", "v_pages")]
     t, h, g = s["t"], c["heads"], c["kv_heads"]
