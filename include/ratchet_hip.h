@@ -269,6 +269,27 @@ int rt_attention(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4
                  const uint64_t k_strides[4], const void* v, const uint64_t v_strides[4], const uint32_t kv_shape[4], const int32_t* lens,
                  void* y, const uint64_t y_strides[4], float* lse, float scale, int causal, uint32_t window, uint32_t sinks);
 
+/* Attention whose scores are changed, or masked by more than positions.  In the order they apply, s = scale * q.k first:
+ *   cap        0: none; otherwise s becomes cap * tanh(s / cap)
+ *   slopes     NULL: none; f32 [heads] on the device: s loses slopes[h] * |p - t|
+ *   documents  NULL: the keys are one text; i32 [B, n_documents + 1] on the device (rt_attention_scored alone), not decreasing: document d of entry b holds the keys
+ *              documents[b][d] .. documents[b][d + 1] - 1.  A query sees keys of the document that its position lies in, and none if that is in no document
+ *   prefix     NULL: none; i32 on the device, [B] or [seqs], with documents [B, n_documents]: so many first keys of a text that all of its queries
+ *              see, also those before them.  Needs causal attention
+ * so that with [lo, hi) the text of p, key t is visible iff lo <= t < hi and, where causal, t - lo < prefix or 0 <= t <= p and (window == 0 or p - t < window or
+ * t - lo < sinks).  All else is as rt_attention and rt_paged_attention have it; the latter's received weights are not to be had here. */
+typedef struct rt_scores {
+    float cap;
+    const float* slopes;
+    const int32_t* documents;
+    uint32_t n_documents;
+    const int32_t* prefix;
+} rt_scores;
+
+int rt_attention_scored(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4], const uint64_t q_strides[4], const void* k,
+                        const uint64_t k_strides[4], const void* v, const uint64_t v_strides[4], const uint32_t kv_shape[4], const int32_t* lens,
+                        void* y, const uint64_t y_strides[4], float* lse, float scale, int causal, uint32_t window, uint32_t sinks, const rt_scores* scores);
+
 /* A KV cache in pages.  k and v: [pages, kv_heads, page_len, head_dim], contiguous.  table: i32 [seqs, table_len], the pages
  * of each sequence in order; token t of sequence b is row t % page_len of page table[b][t / page_len].  An entry outside [0, pages)
  * is a page that is not there: its tokens are not written, are visible to no query and are evicted as zero rows.  lens: i32
@@ -300,6 +321,28 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
                        const rt_paged_kv* kv, const int32_t* starts, void* y, float* lse, const float* weights, float* weights_out, float scale,
                        uint32_t window, uint32_t sinks);
 
+int rt_paged_attention_scored(rt_device* dev, int dt, const void* q, const uint64_t q_strides[2], uint32_t tokens, uint32_t heads, const rt_paged_kv* kv,
+                              const int32_t* starts, void* y, float* lse, float scale, uint32_t window, uint32_t sinks, const rt_scores* scores);
+
+/* Rotary positions of tokens, each its own: row t of x [tokens, heads, head_dim] is turned to positions[t] (i32, on the device; negative
+ * ones turn back) and goes into y.  Columns (i, dim / 2 + i) or, interleaved, (2i, 2i + 1) are a pair, i < dim / 2, and become
+ * factor * (x1 cos - x2 sin, x1 sin + x2 cos) of the angle positions[t] * f_i; columns from dim on pass through.  turns (device, dim / 2 words of
+ * 64 bits): f_i / 2 pi as a fraction of a turn, times 2^64, so that far positions are as exact as near ones; products and sums are f32, rounded once.
+ * dt: F32, F16, BF16; dim even, at most 1024.  Strides (elements, NULL: contiguous) from token to token and from head to head; y may be x with the
+ * same strides, and otherwise overlaps no input.  Beside it rt_rope (ops/rope.rs) has one offset for all of a [B, H, S, D] tensor. */
+int rt_rope_tokens(rt_device* dev, int dt, const void* x, const uint64_t x_strides[2], void* y, const uint64_t y_strides[2], uint32_t tokens, uint32_t heads,
+                   uint32_t head_dim, const int32_t* positions, const uint64_t* turns, uint32_t dim, float factor, int interleaved);
+
+/* The table of rt_rope_tokens, in host memory: f_i = base^(-2i / dim) / divisors[i] (NULL: 1; scaled contexts divide by one number, or by a
+ * number for each frequency).  turns: dim / 2 words. */
+int rt_rope_turns(uint32_t dim, double base, const double* divisors, uint64_t* turns);
+
+/* rt_rope_tokens of q [tokens, heads, head_dim] into y, of k into its pages, and v into its, in one launch: the new tokens of a call (starts as above) at
+ * the positions that the cache gives them.  Rows of no sequence are left alone; where a page is not there, k and v are not written. */
+int rt_paged_rope_append(rt_device* dev, int dt, const rt_paged_kv* kv, const int32_t* starts, uint32_t tokens, const void* q, const uint64_t q_strides[2],
+                         uint32_t heads, void* y, const uint64_t y_strides[2], const void* k, const uint64_t k_strides[2], const void* v, const uint64_t v_strides[2],
+                         const uint64_t* turns, uint32_t dim, float factor, int interleaved);
+
 /* Eviction by accumulated weight: of a sequence with more than `keep` tokens the first `first`, the last `recent` and, for
  * each KV head on its own, the keep - first - recent others with the largest weights stay (equal weights: the lower
  * token; NaN ranks lowest), in their order, as tokens 0 .. keep - 1; shorter sequences stay whole.  The rows go into the pages of
@@ -309,6 +352,20 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
  * twice.  Rows whose page in table_out is not there are dropped; other rows of the pages stay as they were. */
 int rt_paged_evict(rt_device* dev, int elem_bytes, const rt_paged_kv* kv, const float* weights, uint32_t keep, uint32_t first, uint32_t recent,
                    const int32_t* table_out, int32_t* lens_out, float* weights_out);
+
+/* ---- Sampling ----------------------------------------------------------------------------------------------------------
+ * The next token of each row of logits x [rows, vocab] (row_stride elements apart, at least 0), from uniform f32 [rows] in [0, 1).  Every setting is an array with a
+ * number for each row, on the device, or NULL:
+ *   temperature f32  w_i = exp((x_i - max) / temperature); NULL: 1; not above 0: the largest logit is taken
+ *   top_k       i32  the top_k largest logits stay; not above 0, or vocab and more: all
+ *   top_p       f32  of those, in descending order, the ones that have less than top_p of their whole weight in front of them; 1 and more: all
+ *   min_p       f32  of all, those with w_i >= min_p (so many times as likely as the likeliest; above 1 as 1)
+ * tokens[r] is the first index at which the cumulative weight of those that stay, in the order of the indices, exceeds uniform[r] (taken into [0, 1)) times their whole
+ * weight.  Of equal logits the lower index comes first.  probs (NULL: not wanted) f32 [rows]: that token's share of the weight.  Weights are taken in
+ * 64 bits, and rounded to 2^-46 of the largest (2^-(62 - log2 vocab) for more than 2^16 tokens).  -inf and NaN are never chosen; a row of nothing else gives -1 and 0;
+ * +inf shares the weight with its equals.  vocab at most 2^24. */
+int rt_sample(rt_device* dev, int dt, const void* x, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float* temperature, const int32_t* top_k,
+              const float* top_p, const float* min_p, const float* uniform, int32_t* tokens, float* probs);
 
 #ifdef __cplusplus
 }

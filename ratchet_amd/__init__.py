@@ -5,6 +5,6 @@ in-tree into ratchet_amd/libratchet_hip.so.  This package is the thin Python bin
 """
 from . import _lib
 from ._lib import RatchetError
-from .runtime import Buffer, BufferView, Device, Event, PagedCache
+from .runtime import Buffer, BufferView, Device, Event, PagedCache, rope_divisors
 
-__all__ = ["Device", "Buffer", "BufferView", "Event", "PagedCache", "RatchetError", "_lib"]
+__all__ = ["Device", "Buffer", "BufferView", "Event", "PagedCache", "RatchetError", "rope_divisors", "_lib"]

@@ -29,6 +29,8 @@ EXPORTS = [
     "rt_event_elapsed_ms", "rt_binary", "rt_binary_bcast", "rt_unary", "rt_cast", "rt_permute", "rt_slice", "rt_broadcast",
     "rt_concat", "rt_cache", "rt_index_select", "rt_index_select_q8_0", "rt_index_write", "rt_rope", "rt_softmax", "rt_softmax_masked", "rt_layer_norm", "rt_rms_norm", "rt_group_norm", "rt_group_norm_static", "rt_norm_via_f32", "rt_softmax_via_f32", "rt_unary_via_f32", "rt_gated_mul_via_f32",
     "rt_attention", "rt_paged_append", "rt_paged_attention", "rt_paged_evict",
+    "rt_rope_tokens", "rt_rope_turns", "rt_paged_rope_append",
+    "rt_attention_scored", "rt_paged_attention_scored", "rt_sample",
 ]
 
 
@@ -36,6 +38,11 @@ class PagedKV(ctypes.Structure):
     """rt_paged_kv"""
     _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "table", "lens")] + [
         (n, ctypes.c_uint32) for n in ("pages", "kv_heads", "page_len", "head_dim", "seqs", "table_len")]
+
+
+class Scores(ctypes.Structure):
+    """rt_scores"""
+    _fields_ = [("cap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("documents", ctypes.c_void_p), ("n_documents", ctypes.c_uint32), ("prefix", ctypes.c_void_p)]
 
 
 class RatchetError(RuntimeError):
@@ -113,6 +120,13 @@ def load():
     L.rt_paged_append.argtypes = [vp, i, kv, vp, u32, vp, st, vp, st]
     L.rt_paged_attention.argtypes = [vp, i, vp, st, u32, u32, kv, vp, vp, vp, vp, vp, f, u32, u32]
     L.rt_paged_evict.argtypes = [vp, i, kv, vp, u32, u32, u32, vp, vp, vp]
+    L.rt_rope_tokens.argtypes = [vp, i, vp, st, vp, st, u32, u32, u32, vp, vp, u32, f, i]
+    L.rt_rope_turns.argtypes = [u32, ctypes.c_double, vp, vp]
+    L.rt_paged_rope_append.argtypes = [vp, i, kv, vp, u32, vp, st, u32, vp, st, vp, st, vp, st, vp, u32, f, i]
+    sc = ctypes.POINTER(Scores)
+    L.rt_attention_scored.argtypes = L.rt_attention.argtypes + [sc]
+    L.rt_paged_attention_scored.argtypes = [vp, i, vp, st, u32, u32, kv, vp, vp, vp, f, u32, u32, sc]
+    L.rt_sample.argtypes = [vp, i, vp, u64, u32, u32] + [vp] * 7
     for name in EXPORTS:
         fn = getattr(L, name)
         if name not in ("rt_last_error", "rt_status_name"):

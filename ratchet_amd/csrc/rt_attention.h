@@ -3,6 +3,7 @@
 // For one query row at position p (its head reads KV head head / G):
 //     s_t = c * q.k_t  over the visible keys t, c = scale * log2(e)        m = max s_t,  l = sum 2^(s_t - m)
 //     o = sum 2^(s_t - m) v_t / l                                          lse = ln 2 * (m + log2 l)
+// where the call changes its scores (SCORED), with z = scale * q.k_t: s_t = log2(e) * (cap tanh(z / cap) - slope |p - t|)
 // Keys are walked in tiles; m, l and o are kept running in f32 and o, l are scaled by 2^(m_old - m_new) where a tile raises m.
 #ifndef RT_ATTENTION_H
 #define RT_ATTENTION_H
@@ -40,6 +41,13 @@ struct AttnArgs {
     float* scores;                 // NULL, or [tokens, heads, score_pitch]: c q.k of each row and key, -inf where hidden, left for the received weights
     uint32_t score_pitch;
     bool want_scores;              // the caller has use for them
+    // calls that change or mask their scores (rt_scores)
+    bool scored;
+    float most, most_in;           // cap * log2(e), 0: none; scale / cap
+    const float* slopes;
+    const int32_t* documents;
+    uint32_t n_documents;
+    const int32_t* prefix;
 };
 
 // Scores of up to this size are kept between the attention of few rows and the sum of its weights; 64 bytes of q and k a score is what it would take to have them again
@@ -61,6 +69,10 @@ static inline int at_workspace(rt_device* dev, AttnArgs& a, size_t bytes, void**
 int rt_attention_tile_f32(rt_device* dev, AttnArgs& a, bool paged, bool* done);
 int rt_attention_tile_f16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
 int rt_attention_tile_bf16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
+// The same for calls that change or mask their scores
+int rt_attention_scored_f32(rt_device* dev, AttnArgs& a, bool paged, bool* done);
+int rt_attention_scored_f16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
+int rt_attention_scored_bf16(rt_device* dev, AttnArgs& a, bool paged, bool* done);
 // Received weights of a paged call that the kernel above took (rt_attention_weights.h); a.lse holds its rows' statistics
 int rt_attention_weights_f32(rt_device* dev, const AttnArgs& a, const float* weights, float* out);
 int rt_attention_weights_f16(rt_device* dev, const AttnArgs& a, const float* weights, float* out);
@@ -111,6 +123,64 @@ __device__ __forceinline__ int32_t at_limit(const AttnArgs& a, const AttnSeq& s,
 __device__ __forceinline__ int32_t at_position(const AttnSeq& s, uint32_t j) { return (int32_t)j + s.shift; }
 __device__ __forceinline__ bool at_visible(const AttnArgs& a, int32_t t, int32_t limit, int32_t p) {
     return t <= limit && (p - t < a.window || t < a.sinks);
+}
+
+// What a row sees: keys lo .. limit, but where p - t >= window those before `front` alone.  Over rows in order none of the four decreases.
+struct AttnRow {
+    int32_t p, limit, lo, front;
+};
+__device__ __forceinline__ int32_t at_between(int32_t x, int32_t low, int32_t high) { return x < low ? low : x > high ? high : x; }
+// The row at position p of a text that holds keys lo .. hi - 1
+__device__ __forceinline__ AttnRow at_in_text(const AttnArgs& a, int32_t p, int32_t lo, int32_t hi, int32_t prefix) {
+    const int32_t seen = at_between(prefix, 0, hi - lo), wide = a.sinks > seen ? a.sinks : seen;
+    AttnRow r = {p, hi - 1, lo, wide < hi - lo ? lo + wide : hi};
+    if (a.causal) {
+        const int32_t own = p < hi - 1 ? p : hi - 1, shared = lo + seen - 1;
+        r.limit = own > shared ? own : shared;
+        if (r.limit < lo) r.limit = lo - 1;
+    }
+    return r;
+}
+// The document of position p: the last that begins at or before it; n_documents or above where it is in none.  All lanes of a wave take part, with the same p.
+__device__ __forceinline__ uint32_t at_find(const int32_t* starts, uint32_t seqs, uint32_t token);
+__device__ __forceinline__ uint32_t at_document(const AttnArgs& a, uint32_t b, int32_t p) {
+    return at_find(a.documents + (uint64_t)b * (a.n_documents + 1), a.n_documents + 1, (uint32_t)p);
+}
+__device__ __forceinline__ AttnRow at_in_document(const AttnArgs& a, uint32_t b, const AttnSeq& s, int32_t p, uint32_t d) {
+    const int32_t* at = a.documents + (uint64_t)b * (a.n_documents + 1);
+    if (d >= a.n_documents) {                      // in front of the first, or behind the last: a text without keys
+        const int32_t here = at_between(at[d == a.n_documents ? d : 0], 0, s.keys);
+        return at_in_text(a, p, here, here, 0);
+    }
+    const int32_t lo = at_between(at[d], 0, s.keys), hi = at_between(at[d + 1], lo, s.keys);
+    return at_in_text(a, p, lo, hi, a.prefix ? a.prefix[(uint64_t)b * a.n_documents + d] : 0);
+}
+// Row j of sequence b; all lanes take part, with the same row
+template <bool SCORED> __device__ __forceinline__ AttnRow at_row(const AttnArgs& a, uint32_t b, const AttnSeq& s, uint32_t j) {
+    const int32_t p = at_position(s, j);
+    if (!SCORED) return AttnRow{p, at_limit(a, s, j), 0, a.sinks};
+    if (a.documents) return at_in_document(a, b, s, p, at_document(a, b, p));
+    return at_in_text(a, p, 0, s.keys, a.prefix ? a.prefix[b] : 0);
+}
+template <bool SCORED> __device__ __forceinline__ bool at_sees(const AttnArgs& a, const AttnRow& r, int32_t t) {
+    return t <= r.limit && (!SCORED || t >= r.lo) && (r.p - t < a.window || t < r.front);
+}
+
+// cap * tanh(z / cap) in units of log2(e), y = z / cap: tanh y = 1 - 2 / (e^2y + 1), off by about 2^-23 of the cap, which is less than a 16-bit weight's rounding.
+// In f32 the small ones, whose differences that would swamp, take the odd series up to y^9 (below 0.3 the next term is under 6e-8 of it).
+template <typename T> __device__ __forceinline__ float at_capped(float cap, float y) {
+    const float t = __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * 2.885390081777927f) + 1.0f), cap);
+    if (sizeof(T) == 2) return t;
+    const float z = y * y;
+    const float near = cap * __builtin_fmaf(y * z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 62.0f / 2835, -17.0f / 315), 2.0f / 15), -1.0f / 3), y);
+    return __builtin_fabsf(y) < 0.3f ? near : t;
+}
+// The score, in units of log2(e), of a product q.k; slope: in the same units
+template <typename T, bool SCORED> __device__ __forceinline__ float at_changed(const AttnArgs& a, float dot, float slope, int32_t distance) {
+    if (!SCORED) return dot * a.c;
+    float x = a.most != 0.0f ? at_capped<T>(a.most, dot * a.most_in) : dot * a.c;
+    if (a.slopes) x = __builtin_fmaf(-slope, __builtin_fabsf((float)distance), x);
+    return x;
 }
 
 // The page of token t, or -1 if there is none

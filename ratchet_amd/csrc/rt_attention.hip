@@ -11,7 +11,7 @@ constexpr uint32_t GRID_ROW = 1u << 22;          // blocks to a row of the grid:
 // A wave to a (query, head) row.  A lane computes the score of one key of a tile of 64; the tile's weights then go round the wave, key by key, and
 // each lane adds them to its columns.  Hidden keys are skipped there, so nothing they hold is ever multiplied.
 // Simple, and 50 to 800 times slower than the tiles: bound by its scalar dot products and uncoalesced key reads ([4,6,1500,64] f32 14.5 ms, with tiles 0.15)
-template <typename T, bool PAGED>
+template <typename T, bool PAGED, bool SCORED>
 __global__ void __launch_bounds__(BLOCK) attention_any_kernel(AttnArgs a, uint64_t rows) {
     const uint32_t lane = threadIdx.x % 64;
     const uint64_t row = ((uint64_t)blockIdx.y * GRID_ROW + blockIdx.x) * WAVES + threadIdx.x / 64;
@@ -35,14 +35,15 @@ __global__ void __launch_bounds__(BLOCK) attention_any_kernel(AttnArgs a, uint64
     const T* q = (const T*)a.q + b * a.q_b + h * a.q_h + (uint64_t)(s.first + j) * a.q_t;
     const T* k = (const T*)a.k + g * a.k_h + (PAGED ? 0 : b * a.k_b);
     const T* v = (const T*)a.v + g * a.v_h + (PAGED ? 0 : b * a.v_b);
-    const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
+    const AttnRow r = at_row<SCORED>(a, b, s, j);
+    const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
     float m = -INFINITY, l = 0.0f, o[AT_MAX_DIM / 64];
 #pragma unroll
     for (int i = 0; i < AT_MAX_DIM / 64; i++) o[i] = 0.0f;
-    for (int32_t t0 = 0; t0 <= limit; t0 += 64) {
-        if (t0 >= a.sinks && p - (t0 + 63) >= a.window) continue;
+    for (int32_t t0 = r.lo / 64 * 64; t0 <= r.limit; t0 += 64) {
+        if (t0 >= r.front && r.p - (t0 + 63) >= a.window) continue;
         const int32_t t = t0 + (int32_t)lane;
-        bool seen = at_visible(a, t, limit, p);
+        bool seen = at_sees<SCORED>(a, r, t);
         uint64_t k_at = 0, v_at = 0;
         if (seen) {
             if (PAGED) {
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(BLOCK) attention_any_kernel(AttnArgs a, uint64
         if (seen) {
             float dot = 0.0f;
             for (uint32_t d = 0; d < D; d++) dot = __builtin_fmaf(Ar<T>::widen(q[d]), Ar<T>::widen(k[k_at + d]), dot);
-            x = dot * a.c;
+            x = at_changed<T, SCORED>(a, dot, slope, r.p - t);
         }
         uint64_t todo = __ballot(seen);
         if (!todo) continue;
@@ -127,8 +128,10 @@ template <typename T> int launch_any(rt_device* dev, const AttnArgs& a, bool pag
     const uint64_t rows = (uint64_t)(paged ? 1 : a.seqs) * a.tokens * a.heads, blocks = (rows + WAVES - 1) / WAVES;
     RT_REQUIRE(blocks <= 65535ull * GRID_ROW, RT_ERR_SIZE, "attention: too many rows");
     const dim3 grid((unsigned)(blocks < GRID_ROW ? blocks : GRID_ROW), (unsigned)((blocks + GRID_ROW - 1) / GRID_ROW));
-    if (paged) hipLaunchKernelGGL((attention_any_kernel<T, true>), grid, dim3(BLOCK), 0, dev->stream, a, rows);
-    else hipLaunchKernelGGL((attention_any_kernel<T, false>), grid, dim3(BLOCK), 0, dev->stream, a, rows);
+    if (paged && a.scored) hipLaunchKernelGGL((attention_any_kernel<T, true, true>), grid, dim3(BLOCK), 0, dev->stream, a, rows);
+    else if (paged) hipLaunchKernelGGL((attention_any_kernel<T, true, false>), grid, dim3(BLOCK), 0, dev->stream, a, rows);
+    else if (a.scored) hipLaunchKernelGGL((attention_any_kernel<T, false, true>), grid, dim3(BLOCK), 0, dev->stream, a, rows);
+    else hipLaunchKernelGGL((attention_any_kernel<T, false, false>), grid, dim3(BLOCK), 0, dev->stream, a, rows);
     RT_CHECK_LAUNCH("attention_any_kernel");
     if (weights_out) {
         hipLaunchKernelGGL((attention_weights_any_kernel<T>), dim3((a.cap + 63) / 64, a.kv_heads, a.seqs), dim3(64), 0, dev->stream, a, weights, weights_out);
@@ -139,7 +142,9 @@ template <typename T> int launch_any(rt_device* dev, const AttnArgs& a, bool pag
 
 int dispatch(rt_device* dev, int dt, AttnArgs& a, bool paged, const float* weights, float* weights_out) {
     bool done;
-    int rc = dt == RT_F32 ? rt_attention_tile_f32(dev, a, paged, &done) : dt == RT_F16 ? rt_attention_tile_f16(dev, a, paged, &done) : rt_attention_tile_bf16(dev, a, paged, &done);
+    int rc;
+    if (a.scored) rc = dt == RT_F32 ? rt_attention_scored_f32(dev, a, paged, &done) : dt == RT_F16 ? rt_attention_scored_f16(dev, a, paged, &done) : rt_attention_scored_bf16(dev, a, paged, &done);
+    else rc = dt == RT_F32 ? rt_attention_tile_f32(dev, a, paged, &done) : dt == RT_F16 ? rt_attention_tile_f16(dev, a, paged, &done) : rt_attention_tile_bf16(dev, a, paged, &done);
     if (rc || (done && !weights_out)) return rc;
     if (done) {
         switch (dt) {
@@ -174,6 +179,27 @@ int head_rules(const char* who, int dt, uint32_t heads, uint32_t kv_heads, uint3
     a.c = scale * 1.4426950408889634f;
     a.window = window == 0 || window >= MOST_TOKENS ? AT_FAR : (int32_t)window;               // as far as positions go
     a.sinks = sinks > MOST_TOKENS ? AT_MOST_TOKENS : (int32_t)sinks;
+    return RT_OK;
+}
+
+// What changes or masks the scores; `documents`: the call may have them
+int score_rules(const char* who, const rt_scores* scores, float scale, uint32_t batch, bool documents, bool causal, AttnArgs& a) {
+    RT_REQUIRE(scores, RT_ERR_NULL_POINTER, "%s: NULL scores", who);
+    RT_REQUIRE(scores->cap >= 0.0f && isfinite(scores->cap), RT_ERR_ARG, "%s: cap must be finite and not negative", who);
+    RT_REQUIRE(scores->cap == 0.0f || isfinite(scores->cap * 1.4426950408889634f), RT_ERR_ARG, "%s: cap is too large", who);
+    RT_REQUIRE(scores->cap == 0.0f || isfinite(scale / scores->cap), RT_ERR_ARG, "%s: scale / cap is not finite", who);
+    RT_REQUIRE(documents || !scores->documents, RT_ERR_ARG, "%s: sequences are not cut into documents", who);
+    RT_REQUIRE(!scores->documents == !scores->n_documents, RT_ERR_SHAPE, "%s: %u documents", who, scores->n_documents);
+    RT_REQUIRE(!scores->prefix || causal, RT_ERR_ARG, "%s: a prefix needs causal attention", who);
+    RT_REQUIRE(scores->n_documents <= (uint32_t)AT_MOST_TOKENS && (uint64_t)batch * (scores->n_documents + 1ull) <= RT_MAX_NUMEL, RT_ERR_SIZE, "%s: %u documents", who, scores->n_documents);
+    RT_REQUIRE(rt_aligned(scores->slopes, 4) && rt_aligned(scores->documents, 4) && rt_aligned(scores->prefix, 4), RT_ERR_ALIGN, "%s: misaligned pointer", who);
+    a.scored = scores->cap != 0.0f || scores->slopes || scores->documents || scores->prefix;       // else it is attention as it ever was
+    a.most = scores->cap * 1.4426950408889634f;
+    a.most_in = scores->cap != 0.0f ? scale / scores->cap : 0.0f;
+    a.slopes = scores->slopes;
+    a.documents = scores->documents;
+    a.n_documents = scores->n_documents;
+    a.prefix = scores->prefix;
     return RT_OK;
 }
 
@@ -236,12 +262,11 @@ int rt_rows_rules(const char* who, const char* what, uint32_t tokens, uint32_t h
     return RT_OK;
 }
 
-extern "C" {
+namespace {
 
-int rt_attention(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4], const uint64_t q_strides[4], const void* k, const uint64_t k_strides[4],
+int attention(const char* who, rt_device* dev, int dt, const void* q, const uint32_t q_shape[4], const uint64_t q_strides[4], const void* k, const uint64_t k_strides[4],
                  const void* v, const uint64_t v_strides[4], const uint32_t kv_shape[4], const int32_t* lens, void* y, const uint64_t y_strides[4], float* lse,
-                 float scale, int causal, uint32_t window, uint32_t sinks) {
-    static const char* const who = "rt_attention";
+                 float scale, int causal, uint32_t window, uint32_t sinks, const rt_scores* scores, bool scored) {
     AttnArgs a = {};
     RT_REQUIRE(q_shape && kv_shape, RT_ERR_NULL_POINTER, "%s: NULL shape", who);
     int rc = head_rules(who, dt, q_shape[1], kv_shape[1], q_shape[3], scale, window, sinks, a);
@@ -252,6 +277,7 @@ int rt_attention(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4
     RT_REQUIRE(q_shape[2] <= MOST_TOKENS && kv_shape[2] <= MOST_TOKENS, RT_ERR_SIZE, "%s: %u queries, %u keys", who, q_shape[2], kv_shape[2]);
     RT_REQUIRE(causal == 0 || causal == 1, RT_ERR_ARG, "%s: causal is %d", who, causal);
     RT_REQUIRE(causal || (window == 0 && sinks == 0), RT_ERR_ARG, "%s: a window needs causal attention", who);
+    if (scored && (rc = score_rules(who, scores, scale, q_shape[0], true, causal != 0, a))) return rc;
     uint64_t qs[4], ks[4], vs[4], ys[4];
     if ((rc = stride_rules(who, "q", q_shape, q_strides, qs))) return rc;
     if ((rc = stride_rules(who, "k", kv_shape, k_strides, ks))) return rc;
@@ -277,9 +303,9 @@ int rt_attention(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4
     return dispatch(dev, dt, a, false, nullptr, nullptr);
 }
 
-int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_strides[2], uint32_t tokens, uint32_t heads, const rt_paged_kv* kv,
-                       const int32_t* starts, void* y, float* lse, const float* weights, float* weights_out, float scale, uint32_t window, uint32_t sinks) {
-    static const char* const who = "rt_paged_attention";
+int paged_attention(const char* who, rt_device* dev, int dt, const void* q, const uint64_t q_strides[2], uint32_t tokens, uint32_t heads, const rt_paged_kv* kv,
+                       const int32_t* starts, void* y, float* lse, const float* weights, float* weights_out, float scale, uint32_t window, uint32_t sinks,
+                    const rt_scores* scores, bool scored) {
     AttnArgs a = {};
     RT_REQUIRE(kv, RT_ERR_NULL_POINTER, "%s: NULL cache", who);
     int rc = head_rules(who, dt, heads, kv->kv_heads, kv->head_dim, scale, window, sinks, a);
@@ -287,6 +313,7 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
     const size_t e = (size_t)rt_dt_bytes(dt);
     if ((rc = rt_paged_rules(who, kv, e))) return rc;
     if ((rc = rt_rows_rules(who, "q", tokens, heads, kv->head_dim, q_strides, &a.q_t, &a.q_h))) return rc;
+    if (scored && (rc = score_rules(who, scores, scale, kv->seqs, false, true, a))) return rc;
     RT_REQUIRE(q && starts && y, RT_ERR_NULL_POINTER, "%s: NULL operand", who);
     RT_REQUIRE(!weights == !weights_out, RT_ERR_NULL_POINTER, "%s: weights and weights_out go together", who);
     RT_REQUIRE((uint64_t)tokens * heads <= RT_MAX_NUMEL / kv->head_dim, RT_ERR_SIZE, "%s: y is too large", who);
@@ -312,6 +339,32 @@ int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_s
     a.want_scores = weights_out != nullptr;
     a.own_lse = weights_out && !lse ? (size_t)tokens * heads * sizeof(float) : 0;
     return dispatch(dev, dt, a, true, weights, weights_out);
+}
+
+}  // namespace
+
+extern "C" {
+
+int rt_attention(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4], const uint64_t q_strides[4], const void* k, const uint64_t k_strides[4],
+                 const void* v, const uint64_t v_strides[4], const uint32_t kv_shape[4], const int32_t* lens, void* y, const uint64_t y_strides[4], float* lse,
+                 float scale, int causal, uint32_t window, uint32_t sinks) {
+    return attention("rt_attention", dev, dt, q, q_shape, q_strides, k, k_strides, v, v_strides, kv_shape, lens, y, y_strides, lse, scale, causal, window, sinks, nullptr, false);
+}
+
+int rt_attention_scored(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4], const uint64_t q_strides[4], const void* k, const uint64_t k_strides[4],
+                        const void* v, const uint64_t v_strides[4], const uint32_t kv_shape[4], const int32_t* lens, void* y, const uint64_t y_strides[4], float* lse,
+                        float scale, int causal, uint32_t window, uint32_t sinks, const rt_scores* scores) {
+    return attention("rt_attention_scored", dev, dt, q, q_shape, q_strides, k, k_strides, v, v_strides, kv_shape, lens, y, y_strides, lse, scale, causal, window, sinks, scores, true);
+}
+
+int rt_paged_attention(rt_device* dev, int dt, const void* q, const uint64_t q_strides[2], uint32_t tokens, uint32_t heads, const rt_paged_kv* kv,
+                       const int32_t* starts, void* y, float* lse, const float* weights, float* weights_out, float scale, uint32_t window, uint32_t sinks) {
+    return paged_attention("rt_paged_attention", dev, dt, q, q_strides, tokens, heads, kv, starts, y, lse, weights, weights_out, scale, window, sinks, nullptr, false);
+}
+
+int rt_paged_attention_scored(rt_device* dev, int dt, const void* q, const uint64_t q_strides[2], uint32_t tokens, uint32_t heads, const rt_paged_kv* kv,
+                              const int32_t* starts, void* y, float* lse, float scale, uint32_t window, uint32_t sinks, const rt_scores* scores) {
+    return paged_attention("rt_paged_attention_scored", dev, dt, q, q_strides, tokens, heads, kv, starts, y, lse, nullptr, nullptr, scale, window, sinks, scores, true);
 }
 
 }  // extern "C"

@@ -1,0 +1,4 @@
+// The attention kernels of rt_attention_tile.h for f32, for calls that change or mask their scores
+#include "rt_attention_tile.h"
+
+int rt_attention_scored_f32(rt_device* dev, AttnArgs& a, bool paged, bool* done) { return at_dispatch_tile<float, true>(dev, a, paged, done); }

@@ -55,10 +55,12 @@ constexpr uint64_t AT_MOST_BLOCKS = (1u << 24) - 1;   // of a launch, which has 
 
 // ------------------------------------------------------------------------------------------------- who does what
 // Tiles of KT keys that a tile of rows of sequence s may see at most; 1 where there are no keys, for the block that writes the zeros
-template <int KT> __device__ __forceinline__ uint32_t at_span(const AttnArgs& a, const AttnSeq& s) {
+template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_span(const AttnArgs& a, uint32_t b, const AttnSeq& s) {
     uint32_t n = ((uint32_t)s.keys + KT - 1) / KT;
     if (a.window != AT_FAR) {
-        const uint64_t w = ((uint64_t)a.window + AT_ROWS) / KT + 2 + ((uint64_t)a.sinks + KT - 1) / KT;
+        int32_t front = a.sinks;
+        if (SCORED && a.prefix && a.prefix[b] > front) front = a.prefix[b];
+        const uint64_t w = ((uint64_t)a.window + AT_ROWS) / KT + 2 + ((uint64_t)front + KT - 1) / KT;
         n = w < n ? (uint32_t)w : n;
     }
     return n ? n : 1;
@@ -79,12 +81,12 @@ template <bool FEW> __host__ __device__ __forceinline__ uint32_t at_piece_for(ui
     return n < least ? least : n > 0x7fffffffu ? 0x7fffffffu : (uint32_t)n;
 }
 // The same from the device's lengths; the same in every wave.
-template <int KT, bool FEW> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a) {
+template <int KT, bool FEW, bool SCORED> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a) {
     uint64_t work = 0;
     uint32_t tiles = 0;
     for (uint32_t b = __lane_id(); b < a.seqs; b += 64) {
         const AttnSeq s = at_seq<true>(a, b);
-        const uint32_t span = at_span<KT>(a, s), less = FEW ? 0 : s.count / (2 * KT);           // causal: the middle row of the new ones lacks half of them
+        const uint32_t span = at_span<KT, SCORED>(a, b, s), less = FEW ? 0 : s.count / (2 * KT);           // causal: the middle row of the new ones lacks half of them
         work += (uint64_t)at_row_tiles(a, s) * (span > 2 * less ? span - less : (span + 1) / 2);
         tiles += at_row_tiles(a, s);
     }
@@ -98,16 +100,16 @@ __host__ __device__ __forceinline__ uint32_t at_piece_of(uint32_t piece, uint32_
 }
 
 // Sequence b's items are numbered row tile by row tile, at_items of them, after those of the sequences before it.
-template <int KT> __device__ __forceinline__ uint32_t at_items(const AttnArgs& a, uint32_t b, uint32_t piece) {
+template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_items(const AttnArgs& a, uint32_t b, uint32_t piece) {
     const AttnSeq s = at_seq<true>(a, b);
-    const uint32_t span = at_span<KT>(a, s), n = at_piece_of(piece, span);
+    const uint32_t span = at_span<KT, SCORED>(a, b, s), n = at_piece_of(piece, span);
     return at_row_tiles(a, s) * ((span + n - 1) / n);
 }
 // The sequence that item `at` belongs to (a.seqs: none); `at` becomes its number there.  All lanes of a wave take part.
-template <int KT> __device__ __forceinline__ uint32_t at_locate(const AttnArgs& a, uint32_t piece, uint32_t& at) {
+template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_locate(const AttnArgs& a, uint32_t piece, uint32_t& at) {
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.seqs; b0 += 64) {
-        const uint32_t b = b0 + __lane_id(), n = b < a.seqs ? at_items<KT>(a, b, piece) : 0;
+        const uint32_t b = b0 + __lane_id(), n = b < a.seqs ? at_items<KT, SCORED>(a, b, piece) : 0;
         uint32_t sum = n;                                       // of this lane and those below
 #pragma unroll
         for (int i = 1; i < 64; i <<= 1) {
@@ -124,31 +126,42 @@ template <int KT> __device__ __forceinline__ uint32_t at_locate(const AttnArgs& 
     }
     return a.seqs;
 }
-template <int KT> __device__ __forceinline__ uint32_t at_before(const AttnArgs& a, uint32_t piece, uint32_t until) {
+template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_before(const AttnArgs& a, uint32_t piece, uint32_t until) {
     uint32_t sum = 0;
-    for (uint32_t b = __lane_id(); b < until; b += 64) sum += at_items<KT>(a, b, piece);
+    for (uint32_t b = __lane_id(); b < until; b += 64) sum += at_items<KT, SCORED>(a, b, piece);
     return at_wave_sum(sum);
 }
 
-// A row tile's walk over the keys: `tiles` of them, the first `head` from key 0 on, the others from key `from` on
+// A row tile's walk over the keys: `tiles` of them, the first `head` from key `start` on, the others from key `from` on
 struct AttnWalk {
     uint32_t tiles, head;
-    int32_t from;
+    int32_t start, from;
 };
-template <int KT> __device__ __forceinline__ AttnWalk at_walk(const AttnArgs& a, const AttnSeq& s, uint32_t row0, uint32_t rows) {
+template <int KT, bool SCORED> __device__ __forceinline__ AttnWalk at_walk(const AttnArgs& a, uint32_t b, const AttnSeq& s, uint32_t row0, uint32_t rows) {
     const uint32_t j0 = fd_div(row0, a.group_div), j1 = fd_div(row0 + rows - 1, a.group_div);
-    const int32_t last = at_limit(a, s, j1);
-    AttnWalk w = {0, 0, 0};
-    if (last < 0) return w;
+    AttnRow r0 = at_row<SCORED>(a, b, s, j0);
+    int32_t last = at_row<SCORED>(a, b, s, j1).limit;
+    if (SCORED) {                                               // the same in all lanes, which the compiler cannot know
+        r0.p = __builtin_amdgcn_readfirstlane(r0.p);
+        r0.lo = __builtin_amdgcn_readfirstlane(r0.lo);
+        r0.front = __builtin_amdgcn_readfirstlane(r0.front);
+        last = __builtin_amdgcn_readfirstlane(last);
+    }
+    const int32_t start = SCORED ? r0.lo / KT * KT : 0;
+    AttnWalk w = {0, 0, start, start};
+    if (last < r0.lo) return w;
     if (a.window != AT_FAR) {
-        const int32_t first = at_position(s, j0) - a.window + 1;                // the first key of the first row's window
-        const int32_t from = first > 0 ? first / KT * KT : 0;
-        const uint32_t head = ((uint32_t)(a.sinks < from ? a.sinks : from) + KT - 1) / KT;
-        if ((int32_t)(head * KT) < from) {
+        // the first key of the first row's window; what later texts of the tile keep in front lies behind it
+        const int32_t first = r0.p - a.window + 1;
+        const int32_t from = first > r0.lo ? first / KT * KT : start;
+        const int32_t front = r0.front < from ? r0.front : from;
+        const uint32_t head = front > start ? ((uint32_t)(front - start) + KT - 1) / KT : 0;
+        if (start + (int32_t)(head * KT) < from) {
             w.head = head;
             w.from = from;
-            if (from > last) {                                  // rows beyond the last key there is room for: only the sinks are left
-                w.tiles = head < (uint32_t)last / KT + 1 ? head : (uint32_t)last / KT + 1;
+            if (from > last) {                                  // rows beyond the last key there is room for: only the front is left
+                const uint32_t most = (uint32_t)(last - start) / KT + 1;
+                w.tiles = head < most ? head : most;
                 return w;
             }
         }
@@ -277,7 +290,7 @@ __device__ __forceinline__ void at_settle(const v16f& sum) {
 }
 
 // One row over the keys of tiles [tile0, tile1) of a walk, a lane to a key for the scores and to columns for the result: visible keys alone are touched.
-template <typename T, int DT, bool PAGED, int KT>
+template <typename T, int DT, bool PAGED, int KT, bool SCORED>
 __device__ __forceinline__ void at_row_again(const AttnArgs& a, uint32_t b, uint32_t g, AttnSeq s, AttnWalk w, uint32_t tile0, uint32_t tile1, uint32_t row, float* o, float& m_out,
                                           float& l_out) {
     constexpr int COLS = (DT + 63) / 64;
@@ -285,13 +298,14 @@ __device__ __forceinline__ void at_row_again(const AttnArgs& a, uint32_t b, uint
     const T* q = (const T*)a.q + b * a.q_b + h * a.q_h + (uint64_t)(s.first + j) * a.q_t;
     const T* k = (const T*)a.k + g * a.k_h + (PAGED ? 0 : b * a.k_b);
     const T* v = (const T*)a.v + g * a.v_h + (PAGED ? 0 : b * a.v_b);
-    const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
+    const AttnRow r = at_row<SCORED>(a, b, s, j);
+    const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int i = 0; i < COLS; i++) o[i] = 0.0f;
     for (uint32_t tile = tile0; tile < tile1; tile++) {
-        const int32_t t = (tile < w.head ? (int32_t)(tile * KT) : w.from + (int32_t)((tile - w.head) * KT)) + (int32_t)lane;
-        bool seen = lane < KT && at_visible(a, t, limit, p);
+        const int32_t t = (tile < w.head ? w.start + (int32_t)(tile * KT) : w.from + (int32_t)((tile - w.head) * KT)) + (int32_t)lane;
+        bool seen = lane < KT && at_sees<SCORED>(a, r, t);
         uint64_t k_at = 0, v_at = 0;
         if (seen) {
             if (PAGED) {
@@ -309,7 +323,7 @@ __device__ __forceinline__ void at_row_again(const AttnArgs& a, uint32_t b, uint
         if (seen) {
             float dot = 0.0f;
             for (uint32_t d = 0; d < D; d++) dot = __builtin_fmaf(Ar<T>::widen(q[d]), Ar<T>::widen(k[k_at + d]), dot);
-            x = dot * a.c;
+            x = at_changed<T, SCORED>(a, dot, slope, r.p - t);
         }
         uint64_t todo = __ballot(seen);
         if (!todo) continue;
@@ -475,8 +489,8 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
 
 // FEW: pieces are joined by the block that comes last (a joining launch took 10 to 13 us more), and scores are left where they are
 // wanted.  Waves of a SIMD: as many as the registers let, four where the rows have 64 columns and no page table is followed (encoder in f32: 146.5 us a call, with three 148.7)
-template <typename T, int DT, bool EXACT, bool PAGED, bool FEW>
-__global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW), AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW)))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
+template <typename T, int DT, bool EXACT, bool PAGED, bool FEW, bool SCORED>
+__global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW && !SCORED), AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW && !SCORED)))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
     typedef AtShape<T, DT> S;
     constexpr int KT = S::KT, CE = S::CE;
     constexpr float LIFT = AT_LIFT<T, FEW>, LOWER = 1.0f / (1 << AT_LIFT<T, FEW>);              // the weights' factor is 2^LIFT, 1 / LOWER
@@ -492,8 +506,8 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         stride = a.kv_heads;
         g = blockIdx.x % a.kv_heads;
         uint32_t at = blockIdx.x / a.kv_heads;
-        piece = part.split ? __builtin_amdgcn_readfirstlane(at_piece<KT, FEW>(a)) : 0x7fffffffu;
-        b = __builtin_amdgcn_readfirstlane(at_locate<KT>(a, piece, at));
+        piece = part.split ? __builtin_amdgcn_readfirstlane(at_piece<KT, FEW, SCORED>(a)) : 0x7fffffffu;
+        b = __builtin_amdgcn_readfirstlane(at_locate<KT, SCORED>(a, piece, at));
         if (b >= a.seqs) return;
         tile = __builtin_amdgcn_readfirstlane(at);
         piece_at = 0;
@@ -507,7 +521,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
     }
     const AttnSeq s = at_seq<PAGED>(a, b);
     if (PAGED) {
-        const uint32_t span = at_span<KT>(a, s), at = tile;
+        const uint32_t span = at_span<KT, SCORED>(a, b, s), at = tile;
         piece = at_piece_of(piece, span);
         const uint32_t pieces = (span + piece - 1) / piece;
         tile = at / pieces;
@@ -515,7 +529,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         tile = at_row_tiles(a, s) - 1 - tile;
     }
     const uint32_t all = s.count * a.group, row0 = tile * AT_ROWS, rows = all - row0 < AT_ROWS ? all - row0 : AT_ROWS;
-    const AttnWalk w = at_walk<KT>(a, s, row0, rows);
+    const AttnWalk w = at_walk<KT, SCORED>(a, b, s, row0, rows);
     const uint32_t tile0 = piece_at * piece, tile1 = w.tiles - tile0 < piece || tile0 >= w.tiles ? w.tiles : tile0 + piece;
     const bool whole = w.tiles <= piece;                        // no other block has keys of these rows
     if (tile0 >= w.tiles && piece_at > 0) return;
@@ -525,11 +539,40 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
     // ---- this lane's row
     const uint32_t r = wave * 32 + col, row = row0 + (r < rows ? r : rows - 1);
     const uint32_t j = fd_div(row, a.group_div), h = g * a.group + (row - j * a.group);
-    const int32_t limit = at_limit(a, s, j), p = at_position(s, j);
     // and what all rows of the wave see, and any of them
     const bool busy = wave * 32 < rows;
     const uint32_t ja = fd_div(row0 + (busy ? wave * 32 : 0), a.group_div), jz = fd_div(row0 + (wave * 32 + 31 < rows ? wave * 32 + 31 : rows - 1), a.group_div);
-    const int32_t limit_a = at_limit(a, s, ja), limit_z = at_limit(a, s, jz), p_a = at_position(s, ja), p_z = at_position(s, jz);
+    int32_t limit, p, limit_a, limit_z, p_a, p_z;
+    int32_t front = a.sinks, front_a = a.sinks, front_z = a.sinks, lo = 0, lo_a = 0, lo_z = 0;
+    if constexpr (SCORED) {
+        AttnRow me, ra, rz;
+        if (!PAGED && a.documents) {
+            const uint32_t da = at_document(a, b, at_position(s, ja)), dz = at_document(a, b, at_position(s, jz));
+            ra = at_in_document(a, b, s, at_position(s, ja), da);
+            rz = at_in_document(a, b, s, at_position(s, jz), dz);
+            uint32_t d = da;                                    // may be `none in front`, beyond all numbers
+            if (dz <= a.n_documents)
+                for (uint32_t n = da > a.n_documents ? 0 : da + 1; n <= dz; n++)
+                    if (a.documents[(uint64_t)b * (a.n_documents + 1) + n] <= at_position(s, j)) d = n;
+            me = at_in_document(a, b, s, at_position(s, j), d);
+        } else {
+            const int32_t prefix = a.prefix ? a.prefix[b] : 0;
+            me = at_in_text(a, at_position(s, j), 0, s.keys, prefix);
+            ra = at_in_text(a, at_position(s, ja), 0, s.keys, prefix);
+            rz = at_in_text(a, at_position(s, jz), 0, s.keys, prefix);
+        }
+        const auto one = [](int32_t x) __attribute__((always_inline)) { return (int32_t)__builtin_amdgcn_readfirstlane(x); };      // the same in all lanes
+        limit = me.limit; limit_a = one(ra.limit); limit_z = one(rz.limit);
+        p = me.p; p_a = one(ra.p); p_z = one(rz.p);
+        front = me.front; front_a = one(ra.front); front_z = one(rz.front);
+        if (!PAGED) {
+            lo = me.lo; lo_a = one(ra.lo); lo_z = one(rz.lo);
+        }
+    } else {
+        limit = at_limit(a, s, j); limit_a = at_limit(a, s, ja); limit_z = at_limit(a, s, jz);
+        p = at_position(s, j); p_a = at_position(s, ja); p_z = at_position(s, jz);
+    }
+    const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
 
     v4u q[S::STEPS];
     {
@@ -543,7 +586,8 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         }
     }
     // |scale| log2 e; never 0, so that a hidden key's -inf stays
-    const float c = fmaxf(__builtin_fabsf(a.c), 1e-37f);
+    const bool changed = SCORED && (a.most != 0.0f || a.slopes);
+    const float c = changed ? 1.0f : fmaxf(__builtin_fabsf(a.c), 1e-37f);
 
     // ---- this lane's part of a tile's loads: LDS chunk `slot` belongs to row slot / chunks
     uint32_t l_row[S::LOADS], l_k[S::LOADS], l_v[S::LOADS];
@@ -562,7 +606,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
     const unsigned char* vb = (const unsigned char*)a.v + (g * a.v_h + (PAGED ? 0 : b * a.v_b)) * sizeof(T);
     const uint32_t k_row = (uint32_t)(a.k_t * sizeof(T)), v_row = (uint32_t)(a.v_t * sizeof(T));
     const uint32_t k_page = PAGED ? (uint32_t)(a.k_b * sizeof(T)) : 0;
-    auto start_of = [&](uint32_t n) -> int32_t { return n < w.head ? (int32_t)(n * KT) : w.from + (int32_t)((n - w.head) * KT); };
+    auto start_of = [&](uint32_t n) -> int32_t { return n < w.head ? (SCORED && !PAGED ? w.start : 0) + (int32_t)(n * KT) : w.from + (int32_t)((n - w.head) * KT); };
     // paged: the page of key `lane` of tile n, and its row there
     auto look = [&](uint32_t n, uint32_t& slot) -> int32_t {
         int32_t t = start_of(n) + (int32_t)(lane % KT);
@@ -662,7 +706,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         if (n + 1 < tile1) fetch(n + 1, next);
         if (PAGED && n + 2 < tile1) page = look(n + 2, slot);                   // arrives while this tile is worked on
         const int32_t t0 = start_of(n);
-        if (!busy || t0 > limit_z || (t0 >= a.sinks && p_a - (t0 + KT - 1) >= a.window)) return;
+        if (!busy || t0 > limit_z || (SCORED && !PAGED && t0 + KT <= lo_a) || (t0 >= (SCORED ? front_z : a.sinks) && p_a - (t0 + KT - 1) >= a.window)) return;
 
         constexpr int N = S::STEPS * S::HALVES, AHEAD = N < 4 ? N : 4;
         v16f x[S::HALVES], others[S::HALVES][SUMS];
@@ -694,17 +738,39 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         at_settle(SUMS == 1 ? x[S::HALVES - 1] : others[S::HALVES - 1][SUMS - 1]);
 #pragma unroll
         for (int kk = 0; kk < S::HALVES; kk++) at_join_sums(x[kk], others[kk]);
-        if (t0 + KT - 1 > limit_a || (t0 + KT > a.sinks && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
+        if (changed) {
+            const float most_in = __builtin_fabsf(a.most_in), cc = __builtin_fabsf(a.c);
+            if (a.most != 0.0f) {
+#pragma unroll
+                for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[kk][e] = at_capped<T>(a.most, x[kk][e] * most_in);
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[kk][e] *= cc;
+            }
+            if (a.slopes) {
+                const float far = (float)(p - t0 - 4 * (int32_t)half);          // distance of the tile's first key of this half
+#pragma unroll
+                for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(-slope, __builtin_fabsf(far - (float)(32 * kk + e % 4 + 8 * (e / 4))), x[kk][e]);
+            }
+        }
+        if (t0 + KT - 1 > limit_a || (SCORED && !PAGED && t0 < lo_z) || (t0 + KT > (SCORED ? front_a : a.sinks) && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
             // key t = 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile: p - t < window as t > p - window, which saturates where there is no window
-            int32_t lim = limit - t0 - 4 * (int32_t)half, from = __builtin_elementwise_sub_sat(p - t0 - 4 * (int32_t)half, a.window), sink = a.sinks - t0 - 4 * (int32_t)half;
+            int32_t lim = limit - t0 - 4 * (int32_t)half, from = __builtin_elementwise_sub_sat(p - t0 - 4 * (int32_t)half, a.window), sink = (SCORED ? front : a.sinks) - t0 - 4 * (int32_t)half, low = lo - t0 - 4 * (int32_t)half;
             asm volatile("" : "+v"(lim), "+v"(from), "+v"(sink));               // nothing of this is worth registers outside of masked tiles
+            if (SCORED && !PAGED) asm volatile("" : "+v"(low));
             const uint64_t have = there >> (4 * half);
 #pragma unroll
             for (int kk = 0; kk < S::HALVES; kk++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int32_t t = 32 * kk + e % 4 + 8 * (e / 4);
-                    const bool seen = t <= lim && (t > from || t < sink) && (!PAGED || (have >> t) & 1);
+                    const bool seen = t <= lim && (t > from || t < sink) && (!SCORED || PAGED || t >= low) && (!PAGED || (have >> t) & 1);
                     x[kk][e] = seen ? x[kk][e] : -INFINITY;
                 }
         }
@@ -827,7 +893,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         const uint32_t end = wave * 32 + 32 < rows ? wave * 32 + 32 : rows;
         for (uint32_t rr = wave * 32; rr < end; rr++) {
             float oo[(DT + 63) / 64], mm, ll;
-            at_row_again<T, DT, PAGED, KT>(a, b, g, s, w, tile0, tile1, row0 + rr, oo, mm, ll);
+            at_row_again<T, DT, PAGED, KT, SCORED>(a, b, g, s, w, tile0, tile1, row0 + rr, oo, mm, ll);
             const uint32_t jj = fd_div(row0 + rr, a.group_div), hh = g * a.group + (row0 + rr - jj * a.group);
             const uint64_t part_at = (uint64_t)blockIdx.x * AT_ROWS + rr;
             const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
@@ -886,7 +952,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
 
 // Parts of a row to the row: bound by reading them, 512 bytes a row, piece and 128 columns, and by the launch (encoder: 10 us, ragged chunks: 16 us with their search).
 // blockIdx.y: which AT_JOIN_ROWS of a row tile.  blockIdx.x: paged: KV head, sequence and row tile of it, a row tile having more than one piece; contiguous: as the tiles' blocks
-template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_BLOCK) attention_join_kernel(AttnArgs a, AttnPartial part, uint32_t tile_blocks) {
+template <typename T, int KT, bool PAGED, bool SCORED> __global__ void __launch_bounds__(AT_BLOCK) attention_join_kernel(AttnArgs a, AttnPartial part, uint32_t tile_blocks) {
     __shared__ float factors[AT_JOIN_ROWS * AT_MOST_PIECES];
     uint32_t b, g, tile, piece, pieces;
     uint64_t first, stride;
@@ -895,16 +961,16 @@ template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_B
         // numbered as the items are, with one piece a row tile
         g = blockIdx.x % a.kv_heads;
         uint32_t at = blockIdx.x / a.kv_heads;
-        b = __builtin_amdgcn_readfirstlane(at_locate<KT>(a, 0x7fffffffu, at));
+        b = __builtin_amdgcn_readfirstlane(at_locate<KT, SCORED>(a, 0x7fffffffu, at));
         if (b >= a.seqs) return;
         s = at_seq<true>(a, b);
         tile = __builtin_amdgcn_readfirstlane(at);
-        const uint32_t span = at_span<KT>(a, s), all = __builtin_amdgcn_readfirstlane(at_piece<KT, false>(a));
+        const uint32_t span = at_span<KT, SCORED>(a, b, s), all = __builtin_amdgcn_readfirstlane(at_piece<KT, false, SCORED>(a));
         piece = at_piece_of(all, span);
         pieces = (span + piece - 1) / piece;
         if (pieces == 1) return;
         stride = a.kv_heads;
-        first = (__builtin_amdgcn_readfirstlane(at_before<KT>(a, all, b)) + (uint64_t)(at_row_tiles(a, s) - 1 - tile) * pieces) * stride + g;
+        first = (__builtin_amdgcn_readfirstlane(at_before<KT, SCORED>(a, all, b)) + (uint64_t)(at_row_tiles(a, s) - 1 - tile) * pieces) * stride + g;
     } else {
         stride = (uint64_t)a.seqs * a.kv_heads;
         const uint32_t pair = (uint32_t)(blockIdx.x % stride);
@@ -916,7 +982,7 @@ template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_B
         first = (uint64_t)(part.row_tiles - 1 - tile) * part.pieces * stride + pair;
     }
     const uint32_t all_rows = s.count * a.group, row0 = tile * AT_ROWS, rows = all_rows - row0 < AT_ROWS ? all_rows - row0 : AT_ROWS;
-    const AttnWalk w = at_walk<KT>(a, s, row0, rows);
+    const AttnWalk w = at_walk<KT, SCORED>(a, b, s, row0, rows);
     const uint32_t r0 = blockIdx.y * AT_JOIN_ROWS, r1 = r0 + AT_JOIN_ROWS < rows ? r0 + AT_JOIN_ROWS : rows;
     if (w.tiles <= piece || r0 >= rows) return;
     const uint32_t used = (w.tiles + piece - 1) / piece;
@@ -924,7 +990,7 @@ template <typename T, int KT, bool PAGED> __global__ void __launch_bounds__(AT_B
     at_join<T, false>(a, part, s, b, g, row0, r0, r1, first, stride, used, factors);
 }
 
-template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_device* dev, AttnArgs& a, bool* done) {
+template <typename T, int DT, bool EXACT, bool PAGED, bool SCORED> int at_launch_tile(rt_device* dev, AttnArgs& a, bool* done) {
     typedef AtShape<T, DT> S;
     AttnPartial part = {};
     const bool few = (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
@@ -943,7 +1009,7 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
     } else {
         part.row_tiles = (uint32_t)(((uint64_t)a.tokens * a.group + AT_ROWS - 1) / AT_ROWS);
         uint64_t span = (a.cap + S::KT - 1) / S::KT;
-        if (a.window != AT_FAR) {
+        if (a.window != AT_FAR && !a.documents && !a.prefix) {  // (where texts and prefixes end is known on the device)
             const uint64_t w = ((uint64_t)a.window + AT_ROWS) / S::KT + 2 + ((uint64_t)a.sinks + S::KT - 1) / S::KT;
             span = w < span ? w : span;
         }
@@ -977,7 +1043,7 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
     part.o = part.ml + 2 * row_count;
     a.scores = score_bytes ? part.o + row_count * a.dim : nullptr;
     part.arrivals = dev->arrivals;
-    const auto kernel = few ? attention_tile_kernel<T, DT, EXACT, PAGED, true> : attention_tile_kernel<T, DT, EXACT, PAGED, false>;
+    const auto kernel = few ? attention_tile_kernel<T, DT, EXACT, PAGED, true, SCORED> : attention_tile_kernel<T, DT, EXACT, PAGED, false, SCORED>;
     static_assert(S::LDS <= 160 * 1024 && AT_MOST_PIECES * AT_ROWS * 4 <= S::LDS - 16, "LDS");
     static bool raised[2][16] = {};                             // per GPU; setting it twice does no harm
     if (S::LDS > 64 * 1024 && !(dev->ordinal < 16 && raised[few][dev->ordinal])) {
@@ -987,13 +1053,13 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_tile(rt_devi
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(AT_BLOCK), S::LDS, dev->stream, a, part);
     RT_CHECK_LAUNCH("attention_tile_kernel");
     if (part.split && !few) {
-        hipLaunchKernelGGL((attention_join_kernel<T, S::KT, PAGED>), dim3((unsigned)join_tiles, AT_ROWS / AT_JOIN_ROWS), dim3(AT_BLOCK), 0, dev->stream, a, part, (uint32_t)blocks);
+        hipLaunchKernelGGL((attention_join_kernel<T, S::KT, PAGED, SCORED>), dim3((unsigned)join_tiles, AT_ROWS / AT_JOIN_ROWS), dim3(AT_BLOCK), 0, dev->stream, a, part, (uint32_t)blocks);
         RT_CHECK_LAUNCH("attention_join_kernel");
     }
     return RT_OK;
 }
 
-template <typename T> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool paged, bool* done) {
+template <typename T, bool SCORED> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool paged, bool* done) {
     // rows of whole 16-byte chunks on 16-byte boundaries; 32-bit offsets of the rows of a tile, or in a page, and of pages
     const uint64_t e = sizeof(T), most = 0xffffffffull / e, far = (1ull << 31) / 64 / e;
     const uint64_t strides[] = {a.dim, a.q_b, a.q_h, a.q_t, a.k_b, a.k_h, a.k_t, a.v_b, a.v_h, a.v_t, a.y_b, a.y_h, a.y_t};
@@ -1002,7 +1068,7 @@ template <typename T> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool pag
     for (uint64_t x : strides) fits = fits && x * e % 16 == 0;
     *done = fits;
     if (!fits) return RT_OK;
-#define RT_TILE(DT, EXACT) return paged ? at_launch_tile<T, DT, EXACT, true>(dev, a, done) : at_launch_tile<T, DT, EXACT, false>(dev, a, done)
+#define RT_TILE(DT, EXACT) return paged ? at_launch_tile<T, DT, EXACT, true, SCORED>(dev, a, done) : at_launch_tile<T, DT, EXACT, false, SCORED>(dev, a, done)
     if (a.dim == 64) RT_TILE(64, true);
     if (a.dim == 80) RT_TILE(80, true);
     if (a.dim == 96) RT_TILE(96, true);

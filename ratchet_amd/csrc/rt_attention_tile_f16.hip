@@ -1,5 +1,5 @@
 // The attention kernels of rt_attention_tile.h and rt_attention_weights.h for f16
 #include "rt_attention_weights.h"
 
-int rt_attention_tile_f16(rt_device* dev, AttnArgs& a, bool paged, bool* done) { return at_dispatch_tile<half_t>(dev, a, paged, done); }
+int rt_attention_tile_f16(rt_device* dev, AttnArgs& a, bool paged, bool* done) { return at_dispatch_tile<half_t, false>(dev, a, paged, done); }
 int rt_attention_weights_f16(rt_device* dev, const AttnArgs& a, const float* weights, float* out) { return aw_dispatch<half_t>(dev, a, weights, out); }

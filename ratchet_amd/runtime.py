@@ -206,6 +206,33 @@ def _counts(**counts):
             raise ValueError(f"{name} is {n}")
 
 
+def _scores(heads, batch, cap, slopes, documents, prefix):
+    if not (slopes is None or (slopes.dt == _lib.F32 and slopes.shape == (heads,))):
+        raise ValueError("slopes has to be F32 [heads]")
+    texts = 0
+    if documents is not None:
+        if not (documents.dt == _lib.I32 and len(documents.shape) == 2 and documents.shape[0] == batch and documents.shape[1] > 1):
+            raise ValueError("documents has to be I32 [B, n + 1]")
+        texts = documents.shape[1] - 1
+    if not (prefix is None or (prefix.dt == _lib.I32 and prefix.shape == ((batch, texts) if texts else (batch,)))):
+        raise ValueError("prefix has to be I32 [B], or [B, n] with n documents")
+    return ctypes.byref(_lib.Scores(cap, *(x.ptr.value if x is not None else None for x in (slopes, documents)), texts, prefix.ptr.value if prefix is not None else None))
+
+
+def _table_dim(table):
+    if not (table.dt == _lib.U32 and len(table.shape) == 2 and table.shape[1] == 2):
+        raise ValueError("the table has to be U32 [dim / 2, 2], what rope_table gives")
+    return 2 * table.shape[0]
+
+
+def rope_divisors(dim, base, scale, trained, low=1.0, high=32.0):
+    """Divisors that scale a rotary table for a context `scale` times the `trained` one: frequencies that turn fewer than `low` times in the trained context are
+    divided by `scale`, those that turn more than `high` times by 1, those between by a mean of the two (1 / divisor is linear in the turns)."""
+    turns = trained * base ** (-2.0 * np.arange(dim // 2) / dim) / (2 * np.pi)
+    share = np.clip((turns - low) / (high - low), 0, 1)
+    return 1.0 / (share + (1 - share) / scale)
+
+
 class Device:
     """One GPU: its storage pool, and the ops, which are enqueued on a stream of the device's own and return at once.  No other
     stream is ordered with that one, torch's current stream included: who fills a buffer or reads a result through torch (or
@@ -431,10 +458,12 @@ class Device:
 
     # ---- attention, the paged KV cache
     def attention(self, q, k, v, lens=None, causal=True, window=0, sinks=0, scale=None, q_strides=None, k_strides=None, v_strides=None, out=None, out_strides=None,
-                  lse=None):
+                  lse=None, cap=0.0, slopes=None, documents=None, prefix=None):
         """softmax(scale q k^T over the visible keys) v: q [B, heads, Sq, D], k and v [B, kv_heads, Sk, D]; the strides (elements, one for each extent) say
         where they lie in memory, out's too.  lens: I32 [B], the keys of each entry; the last query is at the last key.  window: a query
-        sees that many last keys and the first `sinks`; scale: 1 / sqrt(D) unless given; lse: F32 [B, heads, Sq] for the log of each row's sum."""
+        sees that many last keys and the first `sinks`; scale: 1 / sqrt(D) unless given; lse: F32 [B, heads, Sq] for the log of each row's sum.
+        cap: scores become cap * tanh(score / cap); slopes: F32 [heads], scores lose slope * distance; documents: I32 [B, n + 1], where the n texts of each entry begin
+        (and the last ends): a query sees its own; prefix: I32 [B] ([B, n] with documents), so many first keys (of each text) that all its queries see."""
         if not (len(q.shape) == 4 and len(k.shape) == 4 and k.shape == v.shape and q.dt == k.dt == v.dt):
             raise ValueError(f"attention of {q.shape}, {k.shape}, {v.shape}")
         if not (lens is None or (lens.dt == _lib.I32 and lens.shape == (q.shape[0],))):
@@ -445,9 +474,56 @@ class Device:
             raise ValueError("out or lse does not fit")
         if not (out_strides is None or out.shape == q.shape):
             raise ValueError("out with strides has the shape of q")
-        check(self.lib.rt_attention(self.handle, q.dt, q.ptr, buffer_shape4(q.shape), _strided(q, q_strides, 4), k.ptr, _strided(k, k_strides, 4), v.ptr, _strided(v, v_strides, 4),
-                                    buffer_shape4(k.shape), lens.ptr if lens is not None else None, out.ptr, _strided(out, out_strides, 4), lse.ptr if lse is not None else None,
-                                    q.shape[3] ** -0.5 if scale is None else scale, 1 if causal else 0, window, sinks))
+        args = (self.handle, q.dt, q.ptr, buffer_shape4(q.shape), _strided(q, q_strides, 4), k.ptr, _strided(k, k_strides, 4), v.ptr, _strided(v, v_strides, 4),
+                buffer_shape4(k.shape), lens.ptr if lens is not None else None, out.ptr, _strided(out, out_strides, 4), lse.ptr if lse is not None else None,
+                q.shape[3] ** -0.5 if scale is None else scale, 1 if causal else 0, window, sinks)
+        if not cap and slopes is None and documents is None and prefix is None:
+            check(self.lib.rt_attention(*args))
+        else:
+            check(self.lib.rt_attention_scored(*args, _scores(q.shape[1], q.shape[0], cap, slopes, documents, prefix)))
+        return out
+
+    def rope_table(self, dim, base=10000.0, divisors=None):
+        """What rope_tokens needs of its frequencies base^(-2i / dim) / divisors[i], i < dim / 2: the 64-bit fractions of a turn, as U32 [dim / 2, 2].
+        divisors: None, a number (positions scaled down), or dim / 2 numbers (rope_divisors, or a model's own)."""
+        _counts(dim=dim)
+        if divisors is not None:
+            divisors = np.ascontiguousarray(np.broadcast_to(np.asarray(divisors, np.float64), (dim // 2,)))
+        turns = np.zeros(dim // 2, np.uint64)
+        check(self.lib.rt_rope_turns(dim, base, None if divisors is None else divisors.ctypes.data, turns.ctypes.data))
+        return self.upload(turns.view(np.uint32).reshape(-1, 2))
+
+    def rope_tokens(self, x, positions, table, factor=1.0, interleaved=False, strides=None, out=None, out_strides=None):
+        """Rotary positions: row t of x [tokens, heads, D] turned to positions[t] (I32 [tokens]), pairs of halves, or of neighbours where interleaved, over
+        the columns that `table` (rope_table) has frequencies for; the others pass through.  factor: what the turned columns are multiplied by.
+        strides: elements from token to token and from head to head.  out may be x, with the same strides."""
+        if len(x.shape) != 3:
+            raise ValueError(f"rope_tokens of {x.shape}")
+        if not (positions.dt == _lib.I32 and positions.shape == x.shape[:1]):
+            raise ValueError("positions has to be I32 [tokens]")
+        dim = _table_dim(table)
+        out = out or Buffer(self, x.shape, x.dt)
+        if not (out.dt == x.dt and out.shape == x.shape):
+            raise ValueError("out does not fit")
+        check(self.lib.rt_rope_tokens(self.handle, x.dt, x.ptr, _strided(x, strides, 2), out.ptr, _strided(out, out_strides, 2), *x.shape, positions.ptr, table.ptr, dim, factor,
+                                      1 if interleaved else 0))
+        return out
+
+    def paged_rope_append(self, cache, starts, q, k, v, table, factor=1.0, interleaved=False, q_strides=None, k_strides=None, v_strides=None, out=None, out_strides=None):
+        """rope_tokens of the new tokens q [tokens, heads, D] into out (returned; it may be q, with the same strides) and of k into the cache, and v into the
+        cache as it is, as paged_append puts them there, at the positions that the cache gives them: one launch."""
+        if not (k.shape == v.shape and k.shape[1:] == (cache.kv_heads, cache.head_dim) and k.dt == v.dt == cache.dt):
+            raise ValueError(f"{k.shape} and {v.shape} do not fit the cache")
+        if not (len(q.shape) == 3 and q.shape[0] == k.shape[0] and q.shape[2] == cache.head_dim and q.dt == cache.dt):
+            raise ValueError(f"{q.shape} does not fit the cache")
+        if not (starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,)):
+            raise ValueError("starts has to be I32 [seqs + 1]")
+        dim = _table_dim(table)
+        out = out or Buffer(self, q.shape, q.dt)
+        if not (out.dt == q.dt and out.shape == q.shape):
+            raise ValueError("out does not fit")
+        check(self.lib.rt_paged_rope_append(self.handle, q.dt, cache.ref, starts.ptr, q.shape[0], q.ptr, _strided(q, q_strides, 2), q.shape[1], out.ptr, _strided(out, out_strides, 2),
+                                            k.ptr, _strided(k, k_strides, 2), v.ptr, _strided(v, v_strides, 2), table.ptr, dim, factor, 1 if interleaved else 0))
         return out
 
     def paged_cache(self, k_pages, v_pages, table, lens):
@@ -463,9 +539,11 @@ class Device:
         check(self.lib.rt_paged_append(self.handle, _DT_BYTES[cache.dt], cache.ref, starts.ptr, k.shape[0], k.ptr, _strided(k, k_strides, 2), v.ptr, _strided(v, v_strides, 2)))
         return cache
 
-    def paged_attention(self, q, cache, starts, window=0, sinks=0, scale=None, q_strides=None, out=None, lse=None, weights=None, weights_out=None):
+    def paged_attention(self, q, cache, starts, window=0, sinks=0, scale=None, q_strides=None, out=None, lse=None, weights=None, weights_out=None,
+                        cap=0.0, slopes=None, prefix=None):
         """Causal attention of the new tokens q [tokens, heads, head_dim] (starts as in paged_append, whose rows are in the cache already).
-        weights: F32 cache.weights_shape, the attention weight each cached token has received, updated in place or into weights_out."""
+        weights: F32 cache.weights_shape, the attention weight each cached token has received, updated in place or into weights_out.
+        cap, slopes and prefix (I32 [seqs]) as in attention; not with weights."""
         if not (len(q.shape) == 3 and q.shape[2] == cache.head_dim and q.dt == cache.dt):
             raise ValueError(f"{q.shape} does not fit the cache")
         if not (starts.dt == _lib.I32 and starts.shape == (cache.seqs + 1,)):
@@ -480,6 +558,13 @@ class Device:
             weights_out = weights if weights_out is None else weights_out
             if not (weights.dt == weights_out.dt == _lib.F32 and weights.shape == weights_out.shape == cache.weights_shape):
                 raise ValueError(f"weights have to be F32 {cache.weights_shape}")
+        if cap or slopes is not None or prefix is not None:
+            if weights is not None:
+                raise ValueError("weights of changed scores are not to be had")
+            check(self.lib.rt_paged_attention_scored(self.handle, q.dt, q.ptr, _strided(q, q_strides, 2), q.shape[0], q.shape[1], cache.ref, starts.ptr, out.ptr,
+                                                     lse.ptr if lse is not None else None, q.shape[2] ** -0.5 if scale is None else scale, window, sinks,
+                                                     _scores(q.shape[1], cache.seqs, cap, slopes, None, prefix)))
+            return out
         check(self.lib.rt_paged_attention(self.handle, q.dt, q.ptr, _strided(q, q_strides, 2), q.shape[0], q.shape[1], cache.ref, starts.ptr, out.ptr,
                                           lse.ptr if lse is not None else None, weights.ptr if weights is not None else None,
                                           weights_out.ptr if weights is not None else None, q.shape[2] ** -0.5 if scale is None else scale, window, sinks))
@@ -497,3 +582,20 @@ class Device:
             raise ValueError(f"weights have to be F32 {cache.weights_shape}")
         check(self.lib.rt_paged_evict(self.handle, _DT_BYTES[cache.dt], cache.ref, weights.ptr, keep, first, recent, to.ptr, lens_out.ptr, weights_out.ptr))
         return cache if to is cache.table and lens_out is cache.lens else PagedCache(cache.k_pages, cache.v_pages, to, lens_out)
+
+    # ---- sampling
+    def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, row_stride=None, out=None, probs=None):
+        """The next token of each row of logits [rows, vocab], I32 [rows], from uniform F32 [rows] in [0, 1): the first index at which the cumulative weight of the tokens
+        that stay exceeds uniform times their whole weight.  temperature F32, top_k I32, top_p F32 and min_p F32, each [rows], a number for each
+        row, or None; a temperature of 0 takes the largest logit.  probs: F32 [rows] for the tokens' shares.  row_stride: elements from row to row."""
+        if len(logits.shape) != 2:
+            raise ValueError(f"sample of {logits.shape}")
+        rows, vocab = logits.shape
+        for name, x, dt in (("uniform", uniform, _lib.F32), ("temperature", temperature, _lib.F32), ("top_k", top_k, _lib.I32), ("top_p", top_p, _lib.F32), ("min_p", min_p, _lib.F32),
+                            ("out", out, _lib.I32), ("probs", probs, _lib.F32)):
+            if not (x is None or (x.dt == dt and x.shape == (rows,))):
+                raise ValueError(f"{name} has to be {'F32' if dt == _lib.F32 else 'I32'} [rows]")
+        stride = vocab if row_stride is None else _strided(logits, (row_stride, 1), 2)[0]
+        out = out or Buffer(self, (rows,), _lib.I32)
+        check(self.lib.rt_sample(self.handle, logits.dt, logits.ptr, stride, rows, vocab, *(x.ptr if x is not None else None for x in (temperature, top_k, top_p, min_p, uniform, out, probs))))
+        return out
