@@ -6,8 +6,13 @@
 // All three filters keep a front of the same order, larger logits first and of equal ones the lower index, so what they keep is a cut in it: a logit and
 // the index up to which its equals stay.  Sums of fixed-point numbers are the same in any order and on any split, so atomics and waves need no order.
 //
-// A block to a row, a sixteenth of the row to a wave, the logits in registers where they fit.  A cut is found by a histogram of the weights (or counts)
-// over 2048 equal steps of the logit, then by comparing the few members of the step it lies in; a step with too many members is cut into 2048 again.
+// A block to a row, a sixteenth of the row to a wave; the row is read again for every walk over it, from the L2.  NaN fails every comparison here, and so is never kept.
+//   temperature alone: the waves' sums of weights, then the one wave's share that holds the border is dealt out to all threads again
+//   top-k: the kth largest of the threads' maxima bounds the kth largest logit; what reaches it is listed, and a list of up to 1024 is sorted, cut and drawn from
+//          by itself
+//   top-p: a histogram of the weights over 2048 equal steps of the logit names the step the cut lies in; its members are listed and sorted for
+//          the cut.  A step of too many members is cut into 2048 again, down to equals
+// What bounds it: vector instructions, some 25 for a weight in 64 bits, twice for each logit where many are kept, and the chain of barriers between the phases.
 #include <math.h>
 
 #include "rt_arith.h"
@@ -16,8 +21,13 @@
 namespace {
 
 constexpr int BLOCK = 1024, WAVES = BLOCK / 64;
-constexpr uint32_t BINS = 2048, LIST = 1024, NO_CUT = 0;       // NO_CUT: a key below all keys
+constexpr uint32_t BINS = 2048, LIST = 1024;
 constexpr uint32_t MOST_VOCAB = 1u << 24;
+
+// 2^f = 1 + f q(f) for |f| <= 1/2: q interpolates at Chebyshev's points, the result is 4e-14 off at most
+constexpr int TERMS = 9;
+constexpr double EXP2[TERMS] = {0x1.62e42fefa39efp-1, 0x1.ebfbdff823cedp-3, 0x1.c6b08d7047e8bp-5, 0x1.3b2ab7181b757p-7, 0x1.5d87fe86f8348p-10, 0x1.4308ac85aa619p-13,
+                                0x1.ffcb952673288p-17, 0x1.63d136368c2cep-20, 0x1.b63871c687389p-24};
 
 struct SampleArgs {
     const void* x;
@@ -28,6 +38,7 @@ struct SampleArgs {
     int32_t* tokens;
     float* probs;
     double magic;                                  // 2^(52 - scale): added to a weight, it leaves its fixed-point form in the low bits
+    double exp2[TERMS];                            // here they are one load; as constants in the code, two instructions each
 };
 
 // an order that unsigned integers have; -0 as +0
@@ -35,46 +46,71 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+// a logit and its index as one number: what comes first is larger
+__device__ __forceinline__ uint64_t place_of(float x, int32_t i) { return (uint64_t)key_of(x) << 32 | (0xffffffffu - (uint32_t)i); }
+__device__ __forceinline__ int32_t index_of(uint64_t place) { return (int32_t)(0xffffffffu - (uint32_t)place); }
 
 struct Shared {
-    uint64_t hist[BINS];
-    uint64_t list_key[LIST];                       // key, then the index from the top, so that what comes first is larger
-    uint64_t list_w[LIST];
-    uint64_t wave_sum[WAVES];
-    uint32_t wave_a[WAVES], wave_b[WAVES];
-    uint64_t before;
-    uint32_t bin, count, low, high;
-    uint64_t cut;
-    uint32_t found;
+    uint64_t hist[BINS];                           // or what a list is sorted in, and the weights of a sorted one
+    uint64_t places[LIST];
+    uint64_t sums[WAVES];
+    uint64_t before, cut, total;                   // (cut: a place)
+    uint32_t bin, n, found;
 };
 
-template <typename T> __device__ __forceinline__ T wave_sum(T x) {
-#pragma unroll
-    for (int i = 32; i; i >>= 1) x += __shfl_xor(x, i);
+// Sums over lanes by data moves between them that need no LDS: rows of 16 lanes, then the last lane of a row to the next ones
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, true);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t moved(uint64_t x) {
+    return (uint64_t)moved<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)x);
+}
+__device__ __forceinline__ uint64_t row_upto(uint64_t x) {      // of this lane and those below in its row
+    x += moved<0x111, 0xf>(x);
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
     return x;
 }
-template <typename T> __device__ __forceinline__ T wave_upto(T x) {              // of this lane and those below
-    const int lane = (int)__lane_id();
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) {
-        const T y = __shfl_up(x, i);
-        if (lane >= i) x += y;
-    }
+__device__ __forceinline__ uint64_t wave_upto(uint64_t x) {     // of this lane and those below
+    x = row_upto(x);
+    x += moved<0x142, 0xa>(x);
+    x += moved<0x143, 0xc>(x);
     return x;
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t x, uint32_t lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), (int)lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, (int)lane);
+}
+// the largest of the lanes, in all of them
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    uint32_t y;
+    y = moved<0x111, 0xf>(x), x = y > x ? y : x;
+    y = moved<0x112, 0xf>(x), x = y > x ? y : x;
+    y = moved<0x114, 0xf>(x), x = y > x ? y : x;
+    y = moved<0x118, 0xf>(x), x = y > x ? y : x;
+    y = moved<0x142, 0xa>(x), x = y > x ? y : x;
+    y = moved<0x143, 0xc>(x), x = y > x ? y : x;
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// ITS: vectors that a lane holds; 0: the row is read again for every walk over it
-template <typename T, int ITS> struct Row {
+// What is kept: logits above x, and those that equal it up to index i
+struct Cut {
+    float x;
+    int32_t i;
+    __device__ __forceinline__ bool keeps(float v, int32_t at) const { return v > x || (v == x && at <= i); }
+};
+__device__ __forceinline__ Cut cut_at(uint64_t place) { return Cut{of_key((uint32_t)(place >> 32)), index_of(place)}; }
+
+template <typename T> struct Row {
     static constexpr int VE = 16 / sizeof(T);
     const SampleArgs& a;
     Shared& s;
     const v4u* base;                               // the aligned vectors that cover the row
     uint32_t shift, covered, vectors, per_wave, its, v0, v1;   // elements in front of the row; this wave's vectors
     uint32_t lane, wave, tid;
-    bool infinite;                                 // the largest is +inf: those are 0, the others -inf
     float max;
     double step;                                   // log2(e) / temperature
-    float r[ITS ? ITS * VE : 1];
 
     __device__ __forceinline__ Row(const SampleArgs& a, Shared& s, uint32_t row) : a(a), s(s) {
         const uintptr_t at = (uintptr_t)((const T*)a.x + row * a.stride);
@@ -90,147 +126,204 @@ template <typename T, int ITS> struct Row {
         v0 = wave * per_wave;
         v0 = v0 < vectors ? v0 : vectors;
         v1 = v0 + per_wave < vectors ? v0 + per_wave : vectors;
-        infinite = false;
         max = 0.0f;
         step = 0.0;
     }
-    __device__ __forceinline__ float clean(float x) const {                    // NaN ranks with -inf
-        x = x == x ? x : -INFINITY;
-        return infinite ? (x == INFINITY ? 0.0f : -INFINITY) : x;
-    }
-    __device__ __forceinline__ void vector(uint32_t it, float* to) const {
+    // vector `it` of this lane; elements that are none of the row's are NaN
+    __device__ __forceinline__ v4u vector(uint32_t it) const {
         const uint32_t v = v0 + it * 64 + lane;
         Vec16<T> x;
-        if (v < v1) x.u = base[v];
+        x.u = v4u{~0u, ~0u, ~0u, ~0u};
+        if (v < v1) {
+            x.u = base[v];
+            if (v == 0 || v == vectors - 1) {
+                Vec16<T> none;
+                none.u = v4u{~0u, ~0u, ~0u, ~0u};
 #pragma unroll
-        for (int e = 0; e < VE; e++) {
-            const uint32_t c = v * VE + e;
-            to[e] = v < v1 && c >= shift && c < covered ? clean(Ar<T>::widen(x.e[e])) : -INFINITY;
-        }
-    }
-    __device__ __forceinline__ void load() {
-        if constexpr (ITS != 0) {
-#pragma unroll
-            for (int it = 0; it < ITS; it++)
-                if ((uint32_t)it < its) vector(it, r + it * VE);
-        }
-    }
-    // f(logit, index) for this thread's share; elements beyond the row are -inf
-    template <typename F> __device__ __forceinline__ void each(F f) const {
-        if constexpr (ITS != 0) {
-#pragma unroll
-            for (int it = 0; it < ITS; it++)
-                if ((uint32_t)it < its)
-#pragma unroll
-                    for (int e = 0; e < VE; e++) f(r[it * VE + e], (v0 + it * 64 + lane) * VE + e - shift);
-        } else {
-            for (uint32_t it = 0; it < its; it++) {
-                float x[VE];
-                vector(it, x);
-#pragma unroll
-                for (int e = 0; e < VE; e++) f(x[e], (v0 + it * 64 + lane) * VE + e - shift);
+                for (int e = 0; e < VE; e++) {
+                    const uint32_t c = v * VE + e;
+                    if (c < shift || c >= covered) x.e[e] = none.e[e];
+                }
             }
+        }
+        return x.u;
+    }
+    // f(logit, index) for this thread's share.  Loops stay loops: straight code, which a wave runs once, would wait for its own instructions
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        v4u next = vector(0);
+#pragma unroll 1
+        for (uint32_t it = 0; it < its; it++) {
+            Vec16<T> x;
+            x.u = next;
+            next = vector(it + 1);                              // beyond the last: nothing is loaded
+            const int32_t i = (int32_t)((v0 + it * 64 + lane) * VE) - (int32_t)shift;
+#pragma unroll
+            for (int e = 0; e < VE; e++) f(Ar<T>::widen(x.e[e]), i + e);
         }
     }
     __device__ __forceinline__ double weight(float x) const {
-        // 2^y = 2^n (1 + f q(f)), n the nearest integer: q interpolates at Chebyshev's points, 4e-14 off at most
         const double y = fmax(((double)x - (double)max) * step, -100.0), n = rint(y), f = y - n;
-        double q = 0x1.b63871c687389p-24;
-        q = __builtin_fma(q, f, 0x1.63d136368c2cep-20);
-        q = __builtin_fma(q, f, 0x1.ffcb952673288p-17);
-        q = __builtin_fma(q, f, 0x1.4308ac85aa619p-13);
-        q = __builtin_fma(q, f, 0x1.5d87fe86f8348p-10);
-        q = __builtin_fma(q, f, 0x1.3b2ab7181b757p-7);
-        q = __builtin_fma(q, f, 0x1.c6b08d7047e8bp-5);
-        q = __builtin_fma(q, f, 0x1.ebfbdff823cedp-3);
-        q = __builtin_fma(q, f, 0x1.62e42fefa39efp-1);
+        double q = a.exp2[TERMS - 1];
+#pragma unroll
+        for (int t = TERMS - 2; t >= 0; t--) q = __builtin_fma(q, f, a.exp2[t]);
         return ldexp(__builtin_fma(q, f, 1.0), (int)n);
     }
     __device__ __forceinline__ uint64_t fixed(double w) const { return (uint64_t)__double_as_longlong(w + a.magic) & ((1ull << 52) - 1); }
 
-    // the sum over the block of what each thread brings
-    __device__ __forceinline__ uint64_t block_sum(uint64_t x) {
-        x = wave_sum(x);
-        if (lane == 0) s.wave_sum[wave] = x;
+    // the sum over the block of what each thread brings; upto: of this thread and those below
+    __device__ __forceinline__ uint64_t block_sum(uint64_t x, uint64_t* upto = nullptr) {
+        const uint64_t mine = wave_upto(x);
         __syncthreads();
-        const uint64_t all = wave_sum(lane < WAVES ? s.wave_sum[lane] : 0);
+        if (lane == 63) s.sums[wave] = mine;
         __syncthreads();
-        return all;
+        const uint64_t waves = row_upto(lane < WAVES ? s.sums[lane] : 0);
+        if (upto) *upto = mine + (wave ? lane_of(waves, wave - 1) : 0);
+        return lane_of(waves, WAVES - 1);
     }
-    __device__ __forceinline__ float block_max(float x) {
-#pragma unroll
-        for (int i = 32; i; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
-        if (lane == 0) s.wave_a[wave] = __float_as_uint(x);
+    // the largest two numbers of the block, each among the threads' own
+    __device__ __forceinline__ void block_max(uint32_t& x, uint32_t& y) {
+        x = wave_max(x);
+        y = wave_max(y);
         __syncthreads();
-        x = __uint_as_float(s.wave_a[lane % WAVES]);
-#pragma unroll
-        for (int i = WAVES / 2; i; i >>= 1) x = fmaxf(x, __shfl_xor(x, i));
+        if (lane == 0) s.sums[wave] = (uint64_t)x << 32 | y;
+        __syncthreads();
+        const uint64_t both = s.sums[lane % WAVES];
+        x = wave_max((uint32_t)(both >> 32));
+        y = wave_max((uint32_t)both);
+    }
+    // the lowest and highest key of the block; a thread without one brings low above high
+    __device__ __forceinline__ void key_range(uint32_t& low, uint32_t& high) {
+        low = ~low;
+        block_max(low, high);
+        low = ~low;
+    }
+    // below `whole` and, taken into [0, 1), uniform of it: a sum of whole numbers exceeds u * whole if it exceeds its whole part
+    __device__ __forceinline__ static uint64_t part_of(float uniform, uint64_t whole) {
+        const double u = uniform >= 0.0f ? (uniform < 1.0f ? uniform : 1.0f - 0x1p-24f) : 0.0f;
+        return (uint64_t)(u * (double)whole);
+    }
+
+    // The n numbers of the threads below n, none of them 0, in descending order: a bitonic sort, between lanes where partners are in one wave.  Uses the first half of s.hist.
+    // Few are counted, several threads to a number, which takes fewer barriers and moves: 60 numbers 1.3 us, sorted 2.6.
+    __device__ __forceinline__ uint64_t sorted(uint64_t x, uint32_t n) {
+        uint32_t pad = 64;
+        while (pad < n) pad <<= 1;
+        if (pad <= 256) {
+            uint64_t* const to = s.hist + 256;
+            uint32_t* const rank = (uint32_t*)(s.hist + 512);
+            __syncthreads();
+            if (tid < pad) {
+                s.hist[tid] = x;
+                to[tid] = 0;
+                rank[tid] = 0;
+            }
+            __syncthreads();
+            const uint32_t t = tid & (pad - 1);
+            const uint64_t me = s.hist[t];
+            uint32_t ahead = 0;
+            for (uint32_t j = tid / pad; j < n; j += BLOCK / pad) ahead += s.hist[j] > me;
+            if (t < n) atomicAdd(&rank[t], ahead);
+            __syncthreads();
+            if (tid < n) to[rank[tid]] = x;
+            __syncthreads();
+            x = tid < pad ? to[tid] : 0;
+            __syncthreads();
+            return x;
+        }
+#pragma unroll 1
+        for (uint32_t size = 2; size <= pad; size <<= 1)
+#pragma unroll 1
+            for (uint32_t stride = size / 2; stride; stride >>= 1) {
+                uint64_t other = 0;
+                if (stride >= 64) {
+                    __syncthreads();
+                    s.hist[tid] = x;
+                    __syncthreads();
+                    other = s.hist[tid ^ stride];
+                } else if (wave * 64 < pad) {                   // (the others' numbers are 0, and stay there)
+                    other = __shfl_xor(x, (int)stride);
+                } else {
+                    continue;
+                }
+                const bool larger = ((tid & stride) == 0) == ((tid & size) == 0);
+                x = (x > other) == larger ? x : other;
+            }
         __syncthreads();
         return x;
     }
 
-    // The first index at which the sum of metric(logit, index), by index, exceeds `target`, which is below `total`, the sum of them all; before: the sum in front of it.
-    // First among the waves' shares, whose sums each thread brings its part of, then among the threads, to which the one share is dealt out again.
-    template <typename F> __device__ __forceinline__ uint32_t search(uint64_t mine, bool fraction, float uniform, uint64_t target, F metric, uint64_t& total) {
-        const uint64_t share = wave_sum(mine);
-        if (lane == 0) s.wave_sum[wave] = share;
+    // The first index at which the sum of metric(logit, index), by index, exceeds `target`, or where `fraction` that part of the whole sum, `total`; mine: what this
+    // thread's share adds to it.  First among the waves' shares, then among the threads, to which the one share is dealt out again.
+    template <typename F> __device__ __forceinline__ int32_t search(uint64_t mine, bool fraction, float uniform, uint64_t target, F metric, uint64_t& total) {
+        const uint64_t share = wave_upto(mine);
         __syncthreads();
-        uint64_t upto = wave_upto(lane < WAVES ? s.wave_sum[lane] : 0);
-        total = __shfl(upto, WAVES - 1);
-        if (fraction) {
-            const double u = uniform >= 0.0f ? (uniform < 1.0f ? uniform : 1.0f - 0x1p-24f) : 0.0f;
-            target = (uint64_t)(u * (double)total);             // a sum exceeds u * total if it exceeds its whole part
-        }
-        const uint64_t ahead = __ballot(lane < WAVES && upto <= target);
-        uint32_t w = (uint32_t)__popcll(ahead);
+        if (lane == 63) s.sums[wave] = share;
+        if (tid == 0) s.found = a.vocab - 1;
+        __syncthreads();
+        uint64_t upto = row_upto(lane < WAVES ? s.sums[lane] : 0);
+        total = lane_of(upto, WAVES - 1);
+        if (fraction) target = part_of(uniform, total);
+        uint32_t w = (uint32_t)__popcll(__ballot(lane < WAVES && upto <= target));
         w = w < WAVES ? w : WAVES - 1;
-        uint64_t before = w ? __shfl(upto, (int)w - 1) : 0;
+        w = __builtin_amdgcn_readfirstlane(w);
+        uint64_t before = w ? lane_of(upto, w - 1) : 0;
         uint32_t c0 = w * per_wave * VE, c1 = (w + 1) * per_wave * VE;
         c0 = c0 > shift ? c0 : shift;
         c1 = c1 < covered ? c1 : covered;
         c1 = c1 > c0 ? c1 : c0;
-        const uint32_t each_has = (c1 - c0 + BLOCK - 1) / BLOCK, c = c0 + tid * each_has;
+        const uint32_t some = c0 < c1 ? c0 : shift;             // an element that is there
         const T* x = (const T*)base;
+        const uint32_t rounds = (c1 - c0 + BLOCK - 1) / BLOCK, first = c0 + wave * rounds * 64 + lane;         // of 64 neighbours to a wave
         uint64_t sum = 0;
-        for (uint32_t i = 0; i < each_has; i++)
-            if (c + i < c1) sum += metric(clean(Ar<T>::widen(x[c + i])), c + i - shift);
-        upto = wave_upto(sum);
+        auto weigh = [&](uint32_t round) -> uint64_t {
+            const uint32_t c = first + round * 64;
+            const T v = x[c < c1 ? c : some];
+            return c < c1 ? metric(Ar<T>::widen(v), (int32_t)(c - shift)) : 0;
+        };
+#pragma unroll 1
+        for (uint32_t n = 0; n < rounds; n++) sum += weigh(n);
+        const uint64_t sub = wave_upto(sum);
         __syncthreads();
-        if (lane == 63) s.wave_sum[wave] = upto;
-        if (tid == 0) s.found = a.vocab - 1;
+        if (lane == 63) s.sums[wave] = sub;
         __syncthreads();
-        const uint64_t waves_before = wave_sum(lane < wave ? s.wave_sum[lane] : 0);
-        before += waves_before + upto - sum;
-        if (before <= target && before + sum > target) {
-            for (uint32_t i = 0; i < each_has; i++) {
-                if (c + i >= c1) break;
-                before += metric(clean(Ar<T>::widen(x[c + i])), c + i - shift);
-                if (before > target) {
-                    s.found = c + i - shift;
-                    break;
-                }
+        upto = before + row_upto(lane < WAVES ? s.sums[lane] : 0);
+        w = (uint32_t)__popcll(__ballot(lane < WAVES && upto <= target));
+        w = __builtin_amdgcn_readfirstlane(w < WAVES ? w : WAVES - 1);
+        if (wave == w) {
+            before = w ? lane_of(upto, w - 1) : before;
+#pragma unroll 1
+            for (uint32_t n = 0; n < rounds; n++) {
+                const uint64_t here = before + wave_upto(weigh(n)), beyond = __ballot(here > target);
+                before = lane_of(here, 63);
+                if (!beyond) continue;
+                if (lane == (uint32_t)__builtin_ctzll(beyond)) s.found = first + n * 64 - shift;
+                break;
             }
         }
         __syncthreads();
-        const uint32_t found = s.found;
-        __syncthreads();
-        return found;
+        return (int32_t)s.found;
     }
 
-    // Into s.bin and s.before: the bin of the histogram at which the sum from the top reaches `want`, and the sum in front of it.  s.bin is BINS if none does.
+    __device__ __forceinline__ void clear() {
+        __syncthreads();
+        for (uint32_t i = tid; i < BINS; i += BLOCK) s.hist[i] = 0;
+        if (tid == 0) {
+            s.n = 0;
+            s.bin = BINS;
+        }
+        __syncthreads();
+    }
+    // Into s.bin and s.before: the bin of the histogram at which the sum from the top, and offset, reaches `want`, and the sum in front of it.  s.bin stays BINS if none does.
     __device__ __forceinline__ void find_bin(uint64_t offset, double want) {
         __syncthreads();
-        if (tid == 0) s.bin = BINS;
-        uint64_t h[BINS / BLOCK], sum = 0;
+        uint64_t h[BINS / BLOCK], sum = 0, upto;
 #pragma unroll
         for (uint32_t i = 0; i < BINS / BLOCK; i++) {
             h[i] = s.hist[tid * (BINS / BLOCK) + i];
             sum += h[i];
         }
-        uint64_t upto = wave_upto(sum);
-        if (lane == 63) s.wave_sum[wave] = upto;
-        __syncthreads();
-        uint64_t before = offset + wave_sum(lane < wave ? s.wave_sum[lane] : 0) + upto - sum;
+        block_sum(sum, &upto);
+        uint64_t before = offset + upto - sum;
 #pragma unroll
         for (uint32_t i = 0; i < BINS / BLOCK; i++) {
             if ((double)before < want && !((double)(before + h[i]) < want)) {
@@ -241,73 +334,54 @@ template <typename T, int ITS> struct Row {
         }
         __syncthreads();
     }
-    __device__ __forceinline__ void clear() {
-        __syncthreads();
-        for (uint32_t i = tid; i < BINS; i += BLOCK) s.hist[i] = 0;
-        if (tid == 0) {
-            s.count = 0;
-            s.low = 0xffffffffu;
-            s.high = 0;
-        }
-        __syncthreads();
+    __device__ __forceinline__ void list(float x, int32_t i) {
+        const uint32_t at = atomicAdd(&s.n, 1u);
+        if (at < LIST) s.places[at] = place_of(x, i);
     }
 
-    // The cut at which the sum of the metric, in descending order, reaches `want`: the key of a logit and, from the top, the last index of its equals
-    // that stays, as one number; what is kept is >= it.  in(x, i): takes part; floor: what lies below need not; metric(x): its weight.
-    template <typename In, typename M> __device__ uint64_t select(double want, float floor, In in, M metric) {
-        // equal steps of the logit between the floor and the largest
-        float per = BINS / (max - floor);
-        per = per < 1e30f ? per : 1e30f;
-        auto bin_of = [&](float x) -> uint32_t {
-            const float b = (max - x) * per;
-            return b < (float)(BINS - 1) ? (uint32_t)b : BINS - 1;
-        };
-        clear();
-        each([&](float x, uint32_t i) {
-            if (x >= floor && in(x, i)) atomicAdd((unsigned long long*)&s.hist[bin_of(x)], (unsigned long long)metric(x));
-        });
-        find_bin(0, want);
-        if (s.bin == BINS) return NO_CUT;
-        uint32_t bin = s.bin;
-        uint64_t before = s.before;
-        auto gather = [&](float x, uint32_t i) {
-            const uint32_t at = atomicAdd(&s.count, 1u), key = key_of(x);
-            atomicMin(&s.low, key);
-            atomicMax(&s.high, key);
-            if (at < LIST) {
-                s.list_key[at] = (uint64_t)key << 32 | (0xffffffffu - i);
-                s.list_w[at] = metric(x);
-            }
-        };
-        each([&](float x, uint32_t i) {
-            if (x >= floor && bin_of(x) == bin && in(x, i)) gather(x, i);
-        });
+    // The cut among the members of a step, those with member(x, i), which s.places lists where they are not too many: the last of them that has less than `want` in front of it,
+    // `before` being what lies in front of them all.  metric(x): what one weighs.
+    template <typename In, typename M> __device__ __forceinline__ Cut cut_in_step(uint64_t before, double want, In member, M metric) {
         __syncthreads();
-        while (s.count > LIST && s.low < s.high) {
-            // steps of whole keys between the lowest and the highest of the members
-            const uint32_t low = s.low, high = s.high;
+        uint32_t low = 0xffffffffu, high = 0;
+        if (s.n > LIST) {
+            each([&](float x, int32_t i) {
+                if (!member(x, i)) return;
+                const uint32_t key = key_of(x);
+                low = key < low ? key : low;
+                high = key > high ? key : high;
+            });
+            key_range(low, high);
+        }
+        while (s.n > LIST && low < high) {
+            // steps of whole keys between the lowest and the highest
             uint32_t down = 0;
             while ((high - low) >> down >= BINS) down++;
+            auto among = [&](float x, int32_t i) -> bool { return member(x, i) && key_of(x) >= low && key_of(x) <= high; };
             clear();
-            each([&](float x, uint32_t i) {
-                const uint32_t key = key_of(x);
-                if (key >= low && key <= high && in(x, i)) atomicAdd((unsigned long long*)&s.hist[(high - key) >> down], (unsigned long long)metric(x));
+            each([&](float x, int32_t i) {
+                if (among(x, i)) atomicAdd((unsigned long long*)&s.hist[(high - key_of(x)) >> down], (unsigned long long)metric(x));
             });
             find_bin(before, want);
-            bin = s.bin < BINS ? s.bin : (high - low) >> down;  // (the last sum is the members': it reaches what is wanted)
+            const uint32_t bin = s.bin < BINS ? s.bin : (high - low) >> down;    // (the last sum is the members' whole: it reaches what is wanted)
             if (s.bin < BINS) before = s.before;
-            each([&](float x, uint32_t i) {
+            uint32_t l = 0xffffffffu, h = 0;
+            each([&](float x, int32_t i) {
+                if (!among(x, i) || (high - key_of(x)) >> down != bin) return;
                 const uint32_t key = key_of(x);
-                if (key >= low && key <= high && (high - key) >> down == bin && in(x, i)) gather(x, i);
+                l = key < l ? key : l;
+                h = key > h ? key : h;
+                list(x, i);
             });
-            __syncthreads();
+            key_range(l, h);
+            low = l;
+            high = h;
         }
-        const uint32_t n = s.count;
-        uint64_t cut;
+        const uint32_t n = s.n;
         if (n > LIST) {
             // all alike: as many as it takes, the lower indices first
-            const uint32_t key = s.low;
-            const uint64_t w = s.list_w[0];
+            const float same = of_key(low);
+            const uint64_t w = metric(same);
             uint32_t keep = n;
             if (w) {
                 const double more = (want - (double)before) / (double)w;
@@ -316,123 +390,170 @@ template <typename T, int ITS> struct Row {
                 while (keep < n && (double)(before + keep * w) < want) keep++;
             }
             uint64_t mine = 0, total;
-            auto same = [&](float x, uint32_t i) -> uint64_t { return key_of(x) == key && in(x, i); };
-            each([&](float x, uint32_t i) { mine += same(x, i); });
-            const uint32_t last = search(mine, false, 0.0f, keep - 1, same, total);
-            cut = (uint64_t)key << 32 | (0xffffffffu - last);
-        } else {
-            // each member adds up those in front of it
-            if (tid == 0) s.cut = ~0ull;
-            __syncthreads();
-            if (tid < n) {
-                const uint64_t me = s.list_key[tid];
-                uint64_t sum = before;
-                for (uint32_t j = 0; j < n; j++) sum += s.list_key[j] > me ? s.list_w[j] : 0;
-                if ((double)sum < want) atomicMin((unsigned long long*)&s.cut, (unsigned long long)me);
-            }
-            __syncthreads();
-            cut = s.cut;
+            auto is = [&](float x, int32_t i) -> uint64_t { return x == same && member(x, i); };
+            each([&](float x, int32_t i) { mine += is(x, i); });
+            return Cut{same, search(mine, false, 0.0f, keep ? keep - 1 : 0, is, total)};
         }
+        const uint64_t me = sorted(tid < n ? s.places[tid] : 0, n);
+        const uint64_t w = tid < n ? metric(of_key((uint32_t)(me >> 32))) : 0;
+        uint64_t upto;
+        if (tid == 0) s.cut = 0;                                // (all of them; but one place always is where the sum reaches what is wanted)
+        block_sum(w, &upto);
+        upto += before;
+        if (tid < n && (double)(upto - w) < want && !((double)upto < want)) s.cut = me;
         __syncthreads();
-        return cut;
+        return s.cut ? cut_at(s.cut) : Cut{-INFINITY, -1};
     }
 
-    // A bound that at least k logits reach: the kth largest of the threads' own maxima, rounded down to a step of whole keys
+    // A bound that at least k <= 1024 logits reach: of each wave the (k / 16)th largest of the lanes' own maxima, and of those the least.  -inf if some wave has fewer
     __device__ __forceinline__ float reached_by(uint32_t k, float mine) {
-        const uint32_t key = key_of(mine);
-        clear();
-        if (mine > -INFINITY) {
-            atomicMin(&s.low, key);
-            atomicMax(&s.high, key);
-        }
+        float x = mine;
+#pragma unroll 1
+        for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll 1
+            for (int stride = size / 2; stride; stride >>= 1) {
+                const float other = __shfl_xor(x, stride);
+                x = ((lane & stride) == 0) == ((lane & size) == 0) ? fmaxf(x, other) : fminf(x, other);
+            }
+        uint32_t low = key_of(__shfl(x, (int)((k + WAVES - 1) / WAVES) - 1)), high = low;
+        key_range(low, high);
+        return of_key(low);
+    }
+
+    // Draws from the n places of s.places, which hold all that may be kept: the first k of them, of those the ones with less than p of their weight
+    // in front of them, of those the ones that weigh min_p.
+    __device__ __forceinline__ void draw(uint32_t n, uint32_t k, float p, double min_p, float uniform, int32_t* token, float* prob) {
+        uint64_t* const heavy = s.hist + LIST;
         __syncthreads();
-        const uint32_t low = s.low, high = s.high;
-        uint32_t down = 0;
-        while ((high - low) >> down >= BINS) down++;
-        if (mine > -INFINITY) atomicAdd((unsigned long long*)&s.hist[(high - key) >> down], 1ull);
-        find_bin(0, (double)k);
-        if (s.bin == BINS) return -INFINITY;
-        const uint64_t far = ((uint64_t)(s.bin + 1) << down) - 1;
-        uint32_t bound = far < high - low ? high - (uint32_t)far : low;
-        bound = bound & 0x80000000u ? bound & 0x7fffffffu : ~bound;
-        return __uint_as_float(bound);
+        k = k < n ? k : n;
+        const uint64_t place = sorted(tid < n ? s.places[tid] : 0, n);
+        const double w = tid < k ? weight(of_key((uint32_t)(place >> 32))) : 0.0;
+        uint64_t f = tid < k ? fixed(w) : 0, upto;
+        heavy[tid] = f;
+        const uint64_t total = block_sum(f, &upto);
+        const double want = p > 0.0f ? (double)p * (double)total : 0.5;
+        const bool stays = tid < k && (!(p < 1.0f) || (double)(upto - f) < want) && w >= min_p;
+        const uint32_t kept = (uint32_t)block_sum(stays, nullptr);
+        if (tid == kept - 1) s.total = upto;
+        // those that stay, by index
+        const uint64_t by = sorted(tid < kept ? place << 32 | (tid + 1) : 0, kept);
+        const uint64_t whole = s.total, target = part_of(uniform, whole);
+        f = tid < kept ? heavy[(uint32_t)by - 1] : 0;
+        block_sum(f, &upto);
+        if (tid < kept && upto > target && upto - f <= target) {                // one does
+            *token = index_of(by >> 32);
+            if (prob) *prob = (float)((double)f / (double)whole);
+        }
     }
 };
 
-template <typename T, int ITS> __global__ void __launch_bounds__(BLOCK) sample_kernel(SampleArgs a) {
+template <typename T> __global__ void __launch_bounds__(BLOCK) sample_kernel(SampleArgs a) {
     __shared__ Shared s;
     const uint32_t row = blockIdx.x;
-    Row<T, ITS> r(a, s, row);
+    Row<T> r(a, s, row);
     const float temperature = a.temperature ? a.temperature[row] : 1.0f, uniform = a.uniform[row];
     const int32_t k = a.top_k ? a.top_k[row] : 0;
     const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p_raw = a.min_p ? a.min_p[row] : 0.0f;
-    r.load();
+    int32_t* const token_at = a.tokens + row;
+    float* const prob_at = a.probs ? a.probs + row : nullptr;
     float mine = -INFINITY;
-    r.each([&](float x, uint32_t) { mine = fmaxf(mine, x); });
-    r.max = r.block_max(mine);
-    if (r.max == -INFINITY) {                      // nothing to choose from
-        if (r.tid == 0) {
-            a.tokens[row] = -1;
-            if (a.probs) a.probs[row] = 0.0f;
-        }
-        return;
-    }
+    r.each([&](float x, int32_t) { mine = fmaxf(mine, x); });
+    uint32_t high = key_of(mine), none = 0;
+    r.block_max(high, none);
+    r.max = of_key(high);
     uint64_t total;
-    if (r.max == INFINITY) {
-        r.infinite = true;
-        r.max = 0.0f;
-        r.load();
-        mine = -INFINITY;
-        r.each([&](float x, uint32_t) { mine = fmaxf(mine, x); });
-    }
-    if (!(temperature > 0.0f)) {                   // greedy: the first of the largest
+    if (r.max == -INFINITY || r.max == INFINITY || !(temperature > 0.0f)) {
+        // nothing to choose from; equals that share all the weight; or, greedy, the first of the largest
+        auto top = [&](float x, int32_t) -> uint64_t { return x == r.max && x > -INFINITY; };
         uint64_t n = 0;
-        auto top = [&](float x, uint32_t) -> uint64_t { return x == r.max; };
-        r.each([&](float x, uint32_t i) { n += top(x, i); });
-        const uint32_t token = r.search(n, false, 0.0f, 0, top, total);
+        r.each([&](float x, int32_t i) { n += top(x, i); });
+        uint64_t m = r.block_sum(n);
+        if (!(temperature > 0.0f)) m = m < 1 ? m : 1;
+        if (k > 0 && (uint64_t)k < m) m = (uint64_t)k;
+        if (top_p < 1.0f && m) {
+            const double want = top_p > 0.0f ? ceil((double)top_p * (double)m) : 1.0;
+            m = want < 1.0 ? 1 : want < (double)m ? (uint64_t)want : m;
+        }
+        const int32_t token = r.search(n, false, 0.0f, r.part_of(uniform, m), top, total);
         if (r.tid == 0) {
-            a.tokens[row] = (int32_t)token;
-            if (a.probs) a.probs[row] = 1.0f;
+            *token_at = m ? token : -1;
+            if (prob_at) *prob_at = m ? (float)(1.0 / (double)m) : 0.0f;
         }
         return;
     }
     r.step = 1.4426950408889634 / (double)temperature;
     const double min_p = min_p_raw > 0.0f ? (min_p_raw < 1.0f ? min_p_raw : 1.0f) : 0.0;
-    uint64_t cut = NO_CUT;
-    auto above = [&](float x, uint32_t i) -> bool { return ((uint64_t)key_of(x) << 32 | (0xffffffffu - i)) >= cut && x > -INFINITY; };
-    if (k > 0 && (uint32_t)k < a.vocab) {
-        const float floor = (uint32_t)k <= BLOCK ? r.reached_by((uint32_t)k, mine) : -INFINITY;
-        cut = r.select((double)k, floor, [](float x, uint32_t) -> bool { return x > -INFINITY; }, [](float) -> uint64_t { return 1; });
-    }
-    if (top_p < 1.0f) {
-        uint64_t sum = 0;
-        r.each([&](float x, uint32_t i) {
-            if (above(x, i)) sum += r.fixed(r.weight(x));
-        });
-        sum = r.block_sum(sum);
-        // all of those below this weigh less than half of what may be dropped
+    Cut cut = {-INFINITY, -1};
+    // top-k counts, then top-p weighs.  What lies 48 temperatures below the largest weighs 0 in fixed point: whether it is among the k does not matter
+    for (int phase = 0; phase < 2; phase++) {
+        const bool counts = phase == 0;
+        if (counts ? k <= 0 || (uint32_t)k >= a.vocab : !(top_p < 1.0f)) continue;
+        const Cut front = cut;
         const float p = top_p > 0.0f ? top_p : 0.0f;
-        const float floor = p > 0.0f ? r.max - temperature * 0.7f * __builtin_amdgcn_logf(2.0f * (float)a.vocab / (1.0f - p)) : r.max;
-        const double want = p > 0.0f ? (double)p * (double)sum : 0.5;
-        const uint64_t cut_p = r.select(want, floor, above, [&](float x) -> uint64_t { return r.fixed(r.weight(x)); });
-        cut = cut_p > cut ? cut_p : cut;
+        float floor;
+        if (counts) {
+            floor = (uint32_t)k <= BLOCK ? r.reached_by((uint32_t)k, mine) : -INFINITY;
+            floor = fmaxf(floor, r.max - 48.0f * temperature);
+        } else {
+            // all of those below this weigh less than half of what may be dropped; 0.7 is a little above ln 2
+            floor = p > 0.0f ? r.max - temperature * 0.7f * __builtin_amdgcn_logf(2.0f * (float)a.vocab / (1.0f - p)) : r.max;
+        }
+        floor = fmaxf(floor, -3.4028235e38f);                   // (of an endless temperature: all that are finite)
+        auto in = [&](float x, int32_t i) -> bool { return x >= floor && front.keeps(x, i); };
+        if (counts && (uint32_t)k <= LIST / 4) {
+            r.clear();
+            r.each([&](float x, int32_t i) {
+                if (in(x, i)) r.list(x, i);
+            });
+            __syncthreads();
+            if (s.n <= LIST) {
+                r.draw(s.n, (uint32_t)k, top_p, min_p, uniform, token_at, prob_at);
+                return;
+            }
+        }
+        float per = BINS / (r.max - floor);                     // equal steps of the logit between the floor and the largest
+        per = per < 1e30f ? per : 1e30f;
+        auto bin_of = [&](float x) -> uint32_t {
+            const float b = (r.max - x) * per;
+            return b < (float)(BINS - 1) ? (uint32_t)b : BINS - 1;
+        };
+        auto metric = [&](float x) -> uint64_t { return counts ? 1 : r.fixed(r.weight(x)); };
+        r.clear();
+        uint64_t sum = 0;
+        r.each([&](float x, int32_t i) {
+            if (front.keeps(x, i)) {
+                const uint64_t w = metric(x);
+                sum += w;
+                if (x >= floor) atomicAdd((unsigned long long*)&s.hist[bin_of(x)], (unsigned long long)w);
+            }
+        });
+        const uint64_t whole = r.block_sum(sum);
+        const double want = counts ? (double)k : p > 0.0f ? (double)p * (double)whole : 0.5;
+        r.find_bin(0, want);
+        const uint32_t bin = s.bin;
+        const uint64_t before = s.before;
+        if (bin == BINS) continue;                              // fewer than k
+        r.each([&](float x, int32_t i) {
+            if (in(x, i) && bin_of(x) == bin) r.list(x, i);
+        });
+        cut = r.cut_in_step(before, want, [&](float x, int32_t i) -> bool { return in(x, i) && bin_of(x) == bin; }, metric);
     }
-    auto kept = [&](float x, uint32_t i) -> uint64_t {
-        if (!above(x, i)) return 0;
+    auto kept = [&](float x, int32_t i) -> uint64_t {
+        if (!cut.keeps(x, i)) return 0;
         const double w = r.weight(x);
         return w >= min_p ? r.fixed(w) : 0;
     };
     uint64_t sum = 0;
-    r.each([&](float x, uint32_t i) { sum += kept(x, i); });
-    const uint32_t token = r.search(sum, true, uniform, 0, kept, total);
+    r.each([&](float x, int32_t i) { sum += kept(x, i); });
+    const int32_t token = r.search(sum, true, uniform, 0, kept, total);
     if (r.tid == 0) {
-        a.tokens[row] = (int32_t)token;
-        if (a.probs) a.probs[row] = (float)((double)kept(r.clean(Ar<T>::widen(((const T*)a.x)[row * a.stride + token])), token) / (double)total);
+        *token_at = token;
+        if (prob_at) *prob_at = (float)((double)kept(Ar<T>::widen(((const T*)a.x)[row * a.stride + token]), token) / (double)total);
     }
 }
 
 template <typename T> int launch(rt_device* dev, const SampleArgs& a, uint32_t rows) {
-    hipLaunchKernelGGL((sample_kernel<T, 0>), dim3(rows), dim3(BLOCK), 0, dev->stream, a);
+    hipLaunchKernelGGL((sample_kernel<T>), dim3(rows), dim3(BLOCK), 0, dev->stream, a);
     RT_CHECK_LAUNCH("sample_kernel");
     return RT_OK;
 }
@@ -461,6 +582,7 @@ extern "C" int rt_sample(rt_device* dev, int dt, const void* x, uint64_t row_str
     int scale = 46;                                             // the sum of the weights, at most vocab, stays below 2^62; 46 bits to a weight up to 2^16 tokens
     while ((uint64_t)vocab << scale > 1ull << 62) scale--;
     a.magic = ldexp(1.0, 52 - scale);
+    for (int t = 0; t < TERMS; t++) a.exp2[t] = EXP2[t];
     switch (dt) {
         case RT_F32: return launch<float>(dev, a, rows);
         case RT_F16: return launch<half_t>(dev, a, rows);
