@@ -44,6 +44,7 @@ struct AttnArgs {
     // calls that change or mask their scores (rt_scores)
     bool scored;
     float most, most_in;           // cap * log2(e), 0: none; scale / cap
+    float near[4], near_limit;     // 16-bit products up to near_limit take the polynomial x (near[0] + near[1] x^2 + ..) for the capped score
     const float* slopes;
     const int32_t* documents;
     uint32_t n_documents;
@@ -141,25 +142,46 @@ __device__ __forceinline__ AttnRow at_in_text(const AttnArgs& a, int32_t p, int3
     }
     return r;
 }
-// The document of position p: the last that begins at or before it; n_documents or above where it is in none.  All lanes of a wave take part, with the same p.
 __device__ __forceinline__ uint32_t at_find(const int32_t* starts, uint32_t seqs, uint32_t token);
-__device__ __forceinline__ uint32_t at_document(const AttnArgs& a, uint32_t b, int32_t p) {
-    return at_find(a.documents + (uint64_t)b * (a.n_documents + 1), a.n_documents + 1, (uint32_t)p);
-}
-__device__ __forceinline__ AttnRow at_in_document(const AttnArgs& a, uint32_t b, const AttnSeq& s, int32_t p, uint32_t d) {
-    const int32_t* at = a.documents + (uint64_t)b * (a.n_documents + 1);
-    if (d >= a.n_documents) {                      // in front of the first, or behind the last: a text without keys
-        const int32_t here = at_between(at[d == a.n_documents ? d : 0], 0, s.keys);
-        return at_in_text(a, p, here, here, 0);
+
+// The texts of one entry of a call with documents, by all lanes of a wave: up to 63 are looked at once, a lane to a text, and what is asked of them later is a vote of the lanes
+struct AttnTexts {
+    int32_t start, prefix;                         // of text `lane`, where all fit
+};
+__device__ __forceinline__ AttnTexts at_texts(const AttnArgs& a, uint32_t b) {
+    AttnTexts t = {AT_FAR, 0};
+    if (a.documents && a.n_documents < 64) {
+        const uint32_t lane = __lane_id();
+        if (lane <= a.n_documents) t.start = a.documents[(uint64_t)b * (a.n_documents + 1) + lane];
+        if (a.prefix && lane < a.n_documents) t.prefix = a.prefix[(uint64_t)b * a.n_documents + lane];
     }
-    const int32_t lo = at_between(at[d], 0, s.keys), hi = at_between(at[d + 1], lo, s.keys);
-    return at_in_text(a, p, lo, hi, a.prefix ? a.prefix[(uint64_t)b * a.n_documents + d] : 0);
+    return t;
+}
+// The document of position p, the same in all lanes: the last that begins at or before it; n_documents or above where it is in none
+__device__ __forceinline__ uint32_t at_document(const AttnArgs& a, const AttnTexts& t, uint32_t b, int32_t p) {
+    if (a.n_documents < 64) return (uint32_t)__popcll(__ballot(t.start <= p)) - 1;         // (none in front of the first: the largest number)
+    return __builtin_amdgcn_readfirstlane(at_find(a.documents + (uint64_t)b * (a.n_documents + 1), a.n_documents + 1, (uint32_t)p));
+}
+// Where document d begins (n_documents: where the last one ends).  d may differ from lane to lane, all of which take part
+__device__ __forceinline__ int32_t at_start(const AttnArgs& a, const AttnTexts& t, uint32_t b, uint32_t d) {
+    return a.n_documents < 64 ? __shfl(t.start, (int)d) : a.documents[(uint64_t)b * (a.n_documents + 1) + d];
+}
+__device__ __forceinline__ AttnRow at_in_document(const AttnArgs& a, const AttnTexts& t, uint32_t b, const AttnSeq& s, int32_t p, uint32_t d) {
+    const bool none = d >= a.n_documents;          // in front of the first, or behind the last: a text without keys
+    const uint32_t from = !none ? d : d == a.n_documents ? d : 0, to = !none ? d + 1 : from;
+    const int32_t lo = at_between(at_start(a, t, b, from), 0, s.keys), hi = at_between(at_start(a, t, b, to), lo, s.keys);
+    int32_t prefix = 0;
+    if (a.prefix) {
+        prefix = a.n_documents < 64 ? __shfl(t.prefix, (int)(none ? 0 : d)) : a.prefix[(uint64_t)b * a.n_documents + (none ? 0 : d)];
+        if (none) prefix = 0;
+    }
+    return at_in_text(a, p, lo, hi, prefix);
 }
 // Row j of sequence b; all lanes take part, with the same row
-template <bool SCORED> __device__ __forceinline__ AttnRow at_row(const AttnArgs& a, uint32_t b, const AttnSeq& s, uint32_t j) {
+template <bool SCORED> __device__ __forceinline__ AttnRow at_row(const AttnArgs& a, const AttnTexts& t, uint32_t b, const AttnSeq& s, uint32_t j) {
     const int32_t p = at_position(s, j);
     if (!SCORED) return AttnRow{p, at_limit(a, s, j), 0, a.sinks};
-    if (a.documents) return at_in_document(a, b, s, p, at_document(a, b, p));
+    if (a.documents) return at_in_document(a, t, b, s, p, at_document(a, t, b, p));
     return at_in_text(a, p, 0, s.keys, a.prefix ? a.prefix[b] : 0);
 }
 template <bool SCORED> __device__ __forceinline__ bool at_sees(const AttnArgs& a, const AttnRow& r, int32_t t) {

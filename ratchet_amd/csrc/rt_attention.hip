@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(BLOCK) attention_any_kernel(AttnArgs a, uint64
     const T* q = (const T*)a.q + b * a.q_b + h * a.q_h + (uint64_t)(s.first + j) * a.q_t;
     const T* k = (const T*)a.k + g * a.k_h + (PAGED ? 0 : b * a.k_b);
     const T* v = (const T*)a.v + g * a.v_h + (PAGED ? 0 : b * a.v_b);
-    const AttnRow r = at_row<SCORED>(a, b, s, j);
+    const AttnRow r = at_row<SCORED>(a, SCORED ? at_texts(a, b) : AttnTexts{}, b, s, j);
     const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
     float m = -INFINITY, l = 0.0f, o[AT_MAX_DIM / 64];
 #pragma unroll
@@ -196,6 +196,16 @@ int score_rules(const char* who, const rt_scores* scores, float scale, uint32_t 
     a.scored = scores->cap != 0.0f || scores->slopes || scores->documents || scores->prefix;       // else it is attention as it ever was
     a.most = scores->cap * 1.4426950408889634f;
     a.most_in = scores->cap != 0.0f ? scale / scores->cap : 0.0f;
+    // tanh y = y (t0 + t1 y^2 + t2 y^4 + t3 y^6), through its values at Chebyshev's points of y^2 <= 0.16 and 1e-7 of it off at most.  Only where no power of
+    // scale / cap leaves f32's range
+    const float k = a.most_in < 0.0f ? -a.most_in : a.most_in;
+    a.near_limit = -1.0f;
+    if (k > 0x1p-16f && k < 0x1p16f && a.most > 0x1p-16f && a.most < 0x1p16f) {
+        static const double tanh_terms[4] = {0.9999999013476046, -0.3333135628726226, 0.1327087433318406, -0.04754934670684051};
+        double power = (double)a.most * k;
+        for (int i = 0; i < 4; i++, power *= (double)k * k) a.near[i] = (float)(tanh_terms[i] * power);
+        a.near_limit = 0.4f / k;
+    }
     a.slopes = scores->slopes;
     a.documents = scores->documents;
     a.n_documents = scores->n_documents;

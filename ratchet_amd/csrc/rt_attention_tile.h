@@ -137,10 +137,10 @@ struct AttnWalk {
     uint32_t tiles, head;
     int32_t start, from;
 };
-template <int KT, bool SCORED> __device__ __forceinline__ AttnWalk at_walk(const AttnArgs& a, uint32_t b, const AttnSeq& s, uint32_t row0, uint32_t rows) {
+template <int KT, bool SCORED> __device__ __forceinline__ AttnWalk at_walk(const AttnArgs& a, const AttnTexts& texts, uint32_t b, const AttnSeq& s, uint32_t row0, uint32_t rows) {
     const uint32_t j0 = fd_div(row0, a.group_div), j1 = fd_div(row0 + rows - 1, a.group_div);
-    AttnRow r0 = at_row<SCORED>(a, b, s, j0);
-    int32_t last = at_row<SCORED>(a, b, s, j1).limit;
+    AttnRow r0 = at_row<SCORED>(a, texts, b, s, j0);
+    int32_t last = at_row<SCORED>(a, texts, b, s, j1).limit;
     if (SCORED) {                                               // the same in all lanes, which the compiler cannot know
         r0.p = __builtin_amdgcn_readfirstlane(r0.p);
         r0.lo = __builtin_amdgcn_readfirstlane(r0.lo);
@@ -298,7 +298,7 @@ __device__ __forceinline__ void at_row_again(const AttnArgs& a, uint32_t b, uint
     const T* q = (const T*)a.q + b * a.q_b + h * a.q_h + (uint64_t)(s.first + j) * a.q_t;
     const T* k = (const T*)a.k + g * a.k_h + (PAGED ? 0 : b * a.k_b);
     const T* v = (const T*)a.v + g * a.v_h + (PAGED ? 0 : b * a.v_b);
-    const AttnRow r = at_row<SCORED>(a, b, s, j);
+    const AttnRow r = at_row<SCORED>(a, SCORED && !PAGED ? at_texts(a, b) : AttnTexts{}, b, s, j);
     const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -529,7 +529,8 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         tile = at_row_tiles(a, s) - 1 - tile;
     }
     const uint32_t all = s.count * a.group, row0 = tile * AT_ROWS, rows = all - row0 < AT_ROWS ? all - row0 : AT_ROWS;
-    const AttnWalk w = at_walk<KT, SCORED>(a, b, s, row0, rows);
+    const AttnTexts texts = SCORED && !PAGED ? at_texts(a, b) : AttnTexts{};
+    const AttnWalk w = at_walk<KT, SCORED>(a, texts, b, s, row0, rows);
     const uint32_t tile0 = piece_at * piece, tile1 = w.tiles - tile0 < piece || tile0 >= w.tiles ? w.tiles : tile0 + piece;
     const bool whole = w.tiles <= piece;                        // no other block has keys of these rows
     if (tile0 >= w.tiles && piece_at > 0) return;
@@ -547,14 +548,14 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
     if constexpr (SCORED) {
         AttnRow me, ra, rz;
         if (!PAGED && a.documents) {
-            const uint32_t da = at_document(a, b, at_position(s, ja)), dz = at_document(a, b, at_position(s, jz));
-            ra = at_in_document(a, b, s, at_position(s, ja), da);
-            rz = at_in_document(a, b, s, at_position(s, jz), dz);
+            const uint32_t da = at_document(a, texts, b, at_position(s, ja)), dz = at_document(a, texts, b, at_position(s, jz));
+            ra = at_in_document(a, texts, b, s, at_position(s, ja), da);
+            rz = at_in_document(a, texts, b, s, at_position(s, jz), dz);
             uint32_t d = da;                                    // may be `none in front`, beyond all numbers
             if (dz <= a.n_documents)
                 for (uint32_t n = da > a.n_documents ? 0 : da + 1; n <= dz; n++)
-                    if (a.documents[(uint64_t)b * (a.n_documents + 1) + n] <= at_position(s, j)) d = n;
-            me = at_in_document(a, b, s, at_position(s, j), d);
+                    if (at_start(a, texts, b, n) <= at_position(s, j)) d = n;
+            me = at_in_document(a, texts, b, s, at_position(s, j), d);
         } else {
             const int32_t prefix = a.prefix ? a.prefix[b] : 0;
             me = at_in_text(a, at_position(s, j), 0, s.keys, prefix);
@@ -739,24 +740,46 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
 #pragma unroll
         for (int kk = 0; kk < S::HALVES; kk++) at_join_sums(x[kk], others[kk]);
         if (changed) {
-            const float most_in = __builtin_fabsf(a.most_in), cc = __builtin_fabsf(a.c);
             if (a.most != 0.0f) {
+                bool near = false;
+                if (sizeof(T) == 2) {
+                    float far = 0.0f;
 #pragma unroll
-                for (int kk = 0; kk < S::HALVES; kk++)
+                    for (int kk = 0; kk < S::HALVES; kk++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[kk][e] = at_capped<T>(a.most, x[kk][e] * most_in);
-            } else {
+                        for (int e = 0; e < 16; e++) far = fmaxf(far, __builtin_fabsf(x[kk][e]));
+                    near = __ballot(!(far <= a.near_limit)) == 0;
+                }
+                if (near) {                                     // half of what the exponential and the reciprocal take
 #pragma unroll
-                for (int kk = 0; kk < S::HALVES; kk++)
+                    for (int kk = 0; kk < S::HALVES; kk++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[kk][e] *= cc;
+                        for (int e = 0; e < 16; e++) {
+                            const float z = x[kk][e] * x[kk][e];
+                            x[kk][e] *= __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(a.near[3], z, a.near[2]), z, a.near[1]), z, a.near[0]);
+                        }
+                } else {
+                    const float most_in = __builtin_fabsf(a.most_in);
+#pragma unroll
+                    for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[kk][e] = at_capped<T>(a.most, x[kk][e] * most_in);
+                }
             }
             if (a.slopes) {
-                const float far = (float)(p - t0 - 4 * (int32_t)half);          // distance of the tile's first key of this half
+                const float far = (float)(p - t0 - 4 * (int32_t)half), cc = a.most != 0.0f ? 1.0f : __builtin_fabsf(a.c);    // distance of the tile's first key of this half
+                if (a.causal && !a.prefix) {                    // keys behind the query are hidden: the distance has no other sign
+                    const float first = -slope * far;
 #pragma unroll
-                for (int kk = 0; kk < S::HALVES; kk++)
+                    for (int kk = 0; kk < S::HALVES; kk++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(-slope, __builtin_fabsf(far - (float)(32 * kk + e % 4 + 8 * (e / 4))), x[kk][e]);
+                        for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(x[kk][e], cc, __builtin_fmaf((float)(32 * kk + e % 4 + 8 * (e / 4)), slope, first));
+                } else {
+#pragma unroll
+                    for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(-slope, __builtin_fabsf(far - (float)(32 * kk + e % 4 + 8 * (e / 4))), x[kk][e] * cc);
+                }
             }
         }
         if (t0 + KT - 1 > limit_a || (SCORED && !PAGED && t0 < lo_z) || (t0 + KT > (SCORED ? front_a : a.sinks) && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
@@ -982,7 +1005,7 @@ template <typename T, int KT, bool PAGED, bool SCORED> __global__ void __launch_
         first = (uint64_t)(part.row_tiles - 1 - tile) * part.pieces * stride + pair;
     }
     const uint32_t all_rows = s.count * a.group, row0 = tile * AT_ROWS, rows = all_rows - row0 < AT_ROWS ? all_rows - row0 : AT_ROWS;
-    const AttnWalk w = at_walk<KT, SCORED>(a, b, s, row0, rows);
+    const AttnWalk w = at_walk<KT, SCORED>(a, SCORED && !PAGED ? at_texts(a, b) : AttnTexts{}, b, s, row0, rows);
     const uint32_t r0 = blockIdx.y * AT_JOIN_ROWS, r1 = r0 + AT_JOIN_ROWS < rows ? r0 + AT_JOIN_ROWS : rows;
     if (w.tiles <= piece || r0 >= rows) return;
     const uint32_t used = (w.tiles + piece - 1) / piece;
