@@ -65,7 +65,7 @@ template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_span(const
     }
     return n ? n : 1;
 }
-__device__ __forceinline__ uint32_t at_row_tiles(const AttnArgs& a, const AttnSeq& s) { return (s.count * a.group + AT_ROWS - 1) / AT_ROWS; }
+template <uint32_t ROWS> __device__ __forceinline__ uint32_t at_row_tiles(const AttnArgs& a, const AttnSeq& s) { return (s.count * a.group + ROWS - 1) / ROWS; }
 
 template <typename T> __device__ __forceinline__ T at_wave_sum(T x) {
 #pragma unroll
@@ -81,14 +81,14 @@ template <bool FEW> __host__ __device__ __forceinline__ uint32_t at_piece_for(ui
     return n < least ? least : n > 0x7fffffffu ? 0x7fffffffu : (uint32_t)n;
 }
 // The same from the device's lengths; the same in every wave.
-template <int KT, bool FEW, bool SCORED> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a) {
+template <int KT, bool FEW, bool SCORED, uint32_t ROWS> __device__ __forceinline__ uint32_t at_piece(const AttnArgs& a) {
     uint64_t work = 0;
     uint32_t tiles = 0;
     for (uint32_t b = __lane_id(); b < a.seqs; b += 64) {
         const AttnSeq s = at_seq<true>(a, b);
         const uint32_t span = at_span<KT, SCORED>(a, b, s), less = FEW ? 0 : s.count / (2 * KT);           // causal: the middle row of the new ones lacks half of them
-        work += (uint64_t)at_row_tiles(a, s) * (span > 2 * less ? span - less : (span + 1) / 2);
-        tiles += at_row_tiles(a, s);
+        work += (uint64_t)at_row_tiles<ROWS>(a, s) * (span > 2 * less ? span - less : (span + 1) / 2);
+        tiles += at_row_tiles<ROWS>(a, s);
     }
     return at_piece_for<FEW>((uint64_t)at_wave_sum(tiles) * a.kv_heads, at_wave_sum(work) * a.kv_heads);
 }
@@ -100,16 +100,16 @@ __host__ __device__ __forceinline__ uint32_t at_piece_of(uint32_t piece, uint32_
 }
 
 // Sequence b's items are numbered row tile by row tile, at_items of them, after those of the sequences before it.
-template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_items(const AttnArgs& a, uint32_t b, uint32_t piece) {
+template <int KT, bool SCORED, uint32_t ROWS> __device__ __forceinline__ uint32_t at_items(const AttnArgs& a, uint32_t b, uint32_t piece) {
     const AttnSeq s = at_seq<true>(a, b);
     const uint32_t span = at_span<KT, SCORED>(a, b, s), n = at_piece_of(piece, span);
-    return at_row_tiles(a, s) * ((span + n - 1) / n);
+    return at_row_tiles<ROWS>(a, s) * ((span + n - 1) / n);
 }
 // The sequence that item `at` belongs to (a.seqs: none); `at` becomes its number there.  All lanes of a wave take part.
-template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_locate(const AttnArgs& a, uint32_t piece, uint32_t& at) {
+template <int KT, bool SCORED, uint32_t ROWS> __device__ __forceinline__ uint32_t at_locate(const AttnArgs& a, uint32_t piece, uint32_t& at) {
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.seqs; b0 += 64) {
-        const uint32_t b = b0 + __lane_id(), n = b < a.seqs ? at_items<KT, SCORED>(a, b, piece) : 0;
+        const uint32_t b = b0 + __lane_id(), n = b < a.seqs ? at_items<KT, SCORED, ROWS>(a, b, piece) : 0;
         uint32_t sum = n;                                       // of this lane and those below
 #pragma unroll
         for (int i = 1; i < 64; i <<= 1) {
@@ -126,9 +126,9 @@ template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_locate(con
     }
     return a.seqs;
 }
-template <int KT, bool SCORED> __device__ __forceinline__ uint32_t at_before(const AttnArgs& a, uint32_t piece, uint32_t until) {
+template <int KT, bool SCORED, uint32_t ROWS> __device__ __forceinline__ uint32_t at_before(const AttnArgs& a, uint32_t piece, uint32_t until) {
     uint32_t sum = 0;
-    for (uint32_t b = __lane_id(); b < until; b += 64) sum += at_items<KT, SCORED>(a, b, piece);
+    for (uint32_t b = __lane_id(); b < until; b += 64) sum += at_items<KT, SCORED, ROWS>(a, b, piece);
     return at_wave_sum(sum);
 }
 
@@ -417,7 +417,7 @@ template <bool ATOMIC> __device__ __forceinline__ void at_get(const float* from,
 
 // Joins `used` parts, `stride` blocks apart from block `first` on, of rows r0 .. r1 - 1 of the row tile at row0.  factors: LDS for (r1 - r0) * used floats.
 // First each row's factors 2^(m_k - m) / l, then the sums, eight parts in flight.
-template <typename T, bool ATOMIC>
+template <typename T, bool ATOMIC, uint32_t ROWS>
 __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& part, const AttnSeq& s, uint32_t b, uint32_t g, uint32_t row0, uint32_t r0, uint32_t r1, uint64_t first,
                                         uint64_t stride, uint32_t used, float* factors) {
     const uint32_t D = a.dim, quads = D / 4, n = r1 - r0;
@@ -431,7 +431,7 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
             const uint32_t k = part_lane + 16 * u;
             mk[u] = -INFINITY;
             lk[u] = 0.0f;
-            if (i < n && k < used) at_get<ATOMIC>(part.ml + 2 * ((first + k * stride) * AT_ROWS + r0 + i), mk[u], lk[u]);
+            if (i < n && k < used) at_get<ATOMIC>(part.ml + 2 * ((first + k * stride) * ROWS + r0 + i), mk[u], lk[u]);
         }
 #pragma unroll
         for (uint32_t u = 0; u < (AT_MOST_PIECES + 15) / 16; u++) m = fmaxf(m, mk[u]);
@@ -457,8 +457,8 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n * quads; i += AT_BLOCK) {
         const uint32_t r = i / quads, d = (i - r * quads) * 4;
-        const float* from = part.o + (first * AT_ROWS + r0 + r) * D + d;
-        const uint64_t next = stride * AT_ROWS * D;
+        const float* from = part.o + (first * ROWS + r0 + r) * D + d;
+        const uint64_t next = stride * ROWS * D;
         float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (uint32_t k0 = 0; k0 < used; k0 += 8) {
             float x[8][4];
@@ -487,6 +487,27 @@ __device__ __forceinline__ void at_join(const AttnArgs& a, const AttnPartial& pa
     }
 }
 
+// A tile's rows computed again where they are not finite: row `row`, by a wave, to y or to its part
+template <typename T, int DT, bool PAGED, int KT, bool SCORED, bool ATOMIC>
+__device__ __forceinline__ void at_again(const AttnArgs& a, const AttnPartial& part, uint32_t b, uint32_t g, const AttnSeq& s, const AttnWalk& w, uint32_t tile0, uint32_t tile1,
+                                         uint32_t row, uint64_t part_at, bool whole) {
+    const uint32_t lane = __lane_id(), D = a.dim;
+    float oo[(DT + 63) / 64], mm, ll;
+    at_row_again<T, DT, PAGED, KT, SCORED>(a, b, g, s, w, tile0, tile1, row, oo, mm, ll);
+    const uint32_t jj = fd_div(row, a.group_div), hh = g * a.group + (row - jj * a.group);
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+    T* y = (T*)a.y + b * a.y_b + hh * a.y_h + (uint64_t)(s.first + jj) * a.y_t;
+#pragma unroll
+    for (uint32_t i = 0; i < (DT + 63) / 64; i++) {
+        const float next = __shfl_down(oo[i], 1);
+        if (i * 64 + lane >= D) continue;
+        if (whole) y[i * 64 + lane] = Ar<T>::conv(oo[i] * inv);
+        else if (lane % 2 == 0) at_put<ATOMIC>(part.o + part_at * D + i * 64 + lane, oo[i], next);
+    }
+    if (lane == 0 && !whole) at_put<ATOMIC>(part.ml + 2 * part_at, mm, ll);
+    if (lane == 0 && whole && a.lse) a.lse[b * a.l_b + hh * a.l_h + (uint64_t)(s.first + jj) * a.l_t] = at_lse(mm, ll);
+}
+
 // FEW: pieces are joined by the block that comes last (a joining launch took 10 to 13 us more), and scores are left where they are
 // wanted.  Waves of a SIMD: as many as the registers let, four where the rows have 64 columns and no page table is followed (encoder in f32: 146.5 us a call, with three 148.7)
 template <typename T, int DT, bool EXACT, bool PAGED, bool FEW, bool SCORED>
@@ -506,8 +527,8 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         stride = a.kv_heads;
         g = blockIdx.x % a.kv_heads;
         uint32_t at = blockIdx.x / a.kv_heads;
-        piece = part.split ? __builtin_amdgcn_readfirstlane(at_piece<KT, FEW, SCORED>(a)) : 0x7fffffffu;
-        b = __builtin_amdgcn_readfirstlane(at_locate<KT, SCORED>(a, piece, at));
+        piece = part.split ? __builtin_amdgcn_readfirstlane(at_piece<KT, FEW, SCORED, AT_ROWS>(a)) : 0x7fffffffu;
+        b = __builtin_amdgcn_readfirstlane(at_locate<KT, SCORED, AT_ROWS>(a, piece, at));
         if (b >= a.seqs) return;
         tile = __builtin_amdgcn_readfirstlane(at);
         piece_at = 0;
@@ -526,7 +547,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         const uint32_t pieces = (span + piece - 1) / piece;
         tile = at / pieces;
         piece_at = at - tile * pieces;
-        tile = at_row_tiles(a, s) - 1 - tile;
+        tile = at_row_tiles<AT_ROWS>(a, s) - 1 - tile;
     }
     const uint32_t all = s.count * a.group, row0 = tile * AT_ROWS, rows = all - row0 < AT_ROWS ? all - row0 : AT_ROWS;
     const AttnTexts texts = SCORED && !PAGED ? at_texts(a, b) : AttnTexts{};
@@ -914,23 +935,8 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
             if (32 * i + 8 * (e / 4) + 4 * half < D) fine = fine && __builtin_isfinite(o[i][e]);
     if (__ballot(r < rows && !fine)) {
         const uint32_t end = wave * 32 + 32 < rows ? wave * 32 + 32 : rows;
-        for (uint32_t rr = wave * 32; rr < end; rr++) {
-            float oo[(DT + 63) / 64], mm, ll;
-            at_row_again<T, DT, PAGED, KT, SCORED>(a, b, g, s, w, tile0, tile1, row0 + rr, oo, mm, ll);
-            const uint32_t jj = fd_div(row0 + rr, a.group_div), hh = g * a.group + (row0 + rr - jj * a.group);
-            const uint64_t part_at = (uint64_t)blockIdx.x * AT_ROWS + rr;
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-            T* y = (T*)a.y + b * a.y_b + hh * a.y_h + (uint64_t)(s.first + jj) * a.y_t;
-#pragma unroll
-            for (uint32_t i = 0; i < (DT + 63) / 64; i++) {
-                const float next = __shfl_down(oo[i], 1);
-                if (i * 64 + lane >= D) continue;
-                if (whole) y[i * 64 + lane] = Ar<T>::conv(oo[i] * inv);
-                else if (lane % 2 == 0) at_put<FEW>(part.o + part_at * D + i * 64 + lane, oo[i], next);
-            }
-            if (lane == 0 && !whole) at_put<FEW>(part.ml + 2 * part_at, mm, ll);
-            if (lane == 0 && whole && a.lse) a.lse[b * a.l_b + hh * a.l_h + (uint64_t)(s.first + jj) * a.l_t] = at_lse(mm, ll);
-        }
+        for (uint32_t rr = wave * 32; rr < end; rr++)
+            at_again<T, DT, PAGED, KT, SCORED, FEW>(a, part, b, g, s, w, tile0, tile1, row0 + rr, (uint64_t)blockIdx.x * AT_ROWS + rr, whole);
     } else if (r < rows && whole) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         T* y = (T*)a.y + b * a.y_b + h * a.y_h + (uint64_t)(s.first + j) * a.y_t;
@@ -970,7 +976,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
     if (!FEW || whole) return;
     const uint32_t used = (w.tiles + piece - 1) / piece, first = blockIdx.x - piece_at * stride;
     if (at_last(part.arrivals + first, used, (volatile uint32_t*)(smem + S::LDS - 16)))
-        at_join<T, true>(a, part, s, b, g, row0, 0, rows, first, stride, used, (float*)smem);
+        at_join<T, true, AT_ROWS>(a, part, s, b, g, row0, 0, rows, first, stride, used, (float*)smem);
 }
 
 // Parts of a row to the row: bound by reading them, 512 bytes a row, piece and 128 columns, and by the launch (encoder: 10 us, ragged chunks: 16 us with their search).
@@ -984,16 +990,16 @@ template <typename T, int KT, bool PAGED, bool SCORED> __global__ void __launch_
         // numbered as the items are, with one piece a row tile
         g = blockIdx.x % a.kv_heads;
         uint32_t at = blockIdx.x / a.kv_heads;
-        b = __builtin_amdgcn_readfirstlane(at_locate<KT, SCORED>(a, 0x7fffffffu, at));
+        b = __builtin_amdgcn_readfirstlane(at_locate<KT, SCORED, AT_ROWS>(a, 0x7fffffffu, at));
         if (b >= a.seqs) return;
         s = at_seq<true>(a, b);
         tile = __builtin_amdgcn_readfirstlane(at);
-        const uint32_t span = at_span<KT, SCORED>(a, b, s), all = __builtin_amdgcn_readfirstlane(at_piece<KT, false, SCORED>(a));
+        const uint32_t span = at_span<KT, SCORED>(a, b, s), all = __builtin_amdgcn_readfirstlane(at_piece<KT, false, SCORED, AT_ROWS>(a));
         piece = at_piece_of(all, span);
         pieces = (span + piece - 1) / piece;
         if (pieces == 1) return;
         stride = a.kv_heads;
-        first = (__builtin_amdgcn_readfirstlane(at_before<KT, SCORED>(a, all, b)) + (uint64_t)(at_row_tiles(a, s) - 1 - tile) * pieces) * stride + g;
+        first = (__builtin_amdgcn_readfirstlane(at_before<KT, SCORED, AT_ROWS>(a, all, b)) + (uint64_t)(at_row_tiles<AT_ROWS>(a, s) - 1 - tile) * pieces) * stride + g;
     } else {
         stride = (uint64_t)a.seqs * a.kv_heads;
         const uint32_t pair = (uint32_t)(blockIdx.x % stride);
@@ -1010,7 +1016,7 @@ template <typename T, int KT, bool PAGED, bool SCORED> __global__ void __launch_
     if (w.tiles <= piece || r0 >= rows) return;
     const uint32_t used = (w.tiles + piece - 1) / piece;
     if (first + (used - 1) * stride >= tile_blocks) return;     // as in the tiles' kernel: starts that decrease
-    at_join<T, false>(a, part, s, b, g, row0, r0, r1, first, stride, used, factors);
+    at_join<T, false, AT_ROWS>(a, part, s, b, g, row0, r0, r1, first, stride, used, factors);
 }
 
 template <typename T, int DT, bool EXACT, bool PAGED, bool SCORED> int at_launch_tile(rt_device* dev, AttnArgs& a, bool* done) {
@@ -1082,6 +1088,10 @@ template <typename T, int DT, bool EXACT, bool PAGED, bool SCORED> int at_launch
     return RT_OK;
 }
 
+// rt_attention_few.h: calls of a few rows a sequence
+template <typename T> bool at_fits_few(const AttnArgs& a, bool paged);
+template <typename T> int at_dispatch_few(rt_device* dev, AttnArgs& a, bool paged, bool* done);
+
 template <typename T, bool SCORED> int at_dispatch_tile(rt_device* dev, AttnArgs& a, bool paged, bool* done) {
     // rows of whole 16-byte chunks on 16-byte boundaries; 32-bit offsets of the rows of a tile, or in a page, and of pages
     const uint64_t e = sizeof(T), most = 0xffffffffull / e, far = (1ull << 31) / 64 / e;
@@ -1091,6 +1101,12 @@ template <typename T, bool SCORED> int at_dispatch_tile(rt_device* dev, AttnArgs
     for (uint64_t x : strides) fits = fits && x * e % 16 == 0;
     *done = fits;
     if (!fits) return RT_OK;
+    if constexpr (SCORED) {
+        if (at_fits_few<T>(a, paged)) {
+            const int rc = at_dispatch_few<T>(dev, a, paged, done);
+            if (rc || *done) return rc;
+        }
+    }
 #define RT_TILE(DT, EXACT) return paged ? at_launch_tile<T, DT, EXACT, true, SCORED>(dev, a, done) : at_launch_tile<T, DT, EXACT, false, SCORED>(dev, a, done)
     if (a.dim == 64) RT_TILE(64, true);
     if (a.dim == 80) RT_TILE(80, true);

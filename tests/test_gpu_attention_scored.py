@@ -102,6 +102,31 @@ def dense(dev, rng, dtype, batch, heads, kv_heads, queries, keys, dim, causal=Tr
             ref.check(got_lse[b, h], want_lse, lse_off, ("lse", b, h))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("queries, keys", [(1, 150), (1, 3000), (100, 150)])
+def test_visible_values_that_are_not_finite(dev, dtype, bad, queries, keys):
+    """a value that is seen makes its columns what it is, and others stay right"""
+    q, k, v = (ref.rounded(np.random.default_rng(1).standard_normal(s), dtype) for s in ((2, 4, queries, 64), (2, 2, keys, 64), (2, 2, keys, 64)))
+    v[0, 1, 70, 5] = bad
+    out = ref.values(dev.attention(*(ref.upload(dev, x, dtype) for x in (q, k, v)), cap=5.0, causal=False).to_numpy(), dtype)
+    clean = ref.values(dev.attention(*(ref.upload(dev, x, dtype) for x in (q, k, np.where(np.isfinite(v), v, 0.0))), cap=5.0, causal=False).to_numpy(), dtype)
+    got = out[0, 2:, :, 5]
+    assert np.isnan(got).all() if bad != bad else (got == bad).all()
+    clean[0, 2:, :, 5] = out[0, 2:, :, 5] = 0.0
+    assert np.isfinite(out).all()
+    assert (np.abs(out - clean) <= (4 * ref.HALF_STEP[dtype] + (2 * keys + 64) * U) * np.abs(np.where(np.isfinite(v), v, 0.0)).max()).all()       # (those rows are computed row by row)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, kv_heads, queries", [(16, 1, 1), (17, 1, 1), (12, 4, 1), (5, 1, 3), (8, 8, 1), (8, 8, 16), (4, 2, 8), (4, 2, 9), (3, 3, 2)])
+@pytest.mark.parametrize("dim", [64, 96, 40])
+def test_a_few_rows(dev, dtype, heads, kv_heads, queries, dim):
+    rng = np.random.default_rng(heads + queries)
+    for keys in (1, 63, 64, 65, 700, 2100):
+        dense(dev, rng, dtype, 2, heads, kv_heads, queries, keys, dim, cap=15.0, slopes=alibi(heads), window=0 if keys < 700 else 500, sinks=3)
+
+
 def alibi(heads):
     return 2.0 ** (-8.0 * np.arange(1, heads + 1) / heads)
 
@@ -170,6 +195,9 @@ def test_hidden_keys_hold_anything(dev, dtype, bad, aligned):
     # the keys of the middle document, which no query of the last one sees; and keys beyond a window behind a prefix
     dense(dev, rng, dtype, 1, 2, 2, 60, 200, 64, documents=[[0, 100, 130, 200]], change=change, cap=5.0, aligned=aligned)
     dense(dev, rng, dtype, 1, 2, 2, 40, 200, 64, window=20, prefix=[80], change=change, slopes=alibi(2), aligned=aligned)
+    # the same for a few rows
+    dense(dev, rng, dtype, 2, 4, 2, 1, 200, 64, documents=[[0, 100, 130, 200], [0, 130, 199, 200]], change=change, cap=5.0, aligned=aligned)
+    dense(dev, rng, dtype, 2, 6, 2, 3, 200, 64, window=20, prefix=[80, 3], change=change, slopes=alibi(6), aligned=aligned)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
