@@ -402,7 +402,7 @@ template <typename T, int DT, bool EXACT, bool PAGED> int at_launch_few(rt_devic
             const uint64_t w = ((uint64_t)a.window + AT_ROWS) / S::KT + 2 + ((uint64_t)a.sinks + S::KT - 1) / S::KT;
             span = w < span ? w : span;
         }
-        uint64_t piece = at_piece_for<true>(per, span * per);
+        uint64_t piece = at_piece_for<true, AF_ROWS>(per, span * per);
         piece = at_piece_of((uint32_t)(piece > span ? span : piece), (uint32_t)span);
         if ((span + piece - 1) / piece * per > (most_blocks < RT_ARRIVALS ? most_blocks : RT_ARRIVALS)) piece = span;
         part.piece = (uint32_t)piece;

@@ -42,6 +42,9 @@ template <> inline constexpr int AT_LIFT<half_t, true> = 14;
 // AT_TARGET items (Phi-2 prompt, 512 row tiles: 45 us whole, 55 to 57 shared out; chunks, 320 row tiles: 152 us at 256 items, 125 at 768, 142 at 1536;
 // encoder, 288: 202, 149, 140).
 constexpr uint32_t AT_TARGET_FEW = 1024, AT_TARGET = 768, AT_ENOUGH = 512, AT_LEAST_TILES_FEW = 2, AT_LEAST_TILES = 4;
+// Blocks of 16 rows of 128 columns that the chip holds at once, two a CU.  Four sequences of up to 6000 keys, 8 KV heads: 22 us in one round of pieces of four tiles, 31 in two of
+// pieces of two; one of 1000 keys 13 us in pieces of two, 17 of four; of 6000 20 and 19
+constexpr uint32_t AT_AT_ONCE = 512;
 constexpr uint32_t AT_SHORT = 40;                // tiles of keys to a row tile
 constexpr size_t AT_MOST_PARTS = 1u << 30;       // bytes of parts; a launch that would leave more shares nothing out
 constexpr uint32_t AT_MOST_PIECES = 60;          // of a row tile: their factors for its 128 rows fit the LDS of the smallest tiles
@@ -74,10 +77,14 @@ template <typename T> __device__ __forceinline__ T at_wave_sum(T x) {
 }
 
 // Tiles in a piece of the keys, for `tiles` row tiles in all that have `work` tiles of keys to walk
-template <bool FEW> __host__ __device__ __forceinline__ uint32_t at_piece_for(uint64_t tiles, uint64_t work) {
+template <bool FEW, uint32_t ROWS> __host__ __device__ __forceinline__ uint32_t at_piece_for(uint64_t tiles, uint64_t work) {
     if (!FEW && tiles >= AT_ENOUGH) return 0x7fffffffu;
     constexpr uint32_t target = FEW ? AT_TARGET_FEW : AT_TARGET, least = FEW ? AT_LEAST_TILES_FEW : AT_LEAST_TILES;
-    const uint64_t n = (work + target - 1) / target;
+    uint64_t n = (work + target - 1) / target;
+    if (ROWS != AT_ROWS && n < 4) {                             // blocks of 16 rows: as many as the chip holds at once, while that asks for no more than four tiles
+        const uint64_t once = (work + AT_AT_ONCE - 1) / AT_AT_ONCE;
+        n = once < 4 ? once : 4;
+    }
     return n < least ? least : n > 0x7fffffffu ? 0x7fffffffu : (uint32_t)n;
 }
 // The same from the device's lengths; the same in every wave.
@@ -90,7 +97,7 @@ template <int KT, bool FEW, bool SCORED, uint32_t ROWS> __device__ __forceinline
         work += (uint64_t)at_row_tiles<ROWS>(a, s) * (span > 2 * less ? span - less : (span + 1) / 2);
         tiles += at_row_tiles<ROWS>(a, s);
     }
-    return at_piece_for<FEW>((uint64_t)at_wave_sum(tiles) * a.kv_heads, at_wave_sum(work) * a.kv_heads);
+    return at_piece_for<FEW, ROWS>((uint64_t)at_wave_sum(tiles) * a.kv_heads, at_wave_sum(work) * a.kv_heads);
 }
 // ... and in a piece of this sequence's: pieces of the same size
 __host__ __device__ __forceinline__ uint32_t at_piece_of(uint32_t piece, uint32_t span) {
@@ -248,12 +255,13 @@ __device__ __forceinline__ float at_other(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------------- shape
-// Head dims up to DT columns; EXACT: DT itself, known to the compiler.
-template <typename T, int DT> struct AtShape {
+// Head dims up to DT columns; EXACT: DT itself, known to the compiler.  WIDE: 64 keys to a tile whatever the columns: half as many steps, whose barriers, maxima and waits a
+// single wave of a SIMD hides from nobody (16 capped heads of 256, 4096 tokens with a window of 2048, f16: 268 -> 224 us), where the registers let
+template <typename T, int DT, bool WIDE = false> struct AtShape {
     static constexpr int CE = 16 / sizeof(T);                  // elements of a chunk
     static constexpr int STEPS = (DT + 2 * CE - 1) / (2 * CE); // pairs of chunks in a row
     static constexpr int BLOCKS = (DT + 31) / 32;              // 32-column blocks of the result
-    static constexpr int KT = sizeof(T) == 2 && DT <= 128 ? 64 : 32;
+    static constexpr int KT = sizeof(T) == 2 && (DT <= 128 || WIDE) ? 64 : 32;
     static constexpr int HALVES = KT / 32;
     // Sums that a score is kept in while it grows: a f32 product adds two columns at a time, and 128 additions in a row lose twice what 32 do (a 16-bit one adds 16)
     static constexpr int SUMS = sizeof(T) == 2 || DT <= 64 ? 1 : DT <= 128 ? 2 : 4;
@@ -512,7 +520,7 @@ __device__ __forceinline__ void at_again(const AttnArgs& a, const AttnPartial& p
 // wanted.  Waves of a SIMD: as many as the registers let, four where the rows have 64 columns and no page table is followed (encoder in f32: 146.5 us a call, with three 148.7)
 template <typename T, int DT, bool EXACT, bool PAGED, bool FEW, bool SCORED>
 __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW && !SCORED), AtShape<T, DT>::WAVES + (DT <= 64 && EXACT && !PAGED && !FEW && !SCORED)))) attention_tile_kernel(AttnArgs a, AttnPartial part) {
-    typedef AtShape<T, DT> S;
+    typedef AtShape<T, DT, SCORED && EXACT> S;
     constexpr int KT = S::KT, CE = S::CE;
     constexpr float LIFT = AT_LIFT<T, FEW>, LOWER = 1.0f / (1 << AT_LIFT<T, FEW>);              // the weights' factor is 2^LIFT, 1 / LOWER
     constexpr int SUMS = sizeof(T) == 4 && (PAGED || FEW) ? (S::SUMS > 2 ? S::SUMS : 2) : S::SUMS;  // 64 columns have registers for two where three waves share them
@@ -787,20 +795,19 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
                         for (int e = 0; e < 16; e++) x[kk][e] = at_capped<T>(a.most, x[kk][e] * most_in);
                 }
             }
+            if (a.most == 0.0f) {
+                const float cc = __builtin_fabsf(a.c);
+#pragma unroll
+                for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[kk][e] *= cc;
+            }
             if (a.slopes) {
-                const float far = (float)(p - t0 - 4 * (int32_t)half), cc = a.most != 0.0f ? 1.0f : __builtin_fabsf(a.c);    // distance of the tile's first key of this half
-                if (a.causal && !a.prefix) {                    // keys behind the query are hidden: the distance has no other sign
-                    const float first = -slope * far;
+                const float far = (float)(p - t0 - 4 * (int32_t)half);          // distance of the tile's first key of this half
 #pragma unroll
-                    for (int kk = 0; kk < S::HALVES; kk++)
+                for (int kk = 0; kk < S::HALVES; kk++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(x[kk][e], cc, __builtin_fmaf((float)(32 * kk + e % 4 + 8 * (e / 4)), slope, first));
-                } else {
-#pragma unroll
-                    for (int kk = 0; kk < S::HALVES; kk++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(-slope, __builtin_fabsf(far - (float)(32 * kk + e % 4 + 8 * (e / 4))), x[kk][e] * cc);
-                }
+                    for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(-slope, __builtin_fabsf(far - (float)(32 * kk + e % 4 + 8 * (e / 4))), x[kk][e]);
             }
         }
         if (t0 + KT - 1 > limit_a || (SCORED && !PAGED && t0 < lo_z) || (t0 + KT > (SCORED ? front_a : a.sinks) && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
@@ -1020,7 +1027,7 @@ template <typename T, int KT, bool PAGED, bool SCORED> __global__ void __launch_
 }
 
 template <typename T, int DT, bool EXACT, bool PAGED, bool SCORED> int at_launch_tile(rt_device* dev, AttnArgs& a, bool* done) {
-    typedef AtShape<T, DT> S;
+    typedef AtShape<T, DT, SCORED && EXACT> S;
     AttnPartial part = {};
     const bool few = (uint64_t)a.tokens * a.group <= (uint64_t)AT_FEW_ROWS * (PAGED ? a.seqs : 1);
     const uint64_t most_blocks = AT_MOST_PARTS / (AT_ROWS * ((uint64_t)a.dim + 2) * sizeof(float));
@@ -1044,7 +1051,7 @@ template <typename T, int DT, bool EXACT, bool PAGED, bool SCORED> int at_launch
         }
         const uint64_t less = a.causal ? a.tokens / (2 * S::KT) : 0, mean = span > 2 * less ? span - less : (span + 1) / 2;
         const uint64_t tiles = part.row_tiles * per;
-        uint64_t piece = few ? at_piece_for<true>(tiles, mean * tiles) : at_piece_for<false>(tiles, mean * tiles);
+        uint64_t piece = few ? at_piece_for<true, AT_ROWS>(tiles, mean * tiles) : at_piece_for<false, AT_ROWS>(tiles, mean * tiles);
         // a block to each CU and short walks of 16-bit tiles, one to two microseconds each: parts and their joining cost more than the CUs that end early leave idle.
         // 32 heads of 64, 96 and 128, whole | shared out, us: causal 1024 tokens 21, 25, 29 | 27, 29, 40; 1024 of 2048 keys, all visible 40, 48, 58 | 40, 51, 71; of
         // 2560 47, 58, 72 | 46, 58, 82; of 4096 74, 88, 110 | 69, 89, 116; 8 heads, causal 4096 67, 78, 93 | 45, 62, 82.  A f32 tile takes four times as long
