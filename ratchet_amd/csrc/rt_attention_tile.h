@@ -602,7 +602,6 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         limit = at_limit(a, s, j); limit_a = at_limit(a, s, ja); limit_z = at_limit(a, s, jz);
         p = at_position(s, j); p_a = at_position(s, ja); p_z = at_position(s, jz);
     }
-    const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
 
     v4u q[S::STEPS];
     {
@@ -616,8 +615,10 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         }
     }
     // |scale| log2 e; never 0, so that a hidden key's -inf stays
-    const bool changed = SCORED && (a.most != 0.0f || a.slopes);
+    // capped scores are in units of log2 e from there on; others get their bias in units of the products, divided by c, which then need no product of their own (unless c is next to 0)
+    const bool changed = SCORED && (a.most != 0.0f || (a.slopes && __builtin_fabsf(a.c) < 0x1p-40f));
     const float c = changed ? 1.0f : fmaxf(__builtin_fabsf(a.c), 1e-37f);
+    const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f / c : 0.0f;
 
     // ---- this lane's part of a tile's loads: LDS chunk `slot` belongs to row slot / chunks
     uint32_t l_row[S::LOADS], l_k[S::LOADS], l_v[S::LOADS];
@@ -802,13 +803,13 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
 #pragma unroll
                     for (int e = 0; e < 16; e++) x[kk][e] *= cc;
             }
-            if (a.slopes) {
-                const float far = (float)(p - t0 - 4 * (int32_t)half);          // distance of the tile's first key of this half
+        }
+        if (SCORED && a.slopes) {
+            const float far = (float)(p - t0 - 4 * (int32_t)half);              // distance of the tile's first key of this half
 #pragma unroll
-                for (int kk = 0; kk < S::HALVES; kk++)
+            for (int kk = 0; kk < S::HALVES; kk++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(-slope, __builtin_fabsf(far - (float)(32 * kk + e % 4 + 8 * (e / 4))), x[kk][e]);
-            }
+                for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(-slope, __builtin_fabsf(far - (float)(32 * kk + e % 4 + 8 * (e / 4))), x[kk][e]);
         }
         if (t0 + KT - 1 > limit_a || (SCORED && !PAGED && t0 < lo_z) || (t0 + KT > (SCORED ? front_a : a.sinks) && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
             // key t = 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile: p - t < window as t > p - window, which saturates where there is no window

@@ -147,6 +147,10 @@ template <typename T, int VB, bool INTER, bool PAGED> __global__ void __launch_b
         }
     };
     load(0);
+    // the first frequency of each thread is on its way while the tokens are found
+    uint32_t t_first = 0, i_first = 0;
+    fd_divmod(tid, a.half_div, t_first, i_first);
+    uint64_t turn = tid < ntok * a.half ? a.turns[i_first] : 0;
     if (PAGED) {
         for (uint32_t t = tid / 64; t < ntok; t += BLOCK / 64) {
             const Place p = find_place(a, first + t);
@@ -157,9 +161,10 @@ template <typename T, int VB, bool INTER, bool PAGED> __global__ void __launch_b
     for (uint32_t n = tid; n < ntok * a.half; n += BLOCK) {
         uint32_t t, i;
         fd_divmod(n, a.half_div, t, i);
+        if (n != tid) turn = a.turns[i];
         const int64_t position = PAGED ? s_place[t].position : a.positions[first + t];
         float sn, cs;
-        sincos_turn((uint64_t)position * a.turns[i], sn, cs);
+        sincos_turn((uint64_t)position * turn, sn, cs);
         s_sn[n] = sn * a.factor;
         s_cs[n] = cs * a.factor;
     }

@@ -407,15 +407,13 @@ template <typename T> struct Row {
 
     // A bound that at least k <= 1024 logits reach: of each wave the (k / 16)th largest of the lanes' own maxima, and of those the least.  -inf if some wave has fewer
     __device__ __forceinline__ float reached_by(uint32_t k, float mine) {
-        float x = mine;
+        // bit by bit from the top, the largest key that so many lanes reach
+        const uint32_t key = key_of(mine), most = (k + WAVES - 1) / WAVES;
+        uint32_t low = 0;
 #pragma unroll 1
-        for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll 1
-            for (int stride = size / 2; stride; stride >>= 1) {
-                const float other = __shfl_xor(x, stride);
-                x = ((lane & stride) == 0) == ((lane & size) == 0) ? fmaxf(x, other) : fminf(x, other);
-            }
-        uint32_t low = key_of(__shfl(x, (int)((k + WAVES - 1) / WAVES) - 1)), high = low;
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1)
+            if ((uint32_t)__popcll(__ballot(key >= (low | bit))) >= most) low |= bit;
+        uint32_t high = low;
         key_range(low, high);
         return of_key(low);
     }
@@ -499,7 +497,8 @@ template <typename T> __global__ void __launch_bounds__(BLOCK) sample_kernel(Sam
             floor = p > 0.0f ? r.max - temperature * 0.7f * __builtin_amdgcn_logf(2.0f * (float)a.vocab / (1.0f - p)) : r.max;
         }
         floor = fmaxf(floor, -3.4028235e38f);                   // (of an endless temperature: all that are finite)
-        auto in = [&](float x, int32_t i) -> bool { return x >= floor && front.keeps(x, i); };
+        const bool all = front.x == -INFINITY;                  // nothing is cut yet: what is not finite weighs 0 and lies below the floor
+        auto in = [&](float x, int32_t i) -> bool { return x >= floor && (all || front.keeps(x, i)); };
         if (counts && (uint32_t)k <= LIST / 4) {
             r.clear();
             r.each([&](float x, int32_t i) {
@@ -521,7 +520,7 @@ template <typename T> __global__ void __launch_bounds__(BLOCK) sample_kernel(Sam
         r.clear();
         uint64_t sum = 0;
         r.each([&](float x, int32_t i) {
-            if (front.keeps(x, i)) {
+            if (all || front.keeps(x, i)) {
                 const uint64_t w = metric(x);
                 sum += w;
                 if (x >= floor) atomicAdd((unsigned long long*)&s.hist[bin_of(x)], (unsigned long long)w);
@@ -533,13 +532,17 @@ template <typename T> __global__ void __launch_bounds__(BLOCK) sample_kernel(Sam
         const uint32_t bin = s.bin;
         const uint64_t before = s.before;
         if (bin == BINS) continue;                              // fewer than k
+        // the step's ends, half a step out (a rounded end passes no logit that the end itself does not): few logits lie between them
+        const float width = 1.0f / per;
+        const bool narrow = per > 0x1p-64f && per < 0x1p64f;
+        const float above = bin > 0 && narrow ? r.max - ((float)bin - 0.5f) * width : INFINITY, below = bin < BINS - 1 && narrow ? r.max - ((float)bin + 1.5f) * width : floor;
         r.each([&](float x, int32_t i) {
-            if (in(x, i) && bin_of(x) == bin) r.list(x, i);
+            if (x >= below && x <= above && in(x, i) && bin_of(x) == bin) r.list(x, i);
         });
         cut = r.cut_in_step(before, want, [&](float x, int32_t i) -> bool { return in(x, i) && bin_of(x) == bin; }, metric);
     }
     auto kept = [&](float x, int32_t i) -> uint64_t {
-        if (!cut.keeps(x, i)) return 0;
+        if (!(x >= cut.x) || !cut.keeps(x, i)) return 0;        // most fail the first
         const double w = r.weight(x);
         return w >= min_p ? r.fixed(w) : 0;
     };
