@@ -213,3 +213,26 @@ def test_recorded(dev):
         graph.launch()
         got = out.to_numpy()
         assert np.array_equal(dev.sample(x, u, None, k, p).to_numpy(), got)
+
+
+@pytest.mark.parametrize("dtype, vocab", [("f32", 1000003), ("f16", 1 << 24), ("bf16", 3000001)])
+def test_large_vocabularies(dev, dtype, vocab):
+    rng = np.random.default_rng(14)
+    x = ref.rounded(rng.standard_normal((2, vocab)) * 3, dtype)
+    u = rng.random(2)
+    for settings in (dict(), dict(k=100), dict(p=0.5), dict(k=20000, p=0.9, min_p=1e-4), dict(temperature=0.0)):
+        run(dev, x, dtype, u, **settings)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_twice_is_the_same(dev, dtype):
+    """lists fill in any order, and sums add up in any: the bits of tokens and shares do not change"""
+    rng = np.random.default_rng(15)
+    x, u = ref.upload(dev, logits(rng, 64, 30011, dtype), dtype), dev.upload(rng.random(64).astype(np.float32))
+    p, k = dev.upload(np.full(64, 0.95, np.float32)), dev.upload(rng.integers(1, 3000, 64).astype(np.int32))
+    for settings in (dict(), dict(top_p=p), dict(top_k=k), dict(top_k=k, top_p=p)):
+        probs = dev.empty((64,), _lib.F32)
+        first = dev.sample(x, u, probs=probs, **settings).to_numpy(), probs.to_numpy()
+        for _ in range(5):
+            again = dev.sample(x, u, probs=probs, **settings).to_numpy(), probs.to_numpy()
+            assert np.array_equal(again[0], first[0]) and np.array_equal(again[1], first[1])
