@@ -188,19 +188,27 @@ template <bool SCORED> __device__ __forceinline__ bool at_sees(const AttnArgs& a
     return t <= r.limit && (!SCORED || t >= r.lo) && (r.p - t < a.window || t < r.front);
 }
 
-// cap * tanh(z / cap) in units of log2(e), y = z / cap: tanh y = 1 - 2 / (e^2y + 1), off by about 2^-23 of the cap, which is less than a 16-bit weight's rounding.
-// In f32 the small ones, whose differences that would swamp, take the odd series up to y^9 (below 0.3 the next term is under 6e-8 of it).
-template <typename T> __device__ __forceinline__ float at_capped(float cap, float y) {
-    const float t = __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * 2.885390081777927f) + 1.0f), cap);
-    if (sizeof(T) == 2) return t;
+// cap * tanh(z / cap) in units of log2(e), y = z / cap: tanh y = 1 - 2 / (e^2y + 1), off by less than 2^-21 of the cap.  For a cap up to AT_COARSE that is less than a 16-bit
+// weight's rounding; for a larger one it is too much of small ones, and FINE ones below 1/8 take the series to y^5, 2^-22 of it off at most.
+// In f32 the exponential of |y|, with a Newton step for the reciprocal, is off by 2^-22 at most, and those below 1/2 take the polynomial through tanh's values at Chebyshev's
+// points of y^2 <= 1/4, 2^-26 of it off at most.
+constexpr float AT_COARSE = 1024.0f;               // in units of log2(e)
+template <typename T, bool FINE> __device__ __forceinline__ float at_capped(float cap, float y) {
     const float z = y * y;
-    const float near = cap * __builtin_fmaf(y * z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 62.0f / 2835, -17.0f / 315), 2.0f / 15), -1.0f / 3), y);
-    return __builtin_fabsf(y) < 0.3f ? near : t;
+    if (sizeof(T) == 2) {
+        const float t = __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * 2.885390081777927f) + 1.0f), cap);
+        return FINE && __builtin_fabsf(y) < 0.125f ? cap * y * __builtin_fmaf(z, __builtin_fmaf(z, 2.0f / 15, -1.0f / 3), 1.0f) : t;
+    }
+    const float d = __builtin_amdgcn_exp2f(__builtin_fabsf(y) * 2.885390081777927f) + 1.0f, near_r = __builtin_amdgcn_rcpf(d);
+    const float r = d < 0x1p100f ? near_r * __builtin_fmaf(-d, near_r, 2.0f) : 0.0f;
+    const float t = __builtin_copysignf(__builtin_fmaf(-2.0f * cap, r, cap), y);
+    const float near = cap * (y * __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 0.017131344f, -0.052984239f), 0.133247505f), -0.33333068f), 0.99999999f));
+    return __builtin_fabsf(y) < 0.5f ? near : t;
 }
 // The score, in units of log2(e), of a product q.k; slope: in the same units
 template <typename T, bool SCORED> __device__ __forceinline__ float at_changed(const AttnArgs& a, float dot, float slope, int32_t distance) {
     if (!SCORED) return dot * a.c;
-    float x = a.most != 0.0f ? at_capped<T>(a.most, dot * a.most_in) : dot * a.c;
+    float x = a.most != 0.0f ? at_capped<T, true>(a.most, dot * a.most_in) : dot * a.c;
     if (a.slopes) x = __builtin_fmaf(-slope, __builtin_fabsf((float)distance), x);
     return x;
 }

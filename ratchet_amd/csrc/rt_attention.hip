@@ -196,15 +196,20 @@ int score_rules(const char* who, const rt_scores* scores, float scale, uint32_t 
     a.scored = scores->cap != 0.0f || scores->slopes || scores->documents || scores->prefix;       // else it is attention as it ever was
     a.most = scores->cap * 1.4426950408889634f;
     a.most_in = scores->cap != 0.0f ? scale / scores->cap : 0.0f;
-    // tanh y = y (t0 + t1 y^2 + t2 y^4 + t3 y^6), through its values at Chebyshev's points of y^2 <= 0.16 and 1e-7 of it off at most.  Only where no power of
-    // scale / cap leaves f32's range
+    // tanh y = y (t0 + t1 y^2 + t2 y^4 + t3 y^6), through its values at Chebyshev's points of y^2 <= 0.16 and 1e-7 of it off at most.  Where k^6 is too small for f32, y - y^3 / 3,
+    // 2^-23 of it off below 2^-5.  Only where no power of scale / cap leaves f32's range
     const float k = a.most_in < 0.0f ? -a.most_in : a.most_in;
     a.near_limit = -1.0f;
-    if (k > 0x1p-16f && k < 0x1p16f && a.most > 0x1p-16f && a.most < 0x1p16f) {
+    if (k > 0x1p-19f && k < 0x1p16f && a.most > 0x1p-16f && (a.most < 0x1p16f || k < 1.0f)) {
         static const double tanh_terms[4] = {0.9999999013476046, -0.3333135628726226, 0.1327087433318406, -0.04754934670684051};
         double power = (double)a.most * k;
         for (int i = 0; i < 4; i++, power *= (double)k * k) a.near[i] = (float)(tanh_terms[i] * power);
         a.near_limit = 0.4f / k;
+    } else if (k > 0.0f && k <= 0x1p-19f && a.most > 1.0f) {
+        const double c = (double)a.most * k;
+        a.near[0] = (float)c;
+        a.near[1] = (float)(-c * k * k / 3);
+        a.near_limit = k > 0x1p-55f ? 0x1p-5f / k : 0x1p50f;
     }
     a.slopes = scores->slopes;
     a.documents = scores->documents;

@@ -233,8 +233,17 @@ __global__ void __launch_bounds__(AT_BLOCK) attention_few_kernel(AttnArgs a, Att
         if (changed) {
             if (a.most != 0.0f) {
                 const float most_in = __builtin_fabsf(a.most_in);
+                if (sizeof(T) == 4 || a.most > AT_COARSE) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = at_capped<T>(a.most, x[e] * most_in);
+                    for (int e = 0; e < 4; e++) {
+                        float y = x[e] * most_in;
+                        if (sizeof(T) == 2) asm volatile("" : "+v"(y));   // shares nothing with the others
+                        x[e] = at_capped<T, true>(a.most, y);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = at_capped<T, false>(a.most, x[e] * most_in);
+                }
             } else {
                 const float cc = __builtin_fabsf(a.c);
 #pragma unroll

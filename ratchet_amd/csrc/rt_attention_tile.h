@@ -790,10 +790,11 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
                         }
                 } else {
                     const float most_in = __builtin_fabsf(a.most_in);
+                    if (sizeof(T) == 2 && a.most > AT_COARSE) l = __builtin_nanf("");             // computed again, a row at a time (with FINE ones here as well, 80 columns took 14 % more)
 #pragma unroll
                     for (int kk = 0; kk < S::HALVES; kk++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) x[kk][e] = at_capped<T>(a.most, x[kk][e] * most_in);
+                        for (int e = 0; e < 16; e++) x[kk][e] = at_capped<T, sizeof(T) == 4>(a.most, x[kk][e] * most_in);
                 }
             }
             if (a.most == 0.0f) {

@@ -2,8 +2,9 @@
 
 Bounds are attention_ref.py's with a score's error made larger by what is done to it (u = 2^-24): tanh has a slope of at most 1, and computed as 1 - 2 / (e^2y + 1) it is off by
 2u |y| (1 - tanh^2) < u from the two products that make its argument, u from the exponential (off by 2u), 2u from the sum, 4u from the reciprocal (off by 2u) and u from the last
-operation, in all 9u, with the cap's own rounding and that of log2(e) less than 12u of the cap; in f32 below 0.3 the series leaves out 6e-8 = u of it at most.  A bias is
-off by the roundings of slope * log2(e), of the distance and of the sum, 4u of it and of the score."""
+operation, in all 9u, with the cap's own rounding and that of log2(e) less than 12u of the cap.  In f32, and for a cap
+above 1024 ln 2, a score below an eighth of the cap is a series or a polynomial of it, off by less than 16u of itself: 4u for what is left out, six roundings of a value and
+four of constants.  A bias is off by the roundings of slope * log2(e), of the distance and of the sum, 4u of it and of the score."""
 import numpy as np
 import pytest
 
@@ -36,8 +37,10 @@ def head(q, k, v, see, scale, dtype, cap=0.0, slope=0.0, distance=None):
     s = (q @ k0.T) * scale
     mass = np.where(see, np.abs(q) @ np.abs(k0).T, 0.0).max(axis=1) * abs(scale) * (d + 16) * U
     if cap:
+        near = cap / 8 if dtype == "f32" or cap > 1024 / np.log2(np.e) else 0.0
+        small = np.where(see & (np.abs(s) < near), np.minimum(12 * U * cap, 16 * U * np.abs(s)), np.where(see & (np.abs(s) < np.inf), 12 * U * cap, 0.0)).max(axis=1)
         s = cap * np.tanh(s / cap)
-        mass = mass + 12 * U * cap
+        mass = mass + small
     if slope:
         bias = slope * np.abs(distance)
         s = s - bias
@@ -135,7 +138,7 @@ def alibi(heads):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("cap, biased", [(5.0, False), (50.0, False), (0.0, True), (20.0, True), (1e-3, False), (1e30, False)])
+@pytest.mark.parametrize("cap, biased", [(5.0, False), (50.0, False), (0.0, True), (20.0, True), (1e-3, False), (300.0, False), (1e4, True), (1e30, False)])
 @pytest.mark.parametrize("queries, keys, causal", [(1, 1, True), (1, 777, True), (3, 65, False), (130, 300, True), (64, 64, True), (5, 3, True), (200, 90, False)])
 def test_cap_and_bias(dev, dtype, cap, biased, queries, keys, causal):
     dense(dev, np.random.default_rng(keys), dtype, 2, 4, 2, queries, keys, 64, causal=causal, cap=cap, slopes=alibi(4) if biased else None)
@@ -201,6 +204,20 @@ def test_hidden_keys_hold_anything(dev, dtype, bad, aligned):
     # the same for a few rows
     dense(dev, rng, dtype, 2, 4, 2, 1, 200, 64, documents=[[0, 100, 130, 200], [0, 130, 199, 200]], change=change, cap=5.0, aligned=aligned)
     dense(dev, rng, dtype, 2, 6, 2, 3, 200, 64, window=20, prefix=[80, 3], change=change, slopes=alibi(6), aligned=aligned)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cap", [1e3, 3e4, 1e6, 1e12, 1e18])
+def test_a_large_cap_that_one_row_reaches(dev, dtype, cap):
+    """next to rows whose scores are ordinary: every 16th query's first column is about the cap, as far as the type holds it"""
+    def change(q, k, v):
+        most = min(cap, 3e4) if dtype == "f16" else cap
+        q[0, 0, 3::16, 0] = np.float32(2.0 ** np.floor(np.log2(most)))
+        k[0, 0, 5::7, 0] = 4.0
+        k[0, 0, 6::7, 0] = -4.0
+    dense(dev, np.random.default_rng(5), dtype, 1, 2, 1, 90, 130, 64, cap=cap, change=change)
+    dense(dev, np.random.default_rng(5), dtype, 1, 2, 1, 5, 130, 64, cap=cap, change=change)
+    dense(dev, np.random.default_rng(5), dtype, 1, 2, 1, 40, 70, 20, cap=cap, change=change, aligned=False)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
