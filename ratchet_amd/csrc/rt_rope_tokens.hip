@@ -8,17 +8,19 @@
 // What is left of the nearest quarter turn, at most an eighth, becomes a float (relative error 2^-24) and goes through the Taylor series of sine and cosine, to x^9 and x^10:
 // the terms left out are below 2e-9.  So far positions are as good as near ones, and a negative position turns back.
 //
-// What bounds it: memory.  A block owns some tokens, computes a sine and cosine of each (token, frequency) once, one to a thread, into LDS, and its threads then turn two
-// vectors each of all heads, whose loads are in flight before the sines.
+// What bounds it: memory.  A block owns some tokens, computes a sine and cosine of each (token, frequency) once, into LDS, and its threads then turn two vectors each of all
+// heads, whose loads are in flight before the sines.  f16, 8192 tokens of 64 heads of 96 columns: 41 us, 4.9 TB/s, what a copy reaches.  What a step adds is little next to a
+// launch: 64 tokens of 40 heads of 128 columns 5 us, with the cache (the token's sequence, its length and page come one after the other) 6.
 #include <math.h>
+
+#include <algorithm>
 
 #include "rt_attention.h"
 
 namespace {
 
 constexpr int BLOCK = 256, TRIP = 2;              // units of two vectors that a thread has in flight
-constexpr uint32_t MOST_HALF = 512;               // frequencies: LDS for one token's
-constexpr uint32_t MOST_AT_ONCE = BLOCK;          // (token, frequency) pairs of a block with more than one token
+constexpr uint32_t PAIRS = 1024;                  // (token, frequency) pairs of a block: LDS for their sines and cosines
 constexpr uint32_t GRID_ROW = 1u << 22;           // blocks to a row of the grid: an extent of a launch has fewer than 2^32 threads
 
 struct RopeRows {
@@ -93,8 +95,8 @@ template <typename T, int VB> union Vec {
 template <typename T, int VB, bool INTER, bool PAGED> __global__ void __launch_bounds__(BLOCK) rope_tokens_kernel(RopeRows a) {
     constexpr int VE = VB / sizeof(T);
     typedef typename VecOf<VB>::type V;
-    __shared__ float s_sn[MOST_HALF], s_cs[MOST_HALF];
-    __shared__ Place s_place[PAGED ? MOST_AT_ONCE : 1];
+    __shared__ float s_sn[PAIRS], s_cs[PAIRS];
+    __shared__ Place s_place[PAGED ? BLOCK : 1];
     const uint32_t tid = threadIdx.x;
     uint32_t block, chunk;
     fd_divmod(blockIdx.y * GRID_ROW + blockIdx.x, a.chunk_div, block, chunk);
@@ -258,9 +260,12 @@ int run(rt_device* dev, int dt, RopeRows& a, uint32_t dim, uint32_t head_dim, bo
     const uint32_t heads = a.heads[0] + a.heads[1] + a.heads[2];
     const uint64_t row_units = (uint64_t)heads * a.units;
     RT_REQUIRE(row_units < 1ull << 31, RT_ERR_SIZE, "rope: rows of %u heads of %u columns", heads, head_dim);
-    a.ntok = 1;
+    // Tokens of few heads share a block, a unit to a thread, as far as there are blocks for all CUs.  f16, one token to a block | several: 65536 tokens of a head of 64 columns
+    // 50 us | 8, of 8 heads of 128 57 | 41, 8192 of a head of 128 8.8 | 4.2, cache and all for 16 pieces of 1000 tokens of 1 + 1 heads of 40 19 | 7; two units to a thread
+    // 41 | 43 for 8 heads, and a block's sines in 2 KB of LDS in place of 8 14 us for 65536 tokens of a head of 128 in place of 13.
+    a.ntok = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({PAIRS / a.half, BLOCK / row_units, a.tokens / (uint32_t)dev->num_cus}));
     a.head_chunk = heads;
-    if (row_units * a.tokens < 2ull * dev->num_cus * BLOCK) {
+    if (a.ntok == 1 && row_units * a.tokens < 2ull * dev->num_cus * BLOCK) {
         const uint32_t per = BLOCK / a.units > 1 ? BLOCK / a.units : 1;           // few tokens: a unit to a thread, blocks share a token's heads
         a.head_chunk = per < heads ? per : heads;
     }
@@ -292,7 +297,7 @@ int table_rules(const char* who, int dt, uint32_t head_dim, const uint64_t* turn
     RT_REQUIRE(rt_is_float_dt(dt), RT_ERR_DTYPE, "%s: dtype %d is not F32, F16 or BF16", who, dt);
     RT_REQUIRE(head_dim > 0, RT_ERR_SHAPE, "%s: zero extent", who);
     RT_REQUIRE(dim > 0 && dim % 2 == 0 && dim <= head_dim, RT_ERR_SHAPE, "%s: dim %u must be positive, even and <= %u", who, dim, head_dim);
-    RT_REQUIRE(dim / 2 <= MOST_HALF && head_dim <= 1u << 16, RT_ERR_SIZE, "%s: %u of %u columns", who, dim, head_dim);
+    RT_REQUIRE(dim / 2 <= PAIRS && head_dim <= 1u << 16, RT_ERR_SIZE, "%s: %u of %u columns", who, dim, head_dim);
     RT_REQUIRE(isfinite(factor), RT_ERR_ARG, "%s: factor is not finite", who);
     RT_REQUIRE(interleaved == 0 || interleaved == 1, RT_ERR_ARG, "%s: interleaved is %d", who, interleaved);
     RT_REQUIRE(turns, RT_ERR_NULL_POINTER, "%s: NULL table", who);

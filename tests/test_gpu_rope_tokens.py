@@ -3,12 +3,15 @@
 Bound (u = 2^-24): the angle, less than an eighth of a turn of it, is rounded as a float and times 2 pi, 2u of at most 0.79 in all; the series' terms add less than 1.2u of 1;
 the factor rounds once more: a sine or cosine is off by less than 4u, times |factor|.  Each of two products takes that and a rounding, their sum one more:
 6u |factor| (|x1| + |x2|), and what is stored is rounded to the type (half a step)."""
+import ctypes
+
 import numpy as np
 import pytest
 
 import attention_ref as ref
 from attention_ref import HALF_STEP, TINY, U
 from ratchet_amd import _lib, rope_divisors
+from ratchet_amd._lib import check
 
 pytestmark = pytest.mark.gpu
 DTYPES = ["f32", "f16", "bf16"]
@@ -41,7 +44,10 @@ def turned(x, positions, dim, base, divisors, factor, interleaved, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("tokens, heads, head_dim, dim", [(1, 1, 2, 2), (1, 40, 128, 128), (64, 40, 128, 128), (7, 3, 80, 32), (5, 2, 96, 96), (9, 5, 64, 48), (3, 4, 20, 10), (17, 3, 7, 6),
-                                                          (2, 2, 256, 64), (3, 1, 1024, 1024), (300, 6, 40, 16), (2, 3, 24, 8), (33, 130, 64, 64), (4, 2, 72, 24)])
+                                                          (2, 2, 256, 64), (3, 1, 1024, 1024), (300, 6, 40, 16), (2, 3, 24, 8), (33, 130, 64, 64), (4, 2, 72, 24),
+                                                          # several tokens to a block, the last one's fewer
+                                                          (1500, 1, 64, 64), (2001, 2, 96, 32), (1111, 3, 20, 8), (70001, 1, 2, 2), (3001, 1, 7, 6), (1300, 5, 40, 40), (515, 1, 1024, 1024),
+                                                          (6000, 1, 128, 128)])
 def test_shapes(dev, dtype, interleaved, tokens, heads, head_dim, dim):
     rng = np.random.default_rng(tokens + head_dim + dim)
     x, positions = ref.rounded(rng.standard_normal((tokens, heads, head_dim)), dtype), rng.integers(0, 5000, tokens).astype(np.int32)
@@ -121,14 +127,22 @@ def test_many_tokens(dev):
         ref.check(out[s], want, off, "many")
 
 
-@pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("heads, kv_heads, d, dim", [(4, 2, 64, 64), (3, 1, 20, 8), (8, 8, 80, 32), (2, 2, 7, 6), (40, 8, 128, 128)])
-@pytest.mark.parametrize("page", [16, 7, 1])
-def test_into_the_cache(dev, dtype, interleaved, heads, kv_heads, d, dim, page):
-    rng = np.random.default_rng(d + page)
-    # a first token, a prompt, a later piece, nothing, a page that is missing, more new tokens than lens counts, tokens beyond the table
-    p = ref.Paged(rng, dtype, heads, kv_heads, d, page, [1, 50, 40, 20, 40, 2, 33], [1, 50, 7, 0, 5, 4, 2], holes=[(4, 38 // page)], spare=0)
+def test_many_tokens_of_many_heads(dev):
+    """a token to a block, more than a row of the grid has; all tokens are one row, 2.2 GB of results"""
+    n, heads = (1 << 22) + 1001, 130
+    x = np.random.default_rng(4).standard_normal((1, heads, 2)).astype(np.float16)
+    positions = (np.arange(n) % 5000).astype(np.int32)
+    row, at, table, out = dev.upload(x), dev.upload(positions), dev.rope_table(2), dev.empty((n, heads, 2), _lib.F16)
+    strides = (ctypes.c_uint64 * 2)(0, 2)
+    check(dev.lib.rt_rope_tokens(dev.handle, _lib.F16, row.ptr, strides, out.ptr, None, n, heads, 2, at.ptr, table.ptr, 2, 1.0, 0))
+    for first in (0, (1 << 22) - 500, n - 1000):
+        got = out.view(first * heads * 2, (1000, heads, 2)).to_numpy()
+        want, off = turned(np.repeat(x.astype(np.float64), 1000, axis=0), positions[first:first + 1000], 2, 10000.0, None, 1.0, False, "f16")
+        ref.check(ref.values(got, "f16"), want, off, "many")
+
+
+def into_the_cache(dev, rng, dtype, interleaved, heads, kv_heads, d, dim, page, lens, new, hole):
+    p = ref.Paged(rng, dtype, heads, kv_heads, d, page, lens, new, holes=[hole], spare=0)
     p.lens[1] = p.cap + 3
     k, v = (ref.rounded(rng.standard_normal((p.tokens, kv_heads, d)), dtype) for _ in range(2))
     cache = dev.paged_cache(ref.upload(dev, p.k, dtype), ref.upload(dev, p.v, dtype), dev.upload(p.table), dev.upload(p.lens.astype(np.int32)))
@@ -158,6 +172,24 @@ def test_into_the_cache(dev, dtype, interleaved, heads, kv_heads, d, dim, page):
     here = ref.upload(dev, q, dtype)
     dev.paged_rope_append(cache, dev.upload(starts), here, ref.upload(dev, pad(k), dtype), ref.upload(dev, pad(v), dtype), dev.rope_table(dim), factor=1.25, interleaved=interleaved, out=here)
     assert np.array_equal(ref.values(here.to_numpy(), dtype)[2:-3], got[2:-3]) and np.isnan(ref.values(here.to_numpy(), dtype)[:2]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("heads, kv_heads, d, dim", [(4, 2, 64, 64), (3, 1, 20, 8), (8, 8, 80, 32), (2, 2, 7, 6), (40, 8, 128, 128)])
+@pytest.mark.parametrize("page", [16, 7, 1])
+def test_into_the_cache(dev, dtype, interleaved, heads, kv_heads, d, dim, page):
+    # a first token, a prompt, a later piece, nothing, a page that is missing, more new tokens than lens counts, tokens beyond the table
+    into_the_cache(dev, np.random.default_rng(d + page), dtype, interleaved, heads, kv_heads, d, dim, page, [1, 50, 40, 20, 40, 2, 33], [1, 50, 7, 0, 5, 4, 2], (4, 38 // page))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("heads, kv_heads, d, dim", [(2, 1, 64, 64), (1, 1, 20, 8), (4, 2, 40, 40), (1, 1, 7, 6)])
+def test_many_into_the_cache(dev, dtype, interleaved, heads, kv_heads, d, dim):
+    """several tokens to a block: of two sequences, of none, of pages that are missing"""
+    lens, new = [700, 1, 900, 3, 333, 2, 64, 64], [600, 1, 700, 3, 111, 4, 1, 64]
+    into_the_cache(dev, np.random.default_rng(d), dtype, interleaved, heads, kv_heads, d, dim, 16, lens, new, (2, 30))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
