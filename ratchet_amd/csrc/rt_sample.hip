@@ -8,11 +8,13 @@
 //
 // A block to a row, a sixteenth of the row to a wave; the row is read again for every walk over it, from the L2.  NaN fails every comparison here, and so is never kept.
 //   temperature alone: the waves' sums of weights, then the one wave's share that holds the border is dealt out to all threads again
-//   top-k: the kth largest of the threads' maxima bounds the kth largest logit; what reaches it is listed, and a list of up to 1024 is sorted, cut and drawn from
-//          by itself
+//   top-k: the kth largest of the threads' maxima, to a step of a histogram, bounds the kth largest logit; what reaches it is listed, and a list of up to 1024 is sorted,
+//          cut and drawn from by itself
 //   top-p: a histogram of the weights over 2048 equal steps of the logit names the step the cut lies in; its members are listed and sorted for
 //          the cut.  A step of too many members is cut into 2048 again, down to equals
-// What bounds it: vector instructions, some 25 for a weight in 64 bits, twice for each logit where many are kept, and the chain of barriers between the phases.
+// What bounds it: vector instructions, some 25 for a weight in 64 bits, twice for each logit where many are kept, and the chain of barriers between the phases.  256 rows of
+// 32064 f32 with top-p 38 us: maximum 3.5, histogram 12.4 (of which its atomics 40 clocks a wave), the step's members 4.5, their order 1.4, weights of what is kept 4.8, search
+// 4.3.  64 rows of 50295 f16 with top-k around 50 14.5 us.  One row of 51865 f32, all of it kept, 23 us: one CU reads it at 9 GB/s a wave and fetches the code for the first time.
 #include <math.h>
 
 #include "rt_arith.h"
@@ -204,7 +206,8 @@ template <typename T> struct Row {
     }
 
     // The n numbers of the threads below n, none of them 0, in descending order: a bitonic sort, between lanes where partners are in one wave.  Uses the first half of s.hist.
-    // Few are counted, several threads to a number, which takes fewer barriers and moves: 60 numbers 1.3 us, sorted 2.6.
+    // Few are counted, several threads to a number, which takes fewer barriers and moves (64 rows of 50295 f16, two such sorts, us counted | bitonic: up to 40 of k 16.7 | 21.4,
+    // up to 100 22.9 | 25.3, up to 200 25.4 | 27.8).
     __device__ __forceinline__ uint64_t sorted(uint64_t x, uint32_t n) {
         uint32_t pad = 64;
         while (pad < n) pad <<= 1;
@@ -405,17 +408,20 @@ template <typename T> struct Row {
         return s.cut ? cut_at(s.cut) : Cut{-INFINITY, -1};
     }
 
-    // A bound that at least k <= 1024 logits reach: of each wave the (k / 16)th largest of the lanes' own maxima, and of those the least.  -inf if some wave has fewer
-    __device__ __forceinline__ float reached_by(uint32_t k, float mine) {
-        // bit by bit from the top, the largest key that so many lanes reach
-        const uint32_t key = key_of(mine), most = (k + WAVES - 1) / WAVES;
-        uint32_t low = 0;
-#pragma unroll 1
-        for (uint32_t bit = 1u << 31; bit; bit >>= 1)
-            if ((uint32_t)__popcll(__ballot(key >= (low | bit))) >= most) low |= bit;
-        uint32_t high = low;
-        key_range(low, high);
-        return of_key(low);
+    // A bound that at least k <= 1024 logits reach: that k of the threads' own maxima do, by a histogram of them over equal steps down to `least`, the smallest that is not -inf.  -inf
+    // if so many threads have none
+    __device__ __forceinline__ float reached_by(uint32_t k, float mine, float least) {
+        float per = BINS / (max - least);
+        per = per < 1e30f ? per : 1e30f;
+        clear();
+        if (mine >= least) {
+            const float b = (max - mine) * per;
+            atomicAdd((unsigned long long*)&s.hist[b < (float)(BINS - 1) ? (uint32_t)b : BINS - 1], 1ull);
+        }
+        find_bin(0, (double)k);
+        const uint32_t bin = s.bin;
+        if (bin == BINS) return -INFINITY;
+        return bin < BINS - 1 && per > 0x1p-64f && per < 0x1p64f ? max - ((float)bin + 1.5f) / per : least;        // (half a step out, for the roundings)
     }
 
     // Draws from the n places of s.places, which hold all that may be kept: the first k of them, of those the ones with less than p of their weight
@@ -456,9 +462,10 @@ template <typename T> __global__ void __launch_bounds__(BLOCK) sample_kernel(Sam
     float* const prob_at = a.probs ? a.probs + row : nullptr;
     float mine = -INFINITY;
     r.each([&](float x, int32_t) { mine = fmaxf(mine, x); });
-    uint32_t high = key_of(mine), none = 0;
-    r.block_max(high, none);
+    uint32_t high = key_of(mine), low = mine > -INFINITY ? ~high : 0;
+    r.block_max(high, low);
     r.max = of_key(high);
+    const float least = of_key(~low);              // of the threads' maxima
     uint64_t total;
     if (r.max == -INFINITY || r.max == INFINITY || !(temperature > 0.0f)) {
         // nothing to choose from; equals that share all the weight; or, greedy, the first of the largest
@@ -490,7 +497,7 @@ template <typename T> __global__ void __launch_bounds__(BLOCK) sample_kernel(Sam
         const float p = top_p > 0.0f ? top_p : 0.0f;
         float floor;
         if (counts) {
-            floor = (uint32_t)k <= BLOCK ? r.reached_by((uint32_t)k, mine) : -INFINITY;
+            floor = (uint32_t)k <= BLOCK ? r.reached_by((uint32_t)k, mine, least) : -INFINITY;
             floor = fmaxf(floor, r.max - 48.0f * temperature);
         } else {
             // all of those below this weigh less than half of what may be dropped; 0.7 is a little above ln 2
@@ -499,8 +506,9 @@ template <typename T> __global__ void __launch_bounds__(BLOCK) sample_kernel(Sam
         floor = fmaxf(floor, -3.4028235e38f);                   // (of an endless temperature: all that are finite)
         const bool all = front.x == -INFINITY;                  // nothing is cut yet: what is not finite weighs 0 and lies below the floor
         auto in = [&](float x, int32_t i) -> bool { return x >= floor && (all || front.keeps(x, i)); };
-        if (counts && (uint32_t)k <= LIST / 4) {
-            r.clear();
+        // Listed, where as many hardly ever pass a list, which is then a walk for nothing (64 rows of 50295 f16, us listed | cut by a histogram: k 20 12.6 | 42, 200 18.7 | 49,
+        // 500 33 | 49; 700 59 | 50).  None is listed yet
+        if (counts && (uint32_t)k <= LIST / 2) {
             r.each([&](float x, int32_t i) {
                 if (in(x, i)) r.list(x, i);
             });

@@ -97,6 +97,29 @@ def test_top_k(dev, dtype, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [1, 2, 50, 511, 512, 513, 900])
+def test_top_k_of_rows_in_an_order(dev, dtype, k):
+    """falling, rising, all but some alike, all in one place, few that are finite, ends of the range"""
+    rng = np.random.default_rng(k)
+    n = 20000
+    x = np.sort(rng.standard_normal((8, n)) * 3, axis=1)
+    x[0] = x[0, ::-1]
+    x[1] = x[1, ::-1] - np.log1p(np.arange(n))
+    x[3] = 1.0
+    x[3, ::37] = 2.0
+    x[4, :] = -4.0
+    x[4, 7000:7600] = rng.standard_normal(600)
+    x[5, :] = -np.inf
+    x[5, rng.integers(0, n, 300)] = rng.standard_normal(300)
+    x[6, ::2] = -6e4 if dtype == "f16" else -3.3e38
+    x[6, 1::5] = 6e4 if dtype == "f16" else 3.3e38
+    x[7] = 1.0
+    x = ref.rounded(x, dtype)
+    for p in (1.0, 0.9):
+        run(dev, x, dtype, rng.random(8), k=k, p=p)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("p", [0.0, -1.0, 1e-30, 1e-6, 0.1, 0.5, 0.9, 0.999, 1 - 2.0 ** -24, 1.0, 1.5, np.nan])
 def test_top_p(dev, dtype, p):
     rng = np.random.default_rng(7)
