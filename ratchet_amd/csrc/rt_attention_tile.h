@@ -375,6 +375,7 @@ struct AttnPartial {
 
 // Contiguous: which row tile, counted from the last, has place `at` in the launch.  A launch that the chip holds at once is not balanced by blocks that come later: where
 // a CU gets one block of each `round` tiles, every other round runs backwards, so that a long causal walk shares its CU with a short one.
+// Where a CU holds one block, the next is the longest that is left (256 columns, f16, causal 2048 tokens of 32 heads: 126 us, with turned rounds 154).
 __device__ __forceinline__ uint32_t at_turned(const AttnPartial& part, uint32_t at) {
     if (part.round == 0) return at;
     const uint32_t n = at / part.round, first = n * part.round, count = part.row_tiles - first < part.round ? part.row_tiles - first : part.round;
@@ -1064,7 +1065,8 @@ template <typename T, int DT, bool EXACT, bool PAGED, bool SCORED> int at_launch
         part.pieces = (uint32_t)((span + piece - 1) / piece);
         part.split = part.pieces > 1;
         items = (uint64_t)part.row_tiles * part.pieces;
-        if (a.causal && part.pieces == 1 && tiles > (uint64_t)dev->num_cus && tiles <= 3ull * dev->num_cus) part.round = (uint32_t)(dev->num_cus / per);
+        constexpr uint64_t HELD = 160 * 1024 / S::LDS < S::WAVES ? 160 * 1024 / S::LDS : S::WAVES;             // blocks of a CU at once
+        if (a.causal && part.pieces == 1 && tiles > (uint64_t)dev->num_cus && tiles <= HELD * dev->num_cus) part.round = (uint32_t)(dev->num_cus / per);
         join_tiles = part.row_tiles * per;
     }
     const uint64_t blocks = items * per;
@@ -1123,8 +1125,8 @@ template <typename T, bool SCORED> int at_dispatch_tile(rt_device* dev, AttnArgs
     if (a.dim == 128) RT_TILE(128, true);
     if (a.dim == 192) RT_TILE(192, true);
     if (a.dim == 256) RT_TILE(256, true);
-    // f16, 32 heads, causal 2048 tokens: 40 columns 50 us, in the variant for 128 66; 192 and 256 columns 130 and 160 us,
-    // with each step's columns tested 248 and 262 (f32 603 and 904, 1549 and 2720)
+    // f16, 32 heads, causal 2048 tokens: 40 columns 50 us, in the variant for 128 66; 192 and 256 columns 101 and 123 us (with turned rounds 130 and 160, and then with each
+    // step's columns tested 248 and 262; f32 603 and 904, 1549 and 2720)
     if (a.dim < 64) RT_TILE(64, false);
     if (a.dim < 128) RT_TILE(128, false);
     RT_TILE(256, false);
