@@ -20,7 +20,8 @@
 namespace {
 
 constexpr int BLOCK = 256, TRIP = 2;              // units of two vectors that a thread has in flight
-constexpr uint32_t PAIRS = 1024;                  // (token, frequency) pairs of a block: LDS for their sines and cosines
+constexpr uint32_t MOST_HALF = 512;               // frequencies
+constexpr uint32_t PAIRS = 2 * MOST_HALF;         // (token, frequency) pairs of a block: LDS for their sines and cosines
 constexpr uint32_t GRID_ROW = 1u << 22;           // blocks to a row of the grid: an extent of a launch has fewer than 2^32 threads
 
 struct RopeRows {
@@ -297,7 +298,7 @@ int table_rules(const char* who, int dt, uint32_t head_dim, const uint64_t* turn
     RT_REQUIRE(rt_is_float_dt(dt), RT_ERR_DTYPE, "%s: dtype %d is not F32, F16 or BF16", who, dt);
     RT_REQUIRE(head_dim > 0, RT_ERR_SHAPE, "%s: zero extent", who);
     RT_REQUIRE(dim > 0 && dim % 2 == 0 && dim <= head_dim, RT_ERR_SHAPE, "%s: dim %u must be positive, even and <= %u", who, dim, head_dim);
-    RT_REQUIRE(dim / 2 <= PAIRS && head_dim <= 1u << 16, RT_ERR_SIZE, "%s: %u of %u columns", who, dim, head_dim);
+    RT_REQUIRE(dim / 2 <= MOST_HALF && head_dim <= 1u << 16, RT_ERR_SIZE, "%s: %u of %u columns", who, dim, head_dim);
     RT_REQUIRE(isfinite(factor), RT_ERR_ARG, "%s: factor is not finite", who);
     RT_REQUIRE(interleaved == 0 || interleaved == 1, RT_ERR_ARG, "%s: interleaved is %d", who, interleaved);
     RT_REQUIRE(turns, RT_ERR_NULL_POINTER, "%s: NULL table", who);
