@@ -21,6 +21,9 @@
 // matrix units are busy 47 % and the vector units (scores to weights: six to seven instructions each, by the counters) 62 % of the time, and three waves of a SIMD have both overlap
 // only in part.  f32, [4,6,1500,64]: 154 us, 79 % of it the matrix units, whose f32 products do an eighth of the 16-bit ones' work.  Single tokens, 64 of about
 // 4600 keys in bf16: 242 us, the keys and values once at 5.0 TB/s; a copy reaches 5.2.
+//
+// Changed scores are vector instructions on top: f16, 4096 tokens of 16 heads on 8 of 256 with a window of 2048, capped, 225 us; bf16, 2048 tokens of 32 heads of 128, biased by
+// distance 64, plain 54; 12 texts in 8192 tokens of 32 heads on 8 of 128 119, of which about 40 are what four rounds of blocks take whatever their keys.
 #ifndef RT_ATTENTION_TILE_H
 #define RT_ATTENTION_TILE_H
 
