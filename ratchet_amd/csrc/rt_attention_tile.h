@@ -28,6 +28,7 @@
 #define RT_ATTENTION_TILE_H
 
 #include "rt_attention.h"
+#include "rt_attention_order.h"
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -378,7 +379,7 @@ struct AttnPartial {
 
 // Contiguous: which row tile, counted from the last, has place `at` in the launch.  A launch that the chip holds at once is not balanced by blocks that come later: where
 // a CU gets one block of each `round` tiles, every other round runs backwards, so that a long causal walk shares its CU with a short one.
-// Where a CU holds one block, the next is the longest that is left (256 columns, f16, causal 2048 tokens of 32 heads: 126 us, with turned rounds 154).
+// Which launches are turned: rt_attention_order.h.
 __device__ __forceinline__ uint32_t at_turned(const AttnPartial& part, uint32_t at) {
     if (part.round == 0) return at;
     const uint32_t n = at / part.round, first = n * part.round, count = part.row_tiles - first < part.round ? part.row_tiles - first : part.round;
@@ -1069,7 +1070,7 @@ template <typename T, int DT, bool EXACT, bool PAGED, bool SCORED> int at_launch
         part.split = part.pieces > 1;
         items = (uint64_t)part.row_tiles * part.pieces;
         constexpr uint64_t HELD = 160 * 1024 / S::LDS < S::WAVES ? 160 * 1024 / S::LDS : S::WAVES;             // blocks of a CU at once
-        if (a.causal && part.pieces == 1 && tiles > (uint64_t)dev->num_cus && tiles <= HELD * dev->num_cus) part.round = (uint32_t)(dev->num_cus / per);
+        if (a.causal && part.pieces == 1) part.round = at_round(tiles, per, (uint64_t)dev->num_cus, HELD);
         join_tiles = part.row_tiles * per;
     }
     const uint64_t blocks = items * per;
