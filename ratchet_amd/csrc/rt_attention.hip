@@ -186,7 +186,7 @@ int head_rules(const char* who, int dt, uint32_t heads, uint32_t kv_heads, uint3
 int score_rules(const char* who, const rt_scores* scores, float scale, uint32_t batch, bool documents, bool causal, AttnArgs& a) {
     RT_REQUIRE(scores, RT_ERR_NULL_POINTER, "%s: NULL scores", who);
     RT_REQUIRE(scores->cap >= 0.0f && isfinite(scores->cap), RT_ERR_ARG, "%s: cap must be finite and not negative", who);
-    RT_REQUIRE(scores->cap == 0.0f || isfinite(scores->cap * 1.4426950408889634f), RT_ERR_ARG, "%s: cap is too large", who);
+    RT_REQUIRE(scores->cap == 0.0f || isfinite(2.0f * scores->cap * 1.4426950408889634f), RT_ERR_ARG, "%s: cap is too large", who);        // at_capped multiplies by its double
     RT_REQUIRE(scores->cap == 0.0f || isfinite(scale / scores->cap), RT_ERR_ARG, "%s: scale / cap is not finite", who);
     RT_REQUIRE(documents || !scores->documents, RT_ERR_ARG, "%s: sequences are not cut into documents", who);
     RT_REQUIRE(!scores->documents == !scores->n_documents, RT_ERR_SHAPE, "%s: %u documents", who, scores->n_documents);

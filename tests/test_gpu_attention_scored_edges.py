@@ -1,0 +1,42 @@
+"""Attention with changed scores where its numbers end."""
+import numpy as np
+import pytest
+
+import attention_ref as ref
+from attention_ref import U
+from ratchet_amd import _lib
+
+pytestmark = pytest.mark.gpu
+DTYPES = ["f32", "f16", "bf16"]
+
+
+@pytest.fixture(scope="module")
+def dev():
+    from ratchet_amd import Device
+
+    d = Device(0)
+    yield d
+    d.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("queries", [1, 70])
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("cap", [1.0e38, 1.17e38])
+def test_the_largest_caps(dev, dtype, queries, aligned, cap):
+    """scores of 1.7 cap and its half, its 64th and its negative among those that are 0: the largest has all the weight, and its row is the result.  Products are powers of two,
+    so lse is off by the cap's 12 u (test_gpu_attention_scored.py), 2 u of 1.7 cap for the division by the cap, and 4 u for units and the last product: 24 u of the cap"""
+    rng, d, keys = np.random.default_rng(1), 64, 130
+    q, k, v = np.zeros((1, 2, queries, d)), np.zeros((1, 1, keys, d)), ref.rounded(rng.standard_normal((1, 1, keys, d)), dtype)
+    q[..., 0] = 2.0 ** 60
+    q[0, 1, :, 0] = -2.0 ** 60                                   # the other head's signs are turned
+    top = 2.0 ** 67 / 8
+    k[0, 0, [7, 70, 100, 129], 0] = top, top / 2, top / 64, -top
+    parts = []
+    for x in (q, k, v):
+        parts.append(ref.upload(dev, x, dtype) if aligned else ref.upload(dev, np.concatenate([[0.0], x.ravel()]), dtype).view(1, x.shape))
+    lse = dev.empty((1, 2, queries), _lib.F32)
+    out = ref.values(dev.attention(*parts, causal=False, scale=8.0, cap=cap, lse=lse).to_numpy(), dtype)
+    most = float(np.float32(cap)) * np.tanh(8.0 * 2.0 ** 60 * top / float(np.float32(cap)))
+    assert np.array_equal(out[0, 0], np.broadcast_to(v[0, 0, 7], (queries, d))) and np.array_equal(out[0, 1], np.broadcast_to(v[0, 0, 129], (queries, d)))
+    assert (np.abs(lse.to_numpy() - most) <= 24 * U * cap).all()
