@@ -213,6 +213,12 @@ template <typename T, bool SCORED> __device__ __forceinline__ float at_changed(c
     return x;
 }
 
+// A head's slope in units of log2(e).  One that passes f32's largest there stays finite, so that at distance 0 it takes nothing: a bias that leaves a row its own key
+__device__ __forceinline__ float at_slope(const AttnArgs& a, uint32_t h) {
+    const float slope = a.slopes[h], x = slope * 1.4426950408889634f;
+    return __builtin_isfinite(slope) ? fminf(fmaxf(x, -3.4028235e38f), 3.4028235e38f) : x;
+}
+
 // The page of token t, or -1 if there is none
 __device__ __forceinline__ int32_t at_page(const AttnArgs& a, uint32_t b, uint32_t t, uint32_t& slot) {
     uint32_t at;

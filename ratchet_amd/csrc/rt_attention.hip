@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(BLOCK) attention_any_kernel(AttnArgs a, uint64
     const T* k = (const T*)a.k + g * a.k_h + (PAGED ? 0 : b * a.k_b);
     const T* v = (const T*)a.v + g * a.v_h + (PAGED ? 0 : b * a.v_b);
     const AttnRow r = at_row<SCORED>(a, SCORED ? at_texts(a, b) : AttnTexts{}, b, s, j);
-    const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
+    const float slope = SCORED && a.slopes ? at_slope(a, h) : 0.0f;
     float m = -INFINITY, l = 0.0f, o[AT_MAX_DIM / 64];
 #pragma unroll
     for (int i = 0; i < AT_MAX_DIM / 64; i++) o[i] = 0.0f;

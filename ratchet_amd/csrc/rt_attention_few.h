@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(AT_BLOCK) attention_few_kernel(AttnArgs a, Att
     } else {
         me = at_in_text(a, at_position(s, j), 0, s.keys, a.prefix ? a.prefix[b] : 0);
     }
-    const float slope = a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
+    const float slope = a.slopes ? at_slope(a, h) : 0.0f;
 
     v4u q[S::STEPS];
     {

@@ -311,7 +311,7 @@ __device__ __forceinline__ void at_row_again(const AttnArgs& a, uint32_t b, uint
     const T* k = (const T*)a.k + g * a.k_h + (PAGED ? 0 : b * a.k_b);
     const T* v = (const T*)a.v + g * a.v_h + (PAGED ? 0 : b * a.v_b);
     const AttnRow r = at_row<SCORED>(a, SCORED && !PAGED ? at_texts(a, b) : AttnTexts{}, b, s, j);
-    const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.0f;
+    const float slope = SCORED && a.slopes ? at_slope(a, h) : 0.0f;
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int i = 0; i < COLS; i++) o[i] = 0.0f;
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
     // capped scores are in units of log2 e from there on; others get their bias in units of the products, divided by c, which then need no product of their own (unless c is next to 0)
     const bool changed = SCORED && (a.most != 0.0f || (a.slopes && __builtin_fabsf(a.c) < 0x1p-40f));
     const float c = changed ? 1.0f : fmaxf(__builtin_fabsf(a.c), 1e-37f);
-    const float slope = SCORED && a.slopes ? a.slopes[h] * 1.4426950408889634f / c : 0.0f;
+    const float slope = SCORED && a.slopes ? at_slope(a, h) / c : 0.0f;
 
     // ---- this lane's part of a tile's loads: LDS chunk `slot` belongs to row slot / chunks
     uint32_t l_row[S::LOADS], l_k[S::LOADS], l_v[S::LOADS];
@@ -724,6 +724,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
 #pragma unroll
     for (int i = 0; i < S::BLOCKS; i++) o[i] = v16f{0};
     float m = -INFINITY, l = 0.0f;                              // l: of this lane's half of the keys
+    if (SCORED && a.slopes && !__builtin_isfinite(slope)) l = __builtin_nanf("");                // beyond f32 in units of the products: computed again, a row at a time
 
     int32_t page = 0;                                           // of this lane's key of the tile after next
     uint32_t slot = 0;

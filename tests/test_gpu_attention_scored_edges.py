@@ -5,6 +5,7 @@ import pytest
 import attention_ref as ref
 from attention_ref import U
 from ratchet_amd import _lib
+from test_gpu_attention_scored import head
 
 pytestmark = pytest.mark.gpu
 DTYPES = ["f32", "f16", "bf16"]
@@ -40,3 +41,24 @@ def test_the_largest_caps(dev, dtype, queries, aligned, cap):
     most = float(np.float32(cap)) * np.tanh(8.0 * 2.0 ** 60 * top / float(np.float32(cap)))
     assert np.array_equal(out[0, 0], np.broadcast_to(v[0, 0, 7], (queries, d))) and np.array_equal(out[0, 1], np.broadcast_to(v[0, 0, 129], (queries, d)))
     assert (np.abs(lse.to_numpy() - most) <= 24 * U * cap).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries", [1, 70])
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("slope, scale", [(3e37, 0.125), (2.3e38, 0.125), (2.5e38, -0.125), (3.4028234e38, 0.125), (1e34, 1e-5)])
+def test_a_slope_that_leaves_a_row_its_own_key(dev, dtype, queries, aligned, cap, slope, scale):
+    """next to a head of the same KV head whose slope is ordinary; the bounds are test_gpu_attention_scored.py's, the first head's for a row of one visible key"""
+    rng, keys, d = np.random.default_rng(2), 130, 64
+    q, k, v = (ref.rounded(rng.standard_normal(s), dtype) for s in ((1, 2, queries, d), (1, 1, keys, d), (1, 1, keys, d)))
+    parts = []
+    for x in (q, k, v):
+        parts.append(ref.upload(dev, x, dtype) if aligned else ref.upload(dev, np.concatenate([[0.0], x.ravel()]), dtype).view(1, x.shape))
+    slopes, lse = np.array([slope, 0.125], np.float32), dev.empty((1, 2, queries), _lib.F32)
+    out = ref.values(dev.attention(*parts, scale=scale, cap=cap, slopes=dev.upload(slopes), lse=lse).to_numpy(), dtype)
+    distance = (np.arange(queries) + keys - queries)[:, None] - np.arange(keys)[None, :]
+    for h, (see, s) in enumerate(((distance == 0, 0.0), (distance >= 0, 0.125))):
+        o, want_lse, o_off, lse_off = head(q[0, h], k[0, 0], v[0, 0], see, scale, dtype, cap, s, distance)
+        ref.check(out[0, h], o, o_off, ("o", h))
+        ref.check(lse.to_numpy()[0, h], want_lse, lse_off, ("lse", h))
