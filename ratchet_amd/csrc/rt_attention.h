@@ -177,6 +177,20 @@ __device__ __forceinline__ AttnRow at_in_document(const AttnArgs& a, const AttnT
     }
     return at_in_text(a, p, lo, hi, prefix);
 }
+// The document of position p, a lane's own, among those from da to dz, the same in all lanes, that at_document names for the first and the last row: the last that begins at or
+// before it, in as many steps as their number has bits, so that texts without tokens (an array that repeats its end) are not walked one by one.  All lanes take part.
+__device__ __forceinline__ uint32_t at_document_of(const AttnArgs& a, const AttnTexts& t, uint32_t b, int32_t p, uint32_t da, uint32_t dz) {
+    const uint32_t first = da > a.n_documents ? 0 : da + 1;    // da may be `none in front`, beyond all numbers
+    if (dz > a.n_documents || dz < first) return da;
+    const uint32_t count = dz - first + 1;
+    uint32_t n = 0;                                // of them begin at or before p
+    for (uint32_t step = 1u << (31 - __builtin_clz(count)); step; step >>= 1) {
+        const uint32_t at = n + step;
+        const int32_t start = at_start(a, t, b, first + (at <= count ? at : 1) - 1);
+        if (at <= count && start <= p) n = at;
+    }
+    return n ? first + n - 1 : da;
+}
 // Row j of sequence b; all lanes take part, with the same row
 template <bool SCORED> __device__ __forceinline__ AttnRow at_row(const AttnArgs& a, const AttnTexts& t, uint32_t b, const AttnSeq& s, uint32_t j) {
     const int32_t p = at_position(s, j);

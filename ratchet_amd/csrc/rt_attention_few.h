@@ -118,11 +118,7 @@ __global__ void __launch_bounds__(AT_BLOCK) attention_few_kernel(AttnArgs a, Att
     if (!PAGED && a.documents) {
         const int32_t p_a = at_position(s, fd_div(row0, a.group_div)), p_z = at_position(s, fd_div(row0 + rows - 1, a.group_div));
         const uint32_t da = at_document(a, texts, b, p_a), dz = at_document(a, texts, b, p_z);
-        uint32_t d = da;
-        if (dz <= a.n_documents)
-            for (uint32_t n = da > a.n_documents ? 0 : da + 1; n <= dz; n++)
-                if (at_start(a, texts, b, n) <= at_position(s, j)) d = n;
-        me = at_in_document(a, texts, b, s, at_position(s, j), d);
+        me = at_in_document(a, texts, b, s, at_position(s, j), at_document_of(a, texts, b, at_position(s, j), da, dz));
     } else {
         me = at_in_text(a, at_position(s, j), 0, s.keys, a.prefix ? a.prefix[b] : 0);
     }

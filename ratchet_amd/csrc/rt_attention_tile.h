@@ -585,11 +585,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
             const uint32_t da = at_document(a, texts, b, at_position(s, ja)), dz = at_document(a, texts, b, at_position(s, jz));
             ra = at_in_document(a, texts, b, s, at_position(s, ja), da);
             rz = at_in_document(a, texts, b, s, at_position(s, jz), dz);
-            uint32_t d = da;                                    // may be `none in front`, beyond all numbers
-            if (dz <= a.n_documents)
-                for (uint32_t n = da > a.n_documents ? 0 : da + 1; n <= dz; n++)
-                    if (at_start(a, texts, b, n) <= at_position(s, j)) d = n;
-            me = at_in_document(a, texts, b, s, at_position(s, j), d);
+            me = at_in_document(a, texts, b, s, at_position(s, j), at_document_of(a, texts, b, at_position(s, j), da, dz));
         } else {
             const int32_t prefix = a.prefix ? a.prefix[b] : 0;
             me = at_in_text(a, at_position(s, j), 0, s.keys, prefix);

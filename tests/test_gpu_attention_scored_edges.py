@@ -5,7 +5,7 @@ import pytest
 import attention_ref as ref
 from attention_ref import U
 from ratchet_amd import _lib
-from test_gpu_attention_scored import head
+from test_gpu_attention_scored import dense, head
 
 pytestmark = pytest.mark.gpu
 DTYPES = ["f32", "f16", "bf16"]
@@ -62,3 +62,19 @@ def test_a_slope_that_leaves_a_row_its_own_key(dev, dtype, queries, aligned, cap
         o, want_lse, o_off, lse_off = head(q[0, h], k[0, 0], v[0, 0], see, scale, dtype, cap, s, distance)
         ref.check(out[0, h], o, o_off, ("o", h))
         ref.check(lse.to_numpy()[0, h], want_lse, lse_off, ("lse", h))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [63, 64, 3000])
+def test_texts_padded_with_ends(dev, dtype, n):
+    """an array of a fixed length whose last texts hold nothing, queries behind them all, and texts of nothing in front and between"""
+    rng = np.random.default_rng(n)
+    few = [0, 0, 0, 40, 41, 41, 41, 41, 130, 350]
+    some = [5] * 30 + np.sort(rng.integers(5, 300, 20)).tolist()
+    documents = [few + [350] * (n + 1 - len(few)), some + [some[-1]] * (n + 1 - len(some))]
+    prefix = rng.integers(0, 30, (2, n))
+    dense(dev, rng, dtype, 2, 2, 1, 400, 400, 64, documents=documents, prefix=prefix)
+    dense(dev, rng, dtype, 2, 4, 2, 100, 340, 64, documents=documents, window=17, sinks=2, cap=5.0)
+    dense(dev, rng, dtype, 2, 2, 1, 8, 304, 64, documents=documents, prefix=prefix)
+    dense(dev, rng, dtype, 2, 2, 1, 8, 352, 64, documents=documents, causal=False)
+    dense(dev, rng, dtype, 2, 2, 1, 30, 360, 64, documents=documents, aligned=False)
