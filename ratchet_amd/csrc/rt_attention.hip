@@ -205,7 +205,7 @@ int score_rules(const char* who, const rt_scores* scores, float scale, uint32_t 
         double power = (double)a.most * k;
         for (int i = 0; i < 4; i++, power *= (double)k * k) a.near[i] = (float)(tanh_terms[i] * power);
         a.near_limit = 0.4f / k;
-    } else if (k > 0.0f && k <= 0x1p-19f && a.most > 1.0f) {
+    } else if (k <= 0x1p-19f && a.most > 1.0f) {                  // (a scale of 0 too: capped scores are 0)
         const double c = (double)a.most * k;
         a.near[0] = (float)c;
         a.near[1] = (float)(-c * k * k / 3);

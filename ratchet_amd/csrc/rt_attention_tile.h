@@ -771,6 +771,22 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
         at_settle(SUMS == 1 ? x[S::HALVES - 1] : others[S::HALVES - 1][SUMS - 1]);
 #pragma unroll
         for (int kk = 0; kk < S::HALVES; kk++) at_join_sums(x[kk], others[kk]);
+        const auto each_seen = [&](auto f) __attribute__((always_inline)) {     // each score of the tile, and whether its row sees its key
+            // key t = 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile: p - t < window as t > p - window, which saturates where there is no window
+            int32_t lim = limit - t0 - 4 * (int32_t)half, from = __builtin_elementwise_sub_sat(p - t0 - 4 * (int32_t)half, a.window), sink = (SCORED ? front : a.sinks) - t0 - 4 * (int32_t)half, low = lo - t0 - 4 * (int32_t)half;
+            asm volatile("" : "+v"(lim), "+v"(from), "+v"(sink));               // nothing of this is worth registers outside of masked tiles
+            if (SCORED && !PAGED) asm volatile("" : "+v"(low));
+            const uint64_t have = there >> (4 * half);
+#pragma unroll
+            for (int kk = 0; kk < S::HALVES; kk++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int32_t t = 32 * kk + e % 4 + 8 * (e / 4);
+                    float score = x[kk][e];
+                    f(score, t <= lim && (t > from || t < sink) && (!SCORED || PAGED || t >= low) && (!PAGED || (have >> t) & 1));
+                    x[kk][e] = score;
+                }
+        };
         if (changed) {
             if (a.most != 0.0f) {
                 bool near = false;
@@ -781,6 +797,11 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
 #pragma unroll
                         for (int e = 0; e < 16; e++) far = fmaxf(far, __builtin_fabsf(x[kk][e]));
                     near = __ballot(!(far <= a.near_limit)) == 0;
+                    if (!near && a.most > AT_COARSE) {          // what hidden keys hold does not have the rows computed again
+                        far = 0.0f;
+                        each_seen([&](float& score, bool seen) __attribute__((always_inline)) { far = fmaxf(far, seen ? __builtin_fabsf(score) : 0.0f); });
+                        near = __ballot(!(far <= a.near_limit)) == 0;
+                    }
                 }
                 if (near) {                                     // half of what the exponential and the reciprocal take
 #pragma unroll
@@ -815,19 +836,7 @@ __global__ void __launch_bounds__(AT_BLOCK) __attribute__((amdgpu_waves_per_eu(A
                 for (int e = 0; e < 16; e++) x[kk][e] = __builtin_fmaf(-slope, __builtin_fabsf(far - (float)(32 * kk + e % 4 + 8 * (e / 4))), x[kk][e]);
         }
         if (t0 + KT - 1 > limit_a || (SCORED && !PAGED && t0 < lo_z) || (t0 + KT > (SCORED ? front_a : a.sinks) && p_z - t0 >= a.window) || (PAGED && there != ~0ull)) {
-            // key t = 32 kk + (e % 4) + 8 (e / 4) + 4 half of the tile: p - t < window as t > p - window, which saturates where there is no window
-            int32_t lim = limit - t0 - 4 * (int32_t)half, from = __builtin_elementwise_sub_sat(p - t0 - 4 * (int32_t)half, a.window), sink = (SCORED ? front : a.sinks) - t0 - 4 * (int32_t)half, low = lo - t0 - 4 * (int32_t)half;
-            asm volatile("" : "+v"(lim), "+v"(from), "+v"(sink));               // nothing of this is worth registers outside of masked tiles
-            if (SCORED && !PAGED) asm volatile("" : "+v"(low));
-            const uint64_t have = there >> (4 * half);
-#pragma unroll
-            for (int kk = 0; kk < S::HALVES; kk++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int32_t t = 32 * kk + e % 4 + 8 * (e / 4);
-                    const bool seen = t <= lim && (t > from || t < sink) && (!SCORED || PAGED || t >= low) && (!PAGED || (have >> t) & 1);
-                    x[kk][e] = seen ? x[kk][e] : -INFINITY;
-                }
+            each_seen([&](float& score, bool seen) __attribute__((always_inline)) { score = seen ? score : -INFINITY; });
         }
         if (FEW && a.scores && r < rows) {
             typedef float v4f __attribute__((ext_vector_type(4)));

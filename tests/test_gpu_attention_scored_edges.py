@@ -78,3 +78,47 @@ def test_texts_padded_with_ends(dev, dtype, n):
     dense(dev, rng, dtype, 2, 2, 1, 8, 304, 64, documents=documents, prefix=prefix)
     dense(dev, rng, dtype, 2, 2, 1, 8, 352, 64, documents=documents, causal=False)
     dense(dev, rng, dtype, 2, 2, 1, 30, 360, 64, documents=documents, aligned=False)
+
+
+def large_keys_that_some_rows_do_not_see(q, k, v):
+    """the first text's keys are large and its queries 0, so that its scores are 0 and those of the second text's rows, which do not see them, are far beyond a cap"""
+    q[:, :, :70] = 0.0
+    k[:, :, :70] *= 2.0 ** 12
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("cap", [1e3, 1e7])
+def test_large_keys_that_no_other_row_sees(dev, dtype, dim, cap):
+    rng = np.random.default_rng(dim)
+    dense(dev, rng, dtype, 1, 2, 1, 200, 200, dim, documents=[[0, 70, 200]], cap=cap, change=large_keys_that_some_rows_do_not_see)
+    dense(dev, rng, dtype, 1, 2, 1, 200, 200, dim, documents=[[0, 70, 190]], prefix=[[9, 90]], window=40, sinks=3, slopes=[0.5, 0.01], cap=cap, change=large_keys_that_some_rows_do_not_see)
+    # keys behind the window of all rows but the first, whose query is 0
+    def first(q, k, v):
+        q[:, :, 0] = 0.0
+        k[:, :, 1] *= 2.0 ** 12
+    dense(dev, rng, dtype, 1, 2, 1, 40, 70, dim, window=30, cap=cap, change=first)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("what", ["hidden keys", "no scale"])
+def test_rows_are_computed_again_for_what_they_see_alone(dev, dtype, what):
+    """Computed again a row at a time, this call takes 125 times as long (20 us, 2.5 ms): scores beyond a large cap that no row sees, or that a scale of 0 makes 0, have no part in that"""
+    def took(hidden, scale):
+        rng = np.random.default_rng(3)
+        q, k, v = (rng.standard_normal((1, 8, 1024, 64)) for _ in range(3))
+        if hidden:
+            large_keys_that_some_rows_do_not_see(q, k, v)
+        parts, documents, out = [ref.upload(dev, x, dtype) for x in (q, k, v)], dev.upload(np.array([[0, 70, 1024]], np.int32)), None
+        times = []
+        for _ in range(8):
+            start, stop = dev.event(), dev.event()
+            start.record()
+            for _ in range(5):
+                out = dev.attention(*parts, documents=documents, cap=1e4, scale=scale, out=out)
+            stop.record()
+            times.append(start.elapsed_ms(stop))
+        return min(times)
+
+    usual = took(False, 0.125)
+    assert took(*((True, 0.125) if what == "hidden keys" else (False, 0.0))) < 3 * usual
