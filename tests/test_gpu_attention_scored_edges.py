@@ -5,7 +5,7 @@ import pytest
 import attention_ref as ref
 from attention_ref import U
 from ratchet_amd import _lib
-from test_gpu_attention_scored import dense, head
+from test_gpu_attention_scored import dense, head, paged
 
 pytestmark = pytest.mark.gpu
 DTYPES = ["f32", "f16", "bf16"]
@@ -122,3 +122,42 @@ def test_rows_are_computed_again_for_what_they_see_alone(dev, dtype, what):
 
     usual = took(False, 0.125)
     assert took(*((True, 0.125) if what == "hidden keys" else (False, 0.0))) < 3 * usual
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, kv_heads, dim", [(8, 2, 64), (16, 1, 64), (3, 1, 128), (6, 2, 40)])
+def test_one_sequence_has_most_of_the_tokens(dev, dtype, heads, kv_heads, dim):
+    """no more tokens than sequences, whose average is one, and several row tiles of one of them: whole and partial ones, whole walks and shared ones"""
+    rng = np.random.default_rng(heads + dim)
+    new = [0, 33, 0, 1, 2, 0, 1] + [0] * 33
+    slopes = 2.0 ** (-8.0 * np.arange(1, heads + 1) / heads)
+    long, short = [5, 2500, 0, 700, 65, 0, 1] + [0] * 33, [0, 40, 0, 3, 64, 9, 1] + [0] * 33
+    paged(dev, rng, dtype, heads, kv_heads, dim, 16, long, new, cap=20.0, slopes=slopes)
+    paged(dev, rng, dtype, heads, kv_heads, dim, 24, long, new, window=100, sinks=3, slopes=slopes, holes=[(1, 3), (3, 0)])
+    paged(dev, rng, dtype, heads, kv_heads, dim, 16, long, new, prefix=[0, 2490, 0, 5, 64] + [0] * 35, window=64, cap=9.0)
+    paged(dev, rng, dtype, heads, kv_heads, dim, 16, short, new, cap=20.0, prefix=[3, 39, 1, 0, 64] + [7] * 35)
+    paged(dev, rng, dtype, heads, kv_heads, dim, 16, [30] + short[1:], [40] + [0] * 39, slopes=slopes)           # more tokens than the sequence has
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("queries", [1, 70])
+def test_a_bias_at_a_negative_scale(dev, dtype, aligned, queries):
+    rng = np.random.default_rng(queries)
+    for scale in (-0.2, -1e-6):
+        dense(dev, rng, dtype, 2, 4, 2, queries, 200, 64, scale=scale, slopes=[0.5, 0.1, 0.02, 0.0], aligned=aligned)
+        dense(dev, rng, dtype, 2, 4, 2, queries, 200, 96, scale=scale, slopes=[0.5, 0.1, -0.02, 1.0], window=30, sinks=2, aligned=aligned)
+        dense(dev, rng, dtype, 1, 2, 2, queries, 200, 64, scale=scale, slopes=[0.5, 0.1], causal=False, aligned=aligned)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 90, 0]])
+def test_pages_at_a_negative_scale(dev, dtype, new):
+    """the bits of the opposite queries at the positive one"""
+    rng = np.random.default_rng(4)
+    p = ref.Paged(rng, dtype, 8, 2, 64, 16, [700, 150, 33], new)
+    cache = dev.paged_cache(ref.upload(dev, p.k, dtype), ref.upload(dev, p.v, dtype), dev.upload(p.table), dev.upload(p.lens.astype(np.int32)))
+    starts, slopes = dev.upload(p.starts), dev.upload((2.0 ** -np.arange(1, 9)).astype(np.float32))
+    for options in (dict(), dict(cap=5.0), dict(window=40, sinks=3)):
+        one, two = (dev.paged_attention(ref.upload(dev, q, dtype), cache, starts, scale=scale, slopes=slopes, **options).to_numpy() for q, scale in ((p.q, -0.2), (-p.q, 0.2)))
+        assert np.array_equal(one.view(np.uint8), two.view(np.uint8))
