@@ -270,7 +270,7 @@ int rt_attention(rt_device* dev, int dt, const void* q, const uint32_t q_shape[4
                  void* y, const uint64_t y_strides[4], float* lse, float scale, int causal, uint32_t window, uint32_t sinks);
 
 /* Attention whose scores are changed, or masked by more than positions.  In the order they apply, s = scale * q.k first:
- *   cap        0: none; otherwise s becomes cap * tanh(s / cap)
+ *   cap        0: none; otherwise, up to 1.17e38, s becomes cap * tanh(s / cap).  In 16 bits it is off by up to 2^-21 of a cap up to 710, and so is lse (3e-4 at 700)
  *   slopes     NULL: none; f32 [heads] on the device: s loses slopes[h] * |p - t|
  *   documents  NULL: the keys are one text; i32 [B, n_documents + 1] on the device (rt_attention_scored alone), not decreasing: document d of entry b holds the keys
  *              documents[b][d] .. documents[b][d + 1] - 1.  A query sees keys of the document that its position lies in, and none if that is in no document

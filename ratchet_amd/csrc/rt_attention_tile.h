@@ -23,7 +23,7 @@
 // 4600 keys in bf16: 242 us, the keys and values once at 5.0 TB/s; a copy reaches 5.2.
 //
 // Changed scores are vector instructions on top: f16, 4096 tokens of 16 heads on 8 of 256 with a window of 2048, capped, 225 us; bf16, 2048 tokens of 32 heads of 128, biased by
-// distance 64, plain 54; 12 texts in 8192 tokens of 32 heads on 8 of 128 119, of which about 40 are what four rounds of blocks take whatever their keys.
+// distance 63, plain 54; 12 texts in 8192 tokens of 32 heads on 8 of 128 116, of which about 40 are what four rounds of blocks take whatever their keys.
 #ifndef RT_ATTENTION_TILE_H
 #define RT_ATTENTION_TILE_H
 

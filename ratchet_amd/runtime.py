@@ -227,7 +227,8 @@ def _table_dim(table):
 
 def rope_divisors(dim, base, scale, trained, low=1.0, high=32.0):
     """Divisors that scale a rotary table for a context `scale` times the `trained` one: frequencies that turn fewer than `low` times in the trained context are
-    divided by `scale`, those that turn more than `high` times by 1, those between by a mean of the two (1 / divisor is linear in the turns)."""
+    divided by `scale`, those that turn more than `high` times by 1, those between by a mean of the two (1 / divisor is linear in the turns).  Where a model's own table has
+    another ramp between them, as one that is linear in the frequency's number, give rope_table that table's divisors."""
     turns = trained * base ** (-2.0 * np.arange(dim // 2) / dim) / (2 * np.pi)
     share = np.clip((turns - low) / (high - low), 0, 1)
     return 1.0 / (share + (1 - share) / scale)
