@@ -213,12 +213,13 @@ __global__ void __launch_bounds__(AT_BLOCK) attention_few_kernel(AttnArgs a, Att
     for (int i = 0; i < S::BLOCKS; i++) o[i] = v4f32{0};
     float m = -INFINITY, l = 0.0f;                              // of this wave's keys; l: of this lane's
 
+    // All products of a tile, also those of columns beyond the rows' (of zeros, and to columns of nobody), so that no branch lies between a product and the next read of its sum:
+    // there the compiler counts the wait states of one way round only, and rows of 8 and 16 columns lost their last tile's fourth columns
     auto step = [&](uint32_t n, const lds_byte* cur, uint64_t there) __attribute__((always_inline)) {
         const int32_t t0 = start_of(n) + (int32_t)(16 * wave), t1 = t0 + 4 * (int32_t)quarter;       // this wave's first key, this lane's
         v4f32 x = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < S::STEPS; i++) {
-            if (!EXACT && (uint32_t)(4 * i * CE) >= D) continue;
             v4u k = at_lds16(cur + k_at[i]);
             if ((EXACT ? DT % (4 * CE) != 0 : true) && (4 * i + 4) * CE > (int)D && (4 * i + quarter) * CE >= D) k = v4u{0, 0, 0, 0};
             if constexpr (sizeof(T) == 2) {
@@ -279,13 +280,12 @@ __global__ void __launch_bounds__(AT_BLOCK) attention_few_kernel(AttnArgs a, Att
             const v2u weights = {AtMma<T>::pack(x[0], x[1]), AtMma<T>::pack(x[2], x[3])};
 #pragma unroll
             for (int i = 0; i < S::BLOCKS; i++)
-                if (EXACT || (uint32_t)(16 * i) < D) o[i] = AfMma<T>::pv(at_lds_turned(cur + v_at[i]), weights, o[i]);
+                o[i] = AfMma<T>::pv(at_lds_turned(cur + v_at[i]), weights, o[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < S::BLOCKS; i++)
-                if (EXACT || (uint32_t)(16 * i) < D)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[i] = AfMma<T>::one(at_lds4(cur + (v_at[i] + e * pitch)), x[e], o[i]);
+                for (int e = 0; e < 4; e++) o[i] = AfMma<T>::one(at_lds4(cur + (v_at[i] + e * pitch)), x[e], o[i]);
         }
     };
 

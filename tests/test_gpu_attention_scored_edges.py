@@ -161,3 +161,15 @@ def test_pages_at_a_negative_scale(dev, dtype, new):
     for options in (dict(), dict(cap=5.0), dict(window=40, sinks=3)):
         one, two = (dev.paged_attention(ref.upload(dev, q, dtype), cache, starts, scale=scale, slopes=slopes, **options).to_numpy() for q, scale in ((p.q, -0.2), (-p.q, 0.2)))
         assert np.array_equal(one.view(np.uint8), two.view(np.uint8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [4, 8, 12, 16, 24, 32, 48, 56, 72, 88, 104, 120, 136, 144, 200])
+def test_few_rows_of_any_columns(dev, dtype, dim):
+    """head dims without a variant of their own, whose last products differ: contiguous and paged, walks of one and of several tiles and pieces"""
+    rng = np.random.default_rng(dim)
+    for keys in (1, 64, 65, 130, 700, 1500):
+        dense(dev, rng, dtype, 2, 4, 2, 1, keys, dim, cap=15.0)
+        dense(dev, rng, dtype, 1, 3, 1, 5, keys, dim, slopes=[0.5, 0.1, 0.01], causal=False)
+    dense(dev, rng, dtype, 1, 2, 1, 8, 300, dim, documents=[[0, 100, 293, 300]], prefix=[[3, 50, 1]])
+    paged(dev, rng, dtype, 4, 2, dim, 16, [700, 64, 65, 1], [1, 1, 1, 1], cap=15.0)
