@@ -388,10 +388,10 @@ __global__ void __launch_bounds__(AT_BLOCK) attention_few_kernel(AttnArgs a, Att
         at_join<T, true, AF_ROWS>(a, part, s, b, g, row0, 0, rows, first, stride, used, (float*)smem);
 }
 
-// One token to a sequence on average, and no more rows of a KV head than a tile's; tiles that LDS holds.  The host knows no more of the tokens than their number, so
-// one sequence may have most of them.  bf16, 32 heads on 8 of 128, cap and bias, us here | in tiles of 128 rows: 64 sequences of 2000 keys with a token each 100 | 117; of 64 one with 32
-// tokens and 8000 keys, 32 with one 92 | 100; of 64 one with 64 tokens and 8000 keys 84 | 179; of 40 one with 33 and 3000 keys, 7 with one 49 | 62; of 256 three with 64 tokens, 64 with
-// one 311 | 295; of 256 one with 256 and 8000 keys, whose 64 row tiles to a KV head all walk the keys, 261 | 184 (260 with loads that stay in the L2s).
+// One token to a sequence on average, and no more rows of a KV head than a tile's; tiles that LDS holds.  bf16, 32 heads on 8 of 128, cap and bias, us here | in tiles of 128 rows:
+// a token to each of 64 sequences of 300 keys 35 | 39, of 1500 82 | 96; of 256 91 | 104 and 275 | 324; of 512 200 | 225 and 570 | 664.  The host knows no more of the tokens than their
+// number, so one sequence may have them all, whose row tiles then walk the same keys: 64 tokens of 1000 keys 24 | 44, of 8000 85 | 178; 128 41 | 49 and 144 | 175; 256 71 | 66 and
+// 267 | 184 (260 with loads that stay in the L2s); 512 123 | 138 and 511 | 239.
 template <typename T> bool at_fits_few(const AttnArgs& a, bool paged) {
     return a.group <= AF_ROWS && (paged ? a.tokens <= a.seqs : (uint64_t)a.tokens * a.group <= AF_ROWS) && a.dim * sizeof(T) <= 512;
 }
